@@ -164,6 +164,20 @@ VS_API int vs_hnsw_import_graph(vs_hnsw* index, size_t slots, const void* vector
                          const uint64_t* keys, const uint32_t* adj0, const uint32_t* upper_off, const uint32_t* upper,
                          size_t upper_blocks, int32_t max_level, uint32_t entry_slot);
 
+/* -- the stored rows themselves, for work that reads them in place (include/vs_learn.h) --- */
+/* Slot numbers of members (their row numbers below), -1 for keys that are not members. */
+VS_API int vs_hnsw_slots(vs_hnsw* index, const uint64_t* keys, size_t n, int64_t* slots);
+/* Where the rows lie in HBM: slot s at d_rows + s * stride_bytes, `dimensions` elements of `quantization`, zero padded to the stride.
+ * Valid until the next add / remove / reserve. */
+typedef struct vs_hnsw_row_view {
+    const void* d_rows;
+    const float* d_inverse_norms; /* per slot, cosine indexes of float storage: 1 / |row|, 0 for the zero vector; else NULL */
+    const uint64_t* d_keys;       /* per slot; ~0: removed */
+    size_t slots, removed, dimensions, stride_bytes;
+    int metric, quantization, device;
+} vs_hnsw_row_view;
+VS_API int vs_hnsw_rows(vs_hnsw* index, vs_hnsw_row_view* view);
+
 /* -- multi-GPU: merge `parts` per-shard top-k lists (each nq x k, ascending, padded with
  * key ~0 / +inf) into one nq x k list.  Device buffers; parts are contiguous:
  * d_part_keys[p][q][k].  Follows the RCCL all-gather in the sharded search. ------------- */

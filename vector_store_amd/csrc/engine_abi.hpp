@@ -474,6 +474,39 @@ int vs_hnsw_export_graph(vs_hnsw* h, void* vectors, int32_t* levels, uint64_t* k
     });
 }
 
+int vs_hnsw_slots(vs_hnsw* h, const uint64_t* keys, size_t n, int64_t* slots) {
+    return guarded([&] {
+        need(h && (n == 0 || (keys && slots)), "null argument");
+        h->e.flush_pending();
+        std::lock_guard<std::mutex> g(h->e.mod_mu);
+        std::lock_guard<std::mutex> kg(h->e.key_mu);
+        for (size_t i = 0; i < n; ++i) {
+            const auto it = h->e.lookup.find(keys[i]);
+            slots[i] = it == h->e.lookup.end() ? -1 : (int64_t)it->second;
+        }
+    });
+}
+
+int vs_hnsw_rows(vs_hnsw* h, vs_hnsw_row_view* v) {
+    return guarded([&] {
+        need(h && v, "null argument");
+        Engine& e = h->e;
+        e.flush_pending();
+        std::lock_guard<std::mutex> g(e.mod_mu);
+        std::shared_lock<std::shared_mutex> vg(e.view_mu);
+        v->d_rows = e.d_vectors;
+        v->d_inverse_norms = e.metric == VS_METRIC_COS && e.scalar <= VS_SCALAR_BF16 ? e.d_aux : nullptr;
+        v->d_keys = e.d_keys;
+        v->slots = e.slots;
+        v->removed = e.removed.load();
+        v->dimensions = e.dim;
+        v->stride_bytes = (size_t)e.stride4 * 16;
+        v->metric = e.metric;
+        v->quantization = e.scalar;
+        v->device = e.device;
+    });
+}
+
 int vs_hnsw_import_graph(vs_hnsw* h, size_t n, const void* vectors, const int32_t* levels, const uint64_t* keys,
                          const uint32_t* adj0, const uint32_t* upper_off, const uint32_t* upper, size_t upper_blocks,
                          int32_t max_level, uint32_t entry_slot) {

@@ -1,0 +1,825 @@
+// learn.hip -- libvs_learn.so (include/vs_learn.h): the softmax loss of queries over all rows of a table or index and its gradients
+// (products on the matrix pipe, learn_product.hpp), rows read by number and their gradient.
+#include "../../include/vs_learn.h"
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+#include "learn_lookup.hpp"
+#include "learn_product.hpp"
+
+namespace vs {
+namespace learn {
+
+thread_local std::string g_err;
+struct Fail {
+    int code;
+    std::string msg;
+};
+[[noreturn]] static void fail(int code, std::string msg) { throw Fail{code, std::move(msg)}; }
+static void need(bool cond, const char* what) {
+    if (!cond) fail(VS_ERR_INVALID_ARGUMENT, what);
+}
+static void hip_ok(hipError_t e, const char* what) {
+    if (e != hipSuccess) fail(VS_ERR_DEVICE, std::string(what) + ": " + hipGetErrorString(e));
+}
+static void launched(const char* what) { hip_ok(hipGetLastError(), what); }
+
+// ------------------------------------------------------------------------------------------------ preparation kernels
+// Number formats.  Both sides bf16: the operands are used as they are (bf16 products are exact in f32).  Both sides f16, inner product: the
+// same on the f16 pipe.  Everything else (f32 anywhere, mixed types, f16 under cosine) is split into f16 planes, x = hi + lo with hi = f16(x),
+// lo = f16(x - hi): 22 bits of x.  Three of the four products of two such numbers are summed (lo lo is below 2^-22 of the result), which is
+// f32's accuracy at three times the f16 product's cost -- the matrix pipe's f32 product costs sixteen.  f16's narrow range is met by
+// powers of two: a query row, the rows of a piece of the table (inner product), or the normalised vector (cosine) is scaled so that its
+// largest element lies in [2^12, 2^13]; what is 2^-36 of the largest is lost.
+
+struct QueryPrep {
+    const void* q;
+    int scalar;
+    uint64_t ld;
+    uint32_t n, d, dp;
+    const void* labels;
+    uint32_t label_bytes;
+    uint32_t rows;                 // labels beyond are ignored
+    const uint64_t* keys;          // labels of removed members too
+    float scale;
+    uint32_t cosine, bf, raw;      // bf: bf16 operands; raw: planes hold the values themselves (bf16 or f16)
+    uint16_t* planes;              // nullptr: read in place
+    uint32_t nplanes;
+    uint64_t plane;
+    int32_t* label;
+    float* zf;
+    // backward (g != nullptr)
+    const float* g;
+    const float* lse;
+    float *lse2, *pf, *df, *inv;
+    int32_t *ge, *xe;
+};
+
+constexpr int32_t kNoExponent = -1000000;
+
+__device__ __forceinline__ int32_t exponent_of(float x) {  // x < 2^e (0, infinities and NaN: 0)
+    if (!(x > 0.f) || x == __builtin_inff()) return 0;
+    int e;
+    (void)frexpf(x, &e);
+    return e;
+}
+
+__device__ __forceinline__ void put_planes(uint16_t* to, uint64_t plane, uint32_t nplanes, bool bf, float x) {
+    if (bf) {
+        *to = to_half<true>(x);
+        return;
+    }
+    const uint16_t hi = to_half<false>(x);
+    *to = hi;
+    if (nplanes > 1) to[plane] = to_half<false>(x - from_half<false>(hi));
+}
+
+// one wave per query: its norm, largest element, factors, and its planes
+__global__ __launch_bounds__(256) void query_prep_kernel(QueryPrep a) {
+    const uint32_t lane = threadIdx.x & 63u, i = blockIdx.x * 4u + (threadIdx.x >> 6);
+    if (i >= a.n) return;
+    float ss = 0.f, top = 0.f;
+    if (a.cosine || !a.raw || a.g) {
+        for (uint32_t k = lane; k < a.d; k += 64) {
+            const float x = load_scalar(a.q, a.scalar, (uint64_t)i * a.ld + k);
+            ss = fmaf(x, x, ss);
+            top = fmaxf(top, fabsf(x));
+        }
+        ss = wave_sum(ss);
+        top = wave_max(top);
+    }
+    const float inv = !a.cosine ? 1.f : ss > 0.f ? 1.f / sqrtf(ss) : 0.f;
+    const int32_t e = a.raw || a.cosine ? 0 : exponent_of(top);
+    const float mul = a.raw ? 1.f : a.cosine ? inv * 8192.f : ldexpf(1.f, 13 - e);
+    if (a.planes) {
+        for (uint32_t k = lane; k < a.dp; k += 64) {
+            float x = k < a.d ? load_scalar(a.q, a.scalar, (uint64_t)i * a.ld + k) : 0.f;
+            if (!a.raw) x = a.cosine ? x * mul : ldexpf(x, 13 - e);
+            put_planes(a.planes + (uint64_t)i * a.dp + k, a.plane, a.nplanes, a.bf, x);
+        }
+    }
+    if (lane) return;
+    int64_t y = a.label_bytes == 8 ? reinterpret_cast<const int64_t*>(a.labels)[i] : reinterpret_cast<const int32_t*>(a.labels)[i];
+    if (y < 0 || y >= (int64_t)a.rows || (a.keys && a.keys[y] == ~0ull)) y = -1;
+    a.label[i] = (int32_t)y;
+    const float s2 = a.scale * kLog2e;
+    a.zf[i] = a.raw ? s2 * inv : a.cosine ? s2 * 0x1p-26f : ldexpf(s2, e - 13);
+    if (!a.g) return;
+    a.lse2[i] = a.lse[i] * kLog2e;
+    a.inv[i] = inv;
+    const float g = y >= 0 ? a.g[i] : 0.f;
+    if (a.bf) {
+        a.pf[i] = g * inv * a.scale;
+        a.df[i] = y >= 0 ? 1.f : 0.f;
+        a.ge[i] = 0;
+        a.xe[i] = 0;
+        return;
+    }
+    // f16 probabilities: (p - [label]) * m * 2^13 with g = m * 2^x, 1/2 <= |m| < 1: below 2^13, and full precision down to p = 2^-26
+    int x = 0;
+    const float m = frexpf(g, &x);
+    a.pf[i] = m * 8192.f;
+    a.df[i] = y >= 0 ? ldexpf(a.scale * (a.cosine ? inv * 0x1p-13f : 1.f), x - 13) : 0.f;
+    a.ge[i] = x;
+    a.xe[i] = y < 0 || !(g != 0.f) ? kNoExponent : x + exponent_of(a.cosine ? top * inv : top);
+}
+
+// The queries as an operand of dw = P^T q: rows of padding are zero whatever they held, and (f16) every row carries the power of two of its
+// loss gradient, relative to the largest.  out: [0] the factor that undoes it.
+struct GradQueries {
+    const void* q;
+    int scalar;
+    uint64_t ld;
+    uint32_t n, d, dp, cosine, bf, nplanes;
+    const int32_t *label, *ge, *xe;
+    const float* inv;
+    float scale;
+    uint16_t* planes;
+    uint64_t plane;
+    int32_t* top;  // [1]
+    float* wf;     // [1]
+};
+__global__ __launch_bounds__(1024) void grad_exponent_kernel(GradQueries a) {
+    __shared__ int32_t red[16];
+    int32_t top = kNoExponent;
+    for (uint32_t i = threadIdx.x; i < a.n; i += 1024) top = max(top, a.xe[i]);
+    for (int o = 32; o; o >>= 1) top = max(top, __shfl_xor(top, o));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int x = 1; x < 16; ++x) top = max(top, red[x]);
+        if (top == kNoExponent) top = 0;
+        a.top[0] = top;
+        a.wf[0] = ldexpf(a.scale, top - 26);
+    }
+}
+__global__ __launch_bounds__(256) void grad_queries_kernel(GradQueries a) {
+    const uint32_t lane = threadIdx.x & 63u, i = blockIdx.x * 4u + (threadIdx.x >> 6);
+    if (i >= a.n) return;
+    const bool on = a.label[i] >= 0 && a.xe[i] != kNoExponent;  // (padding, and queries whose loss nobody asks about)
+    const int32_t up = a.bf ? 0 : a.ge[i] - a.top[0] + 13;
+    const float inv = a.cosine && !a.bf ? a.inv[i] : 1.f;
+    for (uint32_t k = lane; k < a.dp; k += 64) {
+        float x = on && k < a.d ? load_scalar(a.q, a.scalar, (uint64_t)i * a.ld + k) : 0.f;
+        if (!a.bf) x = ldexpf(x * inv, up);
+        put_planes(a.planes + (uint64_t)i * a.dp + k, a.plane, a.nplanes, a.bf, x);
+    }
+}
+
+struct RowPrep {
+    const void* w;        // the piece's first row
+    int scalar;
+    uint64_t ld;
+    uint32_t rows, d, dp;
+    const uint64_t* keys;  // of the piece
+    uint32_t cosine, bf, raw, nplanes;
+    uint16_t* planes;
+    uint64_t plane;
+    uint32_t* top;   // bits of the largest |element| of the piece (inner product planes)
+    float* wsc;      // 2^(e - 13)
+    float* inv;      // 1 / |row|
+};
+__global__ __launch_bounds__(256) void rows_top_kernel(RowPrep a) {
+    const uint32_t lane = threadIdx.x & 63u;
+    float top = 0.f;
+    for (uint32_t j = blockIdx.x * 4u + (threadIdx.x >> 6); j < a.rows; j += gridDim.x * 4u) {
+        if (a.keys && a.keys[j] == ~0ull) continue;
+        for (uint32_t k = lane; k < a.d; k += 64) {
+            const float x = fabsf(load_scalar(a.w, a.scalar, (uint64_t)j * a.ld + k));
+            if (x < __builtin_inff()) top = fmaxf(top, x);
+        }
+    }
+    top = wave_max(top);
+    if (lane == 0 && top > 0.f) atomicMax(a.top, __float_as_uint(top));  // (a maximum: the same bits whatever the order)
+}
+// one wave per row of the piece
+__global__ __launch_bounds__(256) void rows_planes_kernel(RowPrep a) {
+    const uint32_t lane = threadIdx.x & 63u, j = blockIdx.x * 4u + (threadIdx.x >> 6);
+    const int32_t e = a.raw || a.cosine ? 0 : exponent_of(__uint_as_float(*a.top));
+    if (blockIdx.x == 0 && threadIdx.x == 0 && a.wsc) *a.wsc = a.raw || a.cosine ? 1.f : ldexpf(1.f, e - 13);
+    if (j >= a.rows) return;
+    const bool live = !(a.keys && a.keys[j] == ~0ull);
+    float inv = 1.f;
+    if (a.cosine && !a.raw) {
+        float ss = 0.f;
+        for (uint32_t k = lane; k < a.d; k += 64) {
+            const float x = load_scalar(a.w, a.scalar, (uint64_t)j * a.ld + k);
+            ss = fmaf(x, x, ss);
+        }
+        ss = wave_sum(ss);
+        inv = live && ss > 0.f ? 1.f / sqrtf(ss) : 0.f;
+        if (lane == 0) a.inv[j] = inv;
+    }
+    for (uint32_t k = lane; k < a.dp; k += 64) {
+        float x = live && k < a.d ? load_scalar(a.w, a.scalar, (uint64_t)j * a.ld + k) : 0.f;
+        if (!a.raw) x = a.cosine ? x * (inv * 8192.f) : ldexpf(x, 13 - e);
+        put_planes(a.planes + (uint64_t)j * a.dp + k, a.plane, a.nplanes, a.bf, x);
+    }
+}
+// 1 / |row| of a table whose rows are used as they are
+__global__ __launch_bounds__(256) void rows_inverse_norm_kernel(const void* w, int scalar, uint64_t ld, uint32_t rows, uint32_t d, float* inv) {
+    const uint32_t lane = threadIdx.x & 63u, j = blockIdx.x * 4u + (threadIdx.x >> 6);
+    if (j >= rows) return;
+    float ss = 0.f;
+    for (uint32_t k = lane; k < d; k += 64) {
+        const float x = load_scalar(w, scalar, (uint64_t)j * ld + k);
+        ss = fmaf(x, x, ss);
+    }
+    ss = wave_sum(ss);
+    if (lane == 0) inv[j] = ss > 0.f ? 1.f / sqrtf(ss) : 0.f;
+}
+__global__ void fill_words_kernel(uint32_t* p, uint32_t v, uint32_t n) {
+    const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x;
+    if (i < n) p[i] = v;
+}
+
+// ------------------------------------------------------------------------------------------------ joins
+__global__ __launch_bounds__(256) void loss_join_kernel(const float2* part, uint32_t part_ld, uint32_t n, const int32_t* label, const float* zlab,
+                                                        float* loss, float* lse) {
+    __shared__ float2 red[4];
+    const uint32_t i = blockIdx.x, lane = threadIdx.x & 63u;
+    float2 a = make_float2(-__builtin_inff(), 0.f);
+    for (uint32_t t = threadIdx.x; t < part_ld; t += 256) a = join_sums(a, part[(size_t)i * part_ld + t]);
+    for (int o = 1; o < 64; o <<= 1) a = join_sums(a, make_float2(__shfl_xor(a.x, o), __shfl_xor(a.y, o)));
+    if (lane == 0) red[threadIdx.x >> 6] = a;
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int x = 1; x < 4; ++x) a = join_sums(a, red[x]);
+    const float l2 = a.x + log2f(a.y);
+    lse[i] = l2 * kLn2;
+    loss[i] = label[i] >= 0 ? (l2 - zlab[i]) * kLn2 : 0.f;
+}
+
+// dq of one query: slices of k in order, pieces in order; after the last piece its factor, the way through the normalisation, the cast
+struct QueryJoin {
+    const float* part;   // [splits][n][dn]
+    uint32_t splits, n, d, dn;
+    const float* wsc;
+    float* acc;          // [n][dn]
+    uint32_t first, last, cosine;
+    const float *df, *inv;
+    const void* q;
+    int scalar;
+    uint64_t ld;
+    void* out;
+    uint64_t out_ld;
+};
+__global__ __launch_bounds__(256) void query_join_kernel(QueryJoin a) {
+    __shared__ float red[4];
+    const uint32_t i = blockIdx.x;
+    const float wsc = a.wsc ? *a.wsc : 1.f, df = a.last ? a.df[i] : 1.f, inv = a.last && a.cosine ? a.inv[i] : 0.f;
+    float dot = 0.f;
+    for (uint32_t k = threadIdx.x; k < a.d; k += 256) {
+        float s = 0.f;
+        for (uint32_t x = 0; x < a.splits; ++x) s += a.part[((size_t)x * a.n + i) * a.dn + k];
+        s *= wsc;
+        if (!a.first) s += a.acc[(size_t)i * a.dn + k];
+        if (a.last && !a.cosine) {
+            store_scalar(a.out, a.scalar, (uint64_t)i * a.out_ld + k, df == 0.f ? 0.f : s * df);
+            continue;
+        }
+        if (a.last) {
+            s *= df;
+            dot = fmaf(s, load_scalar(a.q, a.scalar, (uint64_t)i * a.ld + k) * inv, dot);
+        }
+        a.acc[(size_t)i * a.dn + k] = s;
+    }
+    if (!a.last || !a.cosine) return;
+    dot = wave_sum(dot);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = dot;
+    __syncthreads();
+    dot = (red[0] + red[1]) + (red[2] + red[3]);
+    for (uint32_t k = threadIdx.x; k < a.d; k += 256)  // (each thread reads what it wrote itself)
+        store_scalar(a.out, a.scalar, (uint64_t)i * a.out_ld + k,
+                     df == 0.f ? 0.f : a.acc[(size_t)i * a.dn + k] - load_scalar(a.q, a.scalar, (uint64_t)i * a.ld + k) * inv * dot);
+}
+// cosine: what dw_j has along w_j / |w_j|: sum over queries of g c z, / |w_j|
+__global__ __launch_bounds__(256) void row_along_kernel(const float* tpart, uint32_t parts, uint32_t n, const float* inv, float* coef) {
+    const uint32_t j = blockIdx.x * 256u + threadIdx.x;
+    if (j >= n) return;
+    float s = 0.f;
+    for (uint32_t x = 0; x < parts; ++x) s += tpart[(size_t)x * n + j];
+    coef[j] = s * kLn2 * inv[j];
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+template <class S, int FORM, int EPI, bool BF>
+static void run_product(const ProductArgs& g, hipStream_t st) {
+    static const hipError_t allowed =
+        hipFuncSetAttribute(reinterpret_cast<const void*>(&product_kernel<S, FORM, EPI, BF>), hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS);
+    hip_ok(allowed, "shared memory of the product");
+    const uint64_t tiles = (uint64_t)g.tiles_m * g.tiles_n * g.splits;
+    if (tiles >= (1ull << 31)) fail(VS_ERR_UNSUPPORTED, "too many tiles");
+    constexpr uint32_t resident = 256u * (S::LDS > 80 * 1024 ? 1u : 3u);
+    hipLaunchKernelGGL((product_kernel<S, FORM, EPI, BF>), dim3((uint32_t)std::min<uint64_t>(tiles, resident)), dim3(S::NW * 64), S::LDS, st, g);
+    launched("product");
+}
+template <int FORM, int EPI>
+static void product(ProductArgs g, bool large, bool bf, hipStream_t st) {
+    const uint32_t tm = large ? Large::TM : Small::TM, tn = large ? Large::TN : Small::TN;
+    g.tiles_m = (g.m + tm - 1) / tm;
+    g.tiles_n = (g.n + tn - 1) / tn;
+    if (large) {
+        if (bf) run_product<Large, FORM, EPI, true>(g, st);
+        else run_product<Large, FORM, EPI, false>(g, st);
+    } else {
+        if (bf) run_product<Small, FORM, EPI, true>(g, st);
+        else run_product<Small, FORM, EPI, false>(g, st);
+    }
+}
+// The large tile where it fills the chip: it reads an operand byte per 256 outputs where the small one reads it per 64 / 128.
+static bool use_large(uint64_t m, uint64_t n) { return m > 64 && ((m + 255) / 256) * ((n + 255) / 256) >= 192; }
+
+struct Rows {  // vs_rows resolved
+    const char* data = nullptr;
+    int scalar = 0;
+    size_t rows = 0, dim = 0, ld = 0;  // ld in elements
+    const uint64_t* keys = nullptr;    // only where members were removed
+    const float* inv = nullptr;
+    int metric = -1, device = -1;
+};
+static size_t size_of(int scalar) { return scalar == VS_SCALAR_F32 ? 4 : 2; }
+static void need_scalar(int scalar, const char* what) {
+    if (scalar != VS_SCALAR_F32 && scalar != VS_SCALAR_F16 && scalar != VS_SCALAR_BF16) fail(VS_ERR_UNSUPPORTED, std::string(what) + ": f32, f16 or bf16");
+}
+static Rows resolve(const vs_rows* r) {
+    need(r, "null rows");
+    Rows o;
+    if (r->index) {
+        vs_hnsw_row_view v;
+        const int rc = vs_hnsw_rows(r->index, &v);
+        if (rc != VS_OK) fail(rc, vs_hnsw_last_error());
+        need_scalar(v.quantization, "rows of an index");
+        o.data = (const char*)v.d_rows;
+        o.scalar = v.quantization;
+        o.rows = v.slots;
+        o.dim = v.dimensions;
+        o.ld = v.stride_bytes / size_of(v.quantization);
+        o.keys = v.removed ? v.d_keys : nullptr;
+        o.inv = v.d_inverse_norms;
+        o.metric = v.metric;
+        o.device = v.device;
+    } else {
+        need_scalar(r->scalar, "rows");
+        need(r->rows == 0 || r->d_data, "null rows");
+        need(r->stride >= r->dim, "rows: stride below the dimension");
+        o.data = (const char*)r->d_data;
+        o.scalar = r->scalar;
+        o.rows = r->rows;
+        o.dim = r->dim;
+        o.ld = r->stride;
+    }
+    need(o.dim > 0, "dimension must be > 0");
+    if (o.rows >= (1ull << 31) || o.dim > (1u << 16) || o.ld > (1u << 20)) fail(VS_ERR_UNSUPPORTED, "rows: below 2^31 of them, up to 65,536 elements, strides up to 2^20");
+    return o;
+}
+// The index's device is current for the duration of a call.
+struct OnDevice {
+    int before = -1;
+    explicit OnDevice(int device) {
+        if (device < 0) return;
+        hip_ok(hipGetDevice(&before), "device");
+        if (before == device) before = -1;
+        else hip_ok(hipSetDevice(device), "device");
+    }
+    ~OnDevice() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+struct Layout {  // offsets into the caller's scratch
+    size_t at = 0;
+    size_t take(size_t bytes) {
+        const size_t r = at;
+        at += (bytes + 255) & ~(size_t)255;
+        return r;
+    }
+};
+
+// What a loss call does, from sizes, types, alignment and what is asked of it.
+struct Plan {
+    Rows w;
+    uint32_t n = 0, v = 0, d = 0, dp = 0;
+    bool cosine = false, bf = false, raw = false, q_in_place = false, w_in_place = false, inv_own = false;
+    bool grad_q = false, grad_w = false;
+    uint32_t nq = 1, nw = 1, np = 1, nqg = 1;  // planes of the queries, the rows, the probabilities, the queries of dw
+    uint32_t piece = 0, pieces = 0;
+    bool large_s = false, large_q = false, large_w = false;
+    uint32_t splits = 1, qsteps = 1, tiles_v = 0, trows = 0;
+    size_t o_label, o_zf, o_qplanes, o_top, o_wsc, o_inv, o_wplanes, o_part, o_zlab;
+    size_t o_lse2, o_pf, o_df, o_qinv, o_ge, o_xe, o_exp, o_gplanes, o_prob, o_tpart, o_coef, o_qpart, o_qacc;
+    size_t bytes = 0;
+};
+
+constexpr size_t kPieceBytes = 256ull << 20;    // re-laid rows and probabilities of one piece: what the last-level cache holds
+constexpr size_t kSplitBytes = 128ull << 20;    // f32 slices of dq
+
+static Plan plan(const vs_rows* rows, const vs_softmax* q, bool grad_q, bool grad_w) {
+    Plan p;
+    p.w = resolve(rows);
+    need(q, "null queries");
+    need_scalar(q->scalar, "queries");
+    need(q->n == 0 || (q->d_queries && q->d_labels), "null queries or labels");
+    need(q->label_bytes == 4 || q->label_bytes == 8, "labels: 4 or 8 bytes");
+    need(q->stride >= p.w.dim, "queries: stride below the dimension");
+    need(q->metric == VS_METRIC_IP || q->metric == VS_METRIC_COS, "a loss needs the inner product or the cosine");
+    need(p.w.metric < 0 || p.w.metric == q->metric, "the loss's metric is not the index's");
+    need(std::isfinite(q->scale), "scale must be finite");
+    if (q->n > (1u << 20) || q->stride > (1u << 20)) fail(VS_ERR_UNSUPPORTED, "queries: up to 2^20 of them, strides up to 2^20");
+    const uint32_t n = p.n = (uint32_t)q->n, v = p.v = (uint32_t)p.w.rows, d = p.d = (uint32_t)p.w.dim;
+    p.dp = (d + 63u) & ~63u;
+    p.cosine = q->metric == VS_METRIC_COS;
+    const int tq = q->scalar, tw = p.w.scalar;
+    p.bf = tq == VS_SCALAR_BF16 && tw == VS_SCALAR_BF16;
+    p.raw = p.bf || (tq == VS_SCALAR_F16 && tw == VS_SCALAR_F16 && !p.cosine);
+    p.q_in_place = p.raw && d % 8 == 0 && q->stride % 8 == 0 && (uintptr_t)q->d_queries % 16 == 0;
+    p.w_in_place = p.raw && !p.w.keys && d % 8 == 0 && p.w.ld % 8 == 0 && (uintptr_t)p.w.data % 16 == 0;
+    p.inv_own = p.cosine && !(p.raw && p.w.inv);
+    p.nq = !p.raw && (p.cosine || tq == VS_SCALAR_F32) ? 2 : 1;
+    p.nw = !p.raw && (p.cosine || tw == VS_SCALAR_F32) ? 2 : 1;
+    p.grad_q = grad_q;
+    p.grad_w = grad_w;
+    const bool grad = grad_q || grad_w;
+    p.np = (grad_q && tq == VS_SCALAR_F32) || (grad_w && tw == VS_SCALAR_F32) ? 2 : 1;
+    p.nqg = !p.bf && tw == VS_SCALAR_F32 && p.nq > 1 ? 2 : 1;
+    // pieces of the table: one, unless rows are re-laid or probabilities are kept for the two products that read them
+    const size_t per_row = (p.w_in_place ? 0 : (size_t)p.nw * p.dp * 2) + (grad ? (size_t)p.np * n * 2 : 0);
+    size_t piece = v;
+    if (per_row) piece = std::min<size_t>(v, std::max<size_t>(2048, kPieceBytes / per_row));
+    piece = std::min<size_t>(piece, 1u << 20);
+    if (piece) {
+        const size_t pieces = (v + piece - 1) / piece;
+        piece = ((v + pieces - 1) / pieces + 255) / 256 * 256;
+        p.pieces = (uint32_t)((v + piece - 1) / piece);
+    }
+    p.piece = (uint32_t)piece;
+    p.large_s = use_large(n, piece);
+    p.large_w = use_large(piece, d);
+    p.large_q = n > 64 && d > 128;
+    const uint32_t tm = p.large_q ? 256 : 64, tn = p.large_q ? 256 : 128;
+    const size_t qtiles = (size_t)((n + tm - 1) / tm) * ((d + tn - 1) / tn);
+    const size_t dn = (d + 3u) & ~3u;
+    const uint32_t ksteps = (uint32_t)std::max<size_t>(1, (piece + 63) / 64);
+    if (grad_q && n) {
+        size_t s = std::max<size_t>(1, (p.large_q ? 256 : 768) / qtiles);
+        s = std::min<size_t>(s, std::max<size_t>(1, kSplitBytes / (n * dn * 4)));
+        s = std::min<size_t>(s, std::max<uint32_t>(1, ksteps / 4));
+        p.qsteps = (uint32_t)((ksteps + s - 1) / s);
+        p.splits = (ksteps + p.qsteps - 1) / p.qsteps;
+    }
+    const uint32_t stn = p.large_s ? Large::TN : Small::TN, stm = p.large_s ? Large::TM : Small::TM;
+    p.tiles_v = p.pieces ? (p.pieces - 1) * (p.piece / stn) + (uint32_t)((v - (size_t)(p.pieces - 1) * p.piece + stn - 1) / stn) : 0;
+    p.trows = (n + stm - 1) / stm * 2;  // (both shapes have two wave rows)
+    Layout l;
+    p.o_label = l.take((size_t)n * 4);
+    p.o_zf = l.take((size_t)n * 4);
+    p.o_qplanes = l.take(p.q_in_place ? 0 : (size_t)p.nq * n * p.dp * 2);
+    p.o_top = l.take((size_t)p.pieces * 4);
+    p.o_wsc = l.take((size_t)p.pieces * 4);
+    p.o_inv = l.take(p.inv_own ? (size_t)v * 4 : 0);
+    p.o_wplanes = l.take(p.w_in_place ? 0 : (size_t)p.nw * piece * p.dp * 2);
+    if (!grad) {
+        p.o_part = l.take((size_t)n * p.tiles_v * 8);
+        p.o_zlab = l.take((size_t)n * 4);
+    } else {
+        p.o_lse2 = l.take((size_t)n * 4);
+        p.o_pf = l.take((size_t)n * 4);
+        p.o_df = l.take((size_t)n * 4);
+        p.o_qinv = l.take((size_t)n * 4);
+        p.o_ge = l.take((size_t)n * 4);
+        p.o_xe = l.take((size_t)n * 4);
+        p.o_exp = l.take(8);
+        p.o_gplanes = l.take(grad_w ? (size_t)p.nqg * n * p.dp * 2 : 0);
+        p.o_prob = l.take((size_t)p.np * n * (((size_t)piece + 7) & ~(size_t)7) * 2);
+        p.o_tpart = l.take(grad_w && p.cosine ? (size_t)p.trows * piece * 4 : 0);
+        p.o_coef = l.take(grad_w && p.cosine ? (size_t)piece * 4 : 0);
+        p.o_qpart = l.take(grad_q ? (size_t)p.splits * n * dn * 4 : 0);
+        p.o_qacc = l.take(grad_q && (p.pieces > 1 || p.cosine) ? (size_t)n * dn * 4 : 0);
+    }
+    p.bytes = l.at;
+    return p;
+}
+
+static void plane_pairs(ProductArgs& g, uint32_t na, uint32_t nb, bool all) {
+    // (hi hi, lo hi, hi lo) of what there is; one product only where the result is 16 bits wide
+    g.segs = 1;
+    g.seg_a = g.seg_b = 0;
+    if (!all) return;
+    if (na > 1) g.seg_a |= 1u << (4 * g.segs++);
+    if (nb > 1) g.seg_b |= 1u << (4 * g.segs++);
+}
+
+struct Call {  // what the two calls share
+    const Plan& p;
+    const vs_softmax& q;
+    char* work;
+    hipStream_t st;
+    template <class T>
+    T* at(size_t o) const { return reinterpret_cast<T*>(work + o); }
+
+    void queries(const float* lse, const float* g) const {
+        QueryPrep a = {};
+        a.q = q.d_queries;
+        a.scalar = q.scalar;
+        a.ld = q.stride;
+        a.n = p.n, a.d = p.d, a.dp = p.dp;
+        a.labels = q.d_labels;
+        a.label_bytes = (uint32_t)q.label_bytes;
+        a.rows = p.v;
+        a.keys = p.w.keys;
+        a.scale = q.scale;
+        a.cosine = p.cosine, a.bf = p.bf, a.raw = p.raw;
+        a.planes = p.q_in_place ? nullptr : at<uint16_t>(p.o_qplanes);
+        a.nplanes = p.nq;
+        a.plane = (uint64_t)p.n * p.dp;
+        a.label = at<int32_t>(p.o_label);
+        a.zf = at<float>(p.o_zf);
+        if (g) {
+            a.g = g;
+            a.lse = lse;
+            a.lse2 = at<float>(p.o_lse2), a.pf = at<float>(p.o_pf), a.df = at<float>(p.o_df), a.inv = at<float>(p.o_qinv);
+            a.ge = at<int32_t>(p.o_ge), a.xe = at<int32_t>(p.o_xe);
+        }
+        hipLaunchKernelGGL(query_prep_kernel, dim3((p.n + 3) / 4), dim3(256), 0, st, a);
+        launched("queries");
+    }
+    void tables() const {  // once per call, before the pieces
+        if (!p.raw && !p.cosine) {
+            hipLaunchKernelGGL(fill_words_kernel, dim3((p.pieces + 255) / 256), dim3(256), 0, st, at<uint32_t>(p.o_top), 0u, p.pieces);
+            launched("fill");
+        }
+        if (p.raw && p.inv_own) {
+            hipLaunchKernelGGL(rows_inverse_norm_kernel, dim3((p.v + 3) / 4), dim3(256), 0, st, p.w.data, p.w.scalar, (uint64_t)p.w.ld, p.v, p.d,
+                               at<float>(p.o_inv));
+            launched("norms");
+        }
+    }
+    const float* h() const { return !p.cosine || !p.raw ? nullptr : p.w.inv ? p.w.inv : at<float>(p.o_inv); }       // score factor of a column
+    const float* inv() const { return p.raw && p.w.inv ? p.w.inv : at<float>(p.o_inv); }
+    // the piece's rows as an operand
+    Operand rows(uint32_t x, uint32_t first, uint32_t count) const {
+        const char* data = p.w.data + (size_t)first * p.w.ld * size_of(p.w.scalar);
+        if (p.w_in_place) return Operand{data, 0, p.w.ld * 2, count, p.d};
+        RowPrep a = {};
+        a.w = data;
+        a.scalar = p.w.scalar;
+        a.ld = p.w.ld;
+        a.rows = count, a.d = p.d, a.dp = p.dp;
+        a.keys = p.w.keys ? p.w.keys + first : nullptr;
+        a.cosine = p.cosine, a.bf = p.bf, a.raw = p.raw, a.nplanes = p.nw;
+        a.planes = at<uint16_t>(p.o_wplanes);
+        a.plane = (uint64_t)p.piece * p.dp;
+        a.top = at<uint32_t>(p.o_top) + x;
+        a.wsc = at<float>(p.o_wsc) + x;
+        a.inv = p.cosine && !p.raw ? at<float>(p.o_inv) + first : nullptr;
+        if (!p.raw && !p.cosine) {
+            hipLaunchKernelGGL(rows_top_kernel, dim3(std::min<uint32_t>(2048, (count + 3) / 4)), dim3(256), 0, st, a);
+            launched("rows");
+        }
+        hipLaunchKernelGGL(rows_planes_kernel, dim3((count + 3) / 4), dim3(256), 0, st, a);
+        launched("rows");
+        return Operand{(const char*)a.planes, a.plane * 2, (uint64_t)p.dp * 2, count, p.dp};
+    }
+    // scores of all queries against a piece: operands and factors
+    ProductArgs scores(const Operand& w, uint32_t x, uint32_t first, uint32_t count) const {
+        ProductArgs g = {};
+        g.a = p.q_in_place ? Operand{(const char*)q.d_queries, 0, q.stride * 2, p.n, p.d}
+                           : Operand{at<char>(p.o_qplanes), (uint64_t)p.n * p.dp * 2, (uint64_t)p.dp * 2, p.n, p.dp};
+        g.b = w;
+        g.m = p.n, g.n = count;
+        g.k = std::min(g.a.cols, g.b.cols);  // (a re-laid operand's padding is zero)
+        g.splits = 1;
+        g.ksteps = (g.k + 63) / 64;
+        plane_pairs(g, p.nq, p.nw, true);
+        g.zf = at<float>(p.o_zf);
+        g.h = h() ? h() + first : nullptr;
+        g.wsc = p.raw || p.cosine ? nullptr : at<float>(p.o_wsc) + x;
+        g.keys = p.w.keys ? p.w.keys + first : nullptr;
+        g.label = at<int32_t>(p.o_label);
+        g.col0 = first;
+        return g;
+    }
+};
+
+static void need_work(const Plan& p, const void* work, size_t bytes) {
+    need(bytes >= p.bytes && (p.bytes == 0 || work), "d_work is smaller than the call needs");
+    need((uintptr_t)work % 256 == 0, "d_work must be 256-byte aligned");
+}
+
+static void loss(const vs_rows* rows, const vs_softmax* q, float* d_loss, float* d_lse, void* work, size_t work_bytes, hipStream_t st) {
+    const Plan p = plan(rows, q, false, false);
+    if (!p.n) return;
+    need(d_loss && d_lse, "null outputs");
+    need_work(p, work, work_bytes);
+    OnDevice dev(p.w.device);
+    const Call c{p, *q, (char*)work, st};
+    c.queries(nullptr, nullptr);
+    if (p.v) c.tables();
+    uint32_t tile = 0;
+    for (uint32_t x = 0; x < p.pieces; ++x) {
+        const uint32_t first = x * p.piece, count = std::min(p.piece, p.v - first);
+        const Operand w = c.rows(x, first, count);
+        ProductArgs g = c.scores(w, x, first, count);
+        g.part = c.at<float2>(p.o_part);
+        g.part_ld = p.tiles_v;
+        g.part0 = tile;
+        g.zlab = c.at<float>(p.o_zlab);
+        product<SCORES, EPI_LOSS>(g, p.large_s, p.bf, st);
+        const uint32_t tn = p.large_s ? Large::TN : Small::TN;
+        tile += (count + tn - 1) / tn;
+    }
+    hipLaunchKernelGGL(loss_join_kernel, dim3(p.n), dim3(256), 0, st, c.at<float2>(p.o_part), p.tiles_v, p.n, c.at<int32_t>(p.o_label),
+                       c.at<float>(p.o_zlab), d_loss, d_lse);
+    launched("join");
+}
+
+static void loss_grad(const vs_rows* rows, const vs_softmax* q, const float* d_lse, const float* d_g, void* d_gq, size_t gq_ld, void* d_gw, size_t gw_ld,
+                      void* work, size_t work_bytes, hipStream_t st) {
+    const Plan p = plan(rows, q, d_gq != nullptr, d_gw != nullptr);
+    if (!d_gq && !d_gw) return;
+    need(!d_gq || gq_ld >= p.d, "gradient of the queries: stride below the dimension");
+    need(!d_gw || gw_ld >= p.d, "gradient of the rows: stride below the dimension");
+    need(p.n == 0 || (d_lse && d_g), "null lse or gradient of the loss");
+    need_work(p, work, work_bytes);
+    OnDevice dev(p.w.device);
+    if (!p.n || !p.v) {  // nothing to learn from: the gradients there are are zero
+        if (d_gq && p.n) launch_zero_rows(d_gq, q->scalar, gq_ld, p.n, p.d, st);
+        if (d_gw && p.v) launch_zero_rows(d_gw, p.w.scalar, gw_ld, p.v, p.d, st);
+        launched("zero");
+        return;
+    }
+    const Call c{p, *q, (char*)work, st};
+    c.queries(d_lse, d_g);
+    c.tables();
+    Operand gq = {};
+    if (d_gw) {
+        GradQueries a = {};
+        a.q = q->d_queries;
+        a.scalar = q->scalar;
+        a.ld = q->stride;
+        a.n = p.n, a.d = p.d, a.dp = p.dp, a.cosine = p.cosine, a.bf = p.bf, a.nplanes = p.nqg;
+        a.label = c.at<int32_t>(p.o_label), a.ge = c.at<int32_t>(p.o_ge), a.xe = c.at<int32_t>(p.o_xe);
+        a.inv = c.at<float>(p.o_qinv);
+        a.scale = q->scale;
+        a.planes = c.at<uint16_t>(p.o_gplanes);
+        a.plane = (uint64_t)p.n * p.dp;
+        a.top = c.at<int32_t>(p.o_exp);
+        a.wf = c.at<float>(p.o_exp) + 1;
+        if (!p.bf) hipLaunchKernelGGL(grad_exponent_kernel, dim3(1), dim3(1024), 0, st, a);
+        hipLaunchKernelGGL(grad_queries_kernel, dim3((p.n + 3) / 4), dim3(256), 0, st, a);
+        launched("queries");
+        gq = Operand{(const char*)a.planes, a.plane * 2, (uint64_t)p.dp * 2, p.n, p.dp};
+    }
+    const uint32_t dn = (p.d + 3u) & ~3u;
+    for (uint32_t x = 0; x < p.pieces; ++x) {
+        const uint32_t first = x * p.piece, count = std::min(p.piece, p.v - first);
+        const Operand w = c.rows(x, first, count);
+        ProductArgs g = c.scores(w, x, first, count);
+        g.lse2 = c.at<float>(p.o_lse2);
+        g.pf = c.at<float>(p.o_pf);
+        g.prob = c.at<uint16_t>(p.o_prob);
+        g.prob_ld = (count + 7u) & ~7u;
+        g.prob_plane = (uint64_t)p.n * g.prob_ld;
+        g.prob_planes = p.np;
+        g.tpart = d_gw && p.cosine ? c.at<float>(p.o_tpart) : nullptr;
+        g.graw = d_g;
+        product<SCORES, EPI_PROB>(g, p.large_s, p.bf, st);
+        const Operand prob{(const char*)g.prob, g.prob_plane * 2, (uint64_t)g.prob_ld * 2, p.n, g.prob_ld};
+        if (d_gq) {
+            ProductArgs b = {};
+            b.a = prob;
+            b.b = w;
+            b.m = p.n, b.n = dn, b.k = count;
+            b.splits = p.splits;
+            b.ksteps = p.qsteps;
+            plane_pairs(b, p.np, p.nw, q->scalar == VS_SCALAR_F32);
+            b.out_part = c.at<float>(p.o_qpart);
+            product<DQ, EPI_PART>(b, p.large_q, p.bf, st);
+            QueryJoin j = {};
+            j.part = b.out_part;
+            j.splits = p.splits, j.n = p.n, j.d = p.d, j.dn = dn;
+            j.wsc = p.raw || p.cosine ? nullptr : c.at<float>(p.o_wsc) + x;
+            j.acc = c.at<float>(p.o_qacc);
+            j.first = x == 0, j.last = x + 1 == p.pieces, j.cosine = p.cosine;
+            j.df = c.at<float>(p.o_df), j.inv = c.at<float>(p.o_qinv);
+            j.q = q->d_queries, j.scalar = q->scalar, j.ld = q->stride;
+            j.out = d_gq, j.out_ld = gq_ld;
+            hipLaunchKernelGGL(query_join_kernel, dim3(p.n), dim3(256), 0, st, j);
+            launched("join");
+        }
+        if (d_gw) {
+            if (p.cosine) {
+                const uint32_t stm = p.large_s ? Large::TM : Small::TM;
+                hipLaunchKernelGGL(row_along_kernel, dim3((count + 255) / 256), dim3(256), 0, st, g.tpart, (p.n + stm - 1) / stm * 2, count, c.inv() + first,
+                                   c.at<float>(p.o_coef));
+                launched("rows");
+            }
+            ProductArgs b = {};
+            b.a = prob;
+            b.b = gq;
+            b.m = count, b.n = p.d, b.k = p.n;
+            b.splits = 1;
+            b.ksteps = (p.n + 63) / 64;
+            plane_pairs(b, p.np, p.nqg, p.w.scalar == VS_SCALAR_F32);
+            b.out = (char*)d_gw + (size_t)first * gw_ld * size_of(p.w.scalar);
+            b.out_scalar = p.w.scalar;
+            b.out_ld = gw_ld;
+            b.wf = p.bf ? nullptr : c.at<float>(p.o_exp) + 1;
+            b.rf = p.cosine && !p.raw ? c.inv() + first : nullptr;
+            b.tcoef = p.cosine ? c.at<float>(p.o_coef) : nullptr;
+            b.tinv = p.cosine ? c.inv() + first : nullptr;
+            b.raw = p.w.data + (size_t)first * p.w.ld * size_of(p.w.scalar);
+            b.raw_scalar = p.w.scalar;
+            b.raw_ld = p.w.ld;
+            product<DW, EPI_ROWS>(b, p.large_w, p.bf, st);
+        }
+    }
+}
+
+template <class F>
+static int guarded(F&& f) {
+    try {
+        f();
+        return VS_OK;
+    } catch (const Fail& x) {
+        g_err = x.msg;
+        return x.code;
+    } catch (const std::exception& x) {
+        g_err = x.what();
+        return VS_ERR_DEVICE;
+    } catch (...) {
+        g_err = "unknown error";
+        return VS_ERR_DEVICE;
+    }
+}
+
+}  // namespace learn
+}  // namespace vs
+
+using namespace vs::learn;
+
+extern "C" {
+
+const char* vs_learn_last_error(void) { return g_err.c_str(); }
+
+int vs_lookup_device(const vs_rows* rows, const void* d_ids, size_t id_bytes, size_t n, float scale, void* d_out, int out_scalar, size_t out_stride, void* stream) {
+    return guarded([&] {
+        const Rows r = resolve(rows);
+        need_scalar(out_scalar, "output");
+        need(id_bytes == 4 || id_bytes == 8, "ids: 4 or 8 bytes");
+        need(out_stride >= r.dim, "output: stride below the dimension");
+        if (!n) return;
+        need(d_ids && d_out, "null ids or output");
+        if (n >= (1ull << 31)) fail(VS_ERR_UNSUPPORTED, "below 2^31 ids");
+        OnDevice dev(r.device);
+        launch_lookup(r.data, r.scalar, r.ld, (uint32_t)r.rows, (uint32_t)r.dim, r.keys, d_ids, (uint32_t)id_bytes, (uint32_t)n, scale, d_out, out_scalar, out_stride,
+                      (hipStream_t)stream);
+        launched("lookup");
+    });
+}
+
+size_t vs_lookup_grad_work(size_t n, size_t rows, size_t dim) { return lookup_grad_layout(n, rows, dim).bytes; }
+
+int vs_lookup_grad_device(const void* d_grad, int grad_scalar, size_t grad_stride, const void* d_ids, size_t id_bytes, size_t n, size_t rows, size_t dim, float scale,
+                          int accumulate, void* d_out, int out_scalar, size_t out_stride, void* d_work, size_t work_bytes, void* stream) {
+    return guarded([&] {
+        need_scalar(grad_scalar, "gradient");
+        need_scalar(out_scalar, "output");
+        need(id_bytes == 4 || id_bytes == 8, "ids: 4 or 8 bytes");
+        need(dim > 0 && grad_stride >= dim && out_stride >= dim, "a stride is below the dimension");
+        if (!rows) return;
+        need(d_out, "null output");
+        need(n == 0 || (d_grad && d_ids), "null gradient or ids");
+        if (n >= (1ull << 30) || rows >= (1ull << 31) - 1 || dim > (1u << 16)) fail(VS_ERR_UNSUPPORTED, "below 2^30 ids, 2^31 rows, up to 65,536 elements");
+        const LookupGradLayout l = lookup_grad_layout(n, rows, dim);
+        need(work_bytes >= l.bytes && (l.bytes == 0 || d_work), "d_work is smaller than the call needs");
+        need((uintptr_t)d_work % 256 == 0, "d_work must be 256-byte aligned");
+        launch_lookup_grad(d_grad, grad_scalar, grad_stride, d_ids, (uint32_t)id_bytes, (uint32_t)n, (uint32_t)rows, (uint32_t)dim, scale, accumulate != 0, d_out, out_scalar,
+                           out_stride, l, (char*)d_work, (hipStream_t)stream);
+        launched("lookup gradient");
+    });
+}
+
+size_t vs_softmax_loss_work(const vs_rows* rows, const vs_softmax* q) {
+    size_t bytes = 0;
+    return guarded([&] { bytes = plan(rows, q, false, false).bytes; }) == VS_OK ? bytes : 0;
+}
+int vs_softmax_loss_device(const vs_rows* rows, const vs_softmax* q, float* d_loss, float* d_lse, void* d_work, size_t work_bytes, void* stream) {
+    return guarded([&] { loss(rows, q, d_loss, d_lse, d_work, work_bytes, (hipStream_t)stream); });
+}
+size_t vs_softmax_loss_grad_work(const vs_rows* rows, const vs_softmax* q, int queries, int table) {
+    size_t bytes = 0;
+    return guarded([&] { bytes = plan(rows, q, queries != 0, table != 0).bytes; }) == VS_OK ? bytes : 0;
+}
+int vs_softmax_loss_grad_device(const vs_rows* rows, const vs_softmax* q, const float* d_lse, const float* d_grad_loss, void* d_grad_queries,
+                                size_t grad_queries_stride, void* d_grad_rows, size_t grad_rows_stride, void* d_work, size_t work_bytes, void* stream) {
+    return guarded([&] {
+        loss_grad(rows, q, d_lse, d_grad_loss, d_grad_queries, grad_queries_stride, d_grad_rows, grad_rows_stride, d_work, work_bytes, (hipStream_t)stream);
+    });
+}
+
+}  // extern "C"

@@ -1,0 +1,411 @@
+// learn_product.hpp -- the tiled matrix product behind the softmax loss (learn.hip): C = sum over plane pairs of A B, 16-bit operands, f32
+// accumulation on the matrix pipe, with the loss's own epilogues.
+//
+//   SCORES  A [m x k] rows, B [n x k] rows      z = q w^T          both operands lie along k
+//   DQ      A [m x k] rows, B [k x n] rows      dq = P w           B lies across k
+//   DW      A [k x m] rows, B [k x n] rows      dw = P^T q         both lie across k
+//
+// A workgroup owns TM x TN outputs and walks k in steps of 64 through a ring of two LDS stages that the load units fill by themselves
+// (buffer_load ... lds, 16 bytes per lane: no register round trip).  The buffer descriptors carry the operands' true bounds, so rows, columns
+// and k beyond the end arrive as zeros and no operand has to be padded.  LDS images:
+//   along k:   [row][64 k], 128 bytes per row, 16-byte chunks XOR-swizzled by the row (conflict-free ds_read_b128 fragments);
+//   across k:  [64 k][columns], 32-byte units XOR-swizzled by k; the fragments come through ds_read_b64_tr_b16, which hands each lane four
+//              consecutive k of one column: no transposed copy of P, the queries or the table is ever written.
+// The swizzles are applied to the SOURCE address of the load (the LDS side of such a load is linear).
+// The operands of the MFMA are swapped (B first): a lane then holds four consecutive COLUMNS of one output row, so row-wise softmax sums are
+// mostly in-lane and stores are 8 / 16 bytes wide.
+// Persistent over the output tiles: the ring runs on into the next tile while the epilogue works.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "learn_device.hpp"
+
+namespace vs {
+namespace learn {
+
+enum : int { SCORES = 0, DQ = 1, DW = 2 };
+enum : int { EPI_LOSS = 0, EPI_PROB = 1, EPI_PART = 2, EPI_ROWS = 3 };
+
+struct Operand {
+    const char* p;
+    uint64_t plane;   // bytes between planes
+    uint64_t ld;      // bytes between stored rows
+    uint32_t rows;    // stored rows
+    uint32_t cols;    // valid elements of a stored row (a multiple of 8)
+};
+
+struct ProductArgs {
+    Operand a, b;
+    uint32_t m, n, k;            // outputs and depth
+    uint32_t tiles_m, tiles_n;
+    uint32_t splits, ksteps;     // slices of k and 64-deep steps per slice
+    uint32_t segs;               // plane pairs
+    uint32_t seg_a, seg_b;       // 4 bits each: the planes of pair s
+    // EPI_LOSS / EPI_PROB: z2 = acc * zf[row] * wsc * h[col] (base-2 exponent units)
+    const float* zf;
+    const float* h;              // nullptr: 1
+    const float* wsc;            // nullptr: 1
+    const uint64_t* keys;        // nullptr, or per column: ~0 = not a member
+    const int32_t* label;        // per row: column of the whole table, -1 = ignored
+    uint32_t col0;               // first column of this piece
+    // EPI_LOSS
+    float2* part;                // [m][part_ld] (maximum, sum of 2^(z2 - maximum)) per column tile
+    uint32_t part_ld, part0;
+    float* zlab;                 // z2 at the label
+    // EPI_PROB: P = (2^(z2 - lse2) - [label]) * pf[row] * h[col]
+    const float* lse2;
+    const float* pf;
+    uint16_t* prob;
+    uint64_t prob_plane;         // elements
+    uint32_t prob_ld, prob_planes;
+    float* tpart;                // nullptr, or [row halves of tiles][n]: sums over rows of c z (cosine)
+    const float* graw;           // dloss per row for tpart
+    // EPI_PART
+    float* out_part;             // [splits][m][n]
+    // EPI_ROWS
+    void* out;
+    int out_scalar;
+    uint64_t out_ld;             // elements
+    const float* wf;             // nullptr: 1
+    const float* rf;             // nullptr: 1; per output row
+    const float* tcoef;          // nullptr, or per output row: minus tcoef * (tinv * raw row)
+    const float* tinv;
+    const void* raw;
+    int raw_scalar;
+    uint64_t raw_ld;
+};
+
+constexpr int kBK = 64;
+
+__device__ __forceinline__ uint32_t swz_row(uint32_t row) { return (row >> 1) & 7u; }
+template <int COLS>
+__device__ __forceinline__ uint32_t swz_k(uint32_t k) {
+    return ((k & 3u) | (((k >> 3) & 1u) << 2)) & (COLS / 16 - 1u);
+}
+
+// One operand's stage: 64 deep, X output rows / columns wide (X * 128 bytes of LDS), brought in by NW waves in pieces of 1 KiB.
+template <int X, int NW, bool ACROSS>
+struct Loader {
+    static constexpr int PIECES = X / 8 / NW;
+    static_assert(X % (8 * NW) == 0, "whole pieces per wave");
+    uint32_t off[PIECES];
+    __device__ __forceinline__ void init(uint64_t ld, uint32_t w, uint32_t lane) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const uint32_t at = (w * PIECES + i) * 1024u + lane * 16u;
+            if constexpr (ACROSS) {
+                const uint32_t kr = at / (X * 2), cp = (at % (X * 2)) >> 4;
+                const uint32_t c = ((((cp >> 1) ^ swz_k<X>(kr)) << 1) | (cp & 1u));
+                off[i] = kr * (uint32_t)ld + c * 16u;
+            } else {
+                const uint32_t row = at >> 7, cp = (at >> 4) & 7u;
+                off[i] = row * (uint32_t)ld + ((cp ^ swz_row(row)) << 4);
+            }
+        }
+    }
+    // x0: first output row / column of the tile; k0: first k of the step; kend: end of k (a multiple of 8 along k)
+    __device__ __forceinline__ void stage(const Operand& o, uint32_t plane, uint32_t x0, uint32_t k0, uint32_t kend, char* lds, uint32_t w, uint32_t lane) const {
+        const char* base;
+        uint64_t bytes = 0;
+        if constexpr (ACROSS) {
+            base = o.p + plane * o.plane + (uint64_t)k0 * o.ld + (uint64_t)x0 * 2u;
+            if (k0 < kend && x0 < o.cols) {
+                const uint32_t left = kend - k0 < (uint32_t)kBK ? kend - k0 : (uint32_t)kBK;
+                bytes = (uint64_t)(left - 1u) * o.ld + (uint64_t)(o.cols - x0) * 2u;
+            }
+        } else {
+            base = o.p + plane * o.plane + (uint64_t)x0 * o.ld + (uint64_t)k0 * 2u;
+            if (k0 < kend && x0 < o.rows) bytes = (uint64_t)(o.rows - x0) * o.ld - (uint64_t)k0 * 2u;
+        }
+        const uint32_t limit = bytes > 0x7FFFF000ull ? 0x7FFFF000u : (uint32_t)bytes;
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)limit, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            uint32_t v = off[i];
+            if constexpr (!ACROSS) {
+                if (k0 + kBK > kend) {  // the last step of a depth that is no multiple of 64: chunks beyond it read nothing
+                    const uint32_t row = (w * PIECES + i) * 8u + (lane >> 3);
+                    const uint32_t kc = ((lane & 7u) ^ swz_row(row)) * 8u;
+                    if (k0 + kc >= kend) v = 0x7FFFFFF0u;
+                }
+            }
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(lds + (w * PIECES + i) * 1024u), 16, v, 0, 0, 0);
+        }
+    }
+};
+
+// Fragment of 16 output rows / columns x 32 k (eight k per lane: k = kk * 32 + 8 * (lane / 16) + 0..7).
+template <int X, bool ACROSS, class Frag>
+__device__ __forceinline__ Frag read_fragment(const char* lds, uint32_t x, uint32_t kk, uint32_t lane) {
+    if constexpr (ACROSS) {
+        using s4 = __attribute__((ext_vector_type(4))) short;
+        using s8 = __attribute__((ext_vector_type(8))) short;
+        const uint32_t i = lane & 15u, k = kk * 32u + (lane >> 4) * 8u + (i >> 2);
+        const uint32_t u = x >> 4;
+        const auto at = [&](uint32_t kr) {
+            return (__attribute__((address_space(3))) s4*)(lds + kr * (X * 2u) + ((u ^ swz_k<X>(kr)) << 5) + (i & 3u) * 8u);
+        };
+        const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(k));
+        const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(k + 4u));
+        const s8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        return __builtin_bit_cast(Frag, v);
+    } else {
+        const uint32_t row = x + (lane & 15u), kc = kk * 4u + (lane >> 4);
+        return *reinterpret_cast<const Frag*>(lds + row * 128u + ((kc ^ swz_row(row)) << 4));
+    }
+}
+
+template <bool BF16>
+struct Half {
+    using frag = __attribute__((ext_vector_type(8))) _Float16;
+    static __device__ __forceinline__ f32x4 mma(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Half<true> {
+    using frag = __attribute__((ext_vector_type(8))) __bf16;
+    static __device__ __forceinline__ f32x4 mma(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+
+// WM x WN waves, each MT x NT blocks of 16 x 16.
+template <int TM_, int TN_, int WM_, int WN_>
+struct Shape {
+    static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, NW = WM_ * WN_;
+    static constexpr int MT = TM_ / WM_ / 16, NT = TN_ / WN_ / 16;
+    static constexpr int A_BYTES = TM_ * 128, B_BYTES = TN_ * 128, STAGE = A_BYTES + B_BYTES;
+    static constexpr int EPI_BYTES = WN_ * TM_ * 8;  // EPI_LOSS: (maximum, sum) per wave column and row
+    static constexpr int LDS = 2 * STAGE + EPI_BYTES;
+};
+using Large = Shape<256, 256, 2, 4>;   // one workgroup per CU, 136 KiB of LDS
+using Small = Shape<64, 128, 2, 2>;    // 50 KiB: three workgroups per CU
+
+template <class S, int FORM, int EPI, bool BF16>
+__global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
+    constexpr bool A_ACROSS = FORM == DW, B_ACROSS = FORM != SCORES;
+    using H = Half<BF16>;
+    using frag = typename H::frag;
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    const uint32_t lane = threadIdx.x & 63u, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = w / S::WN, wn = w % S::WN;
+    const uint32_t per_split = g.tiles_m * g.tiles_n, tiles = per_split * g.splits;
+    if (blockIdx.x >= tiles) return;
+    // blocks b, b + 8, b + 16 ... share an XCD and its L2: they take the row tiles of the same column tile one after the other
+    const auto place = [&](uint32_t t, uint32_t& tm, uint32_t& tn, uint32_t& sp) {
+        sp = t / per_split;
+        const uint32_t r = t - sp * per_split;
+        const uint32_t group = r / (8u * g.tiles_m), in = r - group * 8u * g.tiles_m;
+        const uint32_t left = g.tiles_n - group * 8u, width = left < 8u ? left : 8u;
+        tm = in / width;
+        tn = group * 8u + in % width;
+    };
+    Loader<S::TM, S::NW, A_ACROSS> la;
+    Loader<S::TN, S::NW, B_ACROSS> lb;
+    la.init(g.a.ld, w, lane);
+    lb.init(g.b.ld, w, lane);
+    const uint32_t steps = g.ksteps * g.segs;
+    const uint32_t my_tiles = (tiles - 1u - blockIdx.x) / gridDim.x + 1u;
+    const uint32_t total = my_tiles * steps;
+    uint32_t p = 0, p_tile = blockIdx.x, p_seg = 0, p_ks = 0, p_tm, p_tn, p_sp;
+    place(p_tile, p_tm, p_tn, p_sp);
+    const auto prefetch = [&]() {
+        char* st = lds + (p & 1u) * S::STAGE;
+        const uint32_t k0 = (p_sp * g.ksteps + p_ks) * kBK;
+        la.stage(g.a, (g.seg_a >> (4u * p_seg)) & 15u, p_tm * S::TM, k0, g.k, st, w, lane);
+        lb.stage(g.b, (g.seg_b >> (4u * p_seg)) & 15u, p_tn * S::TN, k0, g.k, st + S::A_BYTES, w, lane);
+        ++p;
+        if (++p_ks == g.ksteps) {
+            p_ks = 0;
+            if (++p_seg == g.segs) {
+                p_seg = 0;
+                p_tile += gridDim.x;
+                if (p_tile < tiles) place(p_tile, p_tm, p_tn, p_sp);
+            }
+        }
+    };
+    prefetch();
+    uint32_t at = 0;
+    for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        uint32_t tm, tn, sp;
+        place(tile, tm, tn, sp);
+        f32x4 acc[S::MT][S::NT];
+#pragma unroll
+        for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+            for (int j = 0; j < S::NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (uint32_t s = 0; s < steps; ++s, ++at) {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();  // stage `at` is whole; nobody reads stage at - 1 any more
+            asm volatile("" ::: "memory");
+            if (p < total) prefetch();
+            const char* sa = lds + (at & 1u) * S::STAGE;
+            const char* sb = sa + S::A_BYTES;
+#pragma unroll
+            for (uint32_t kk = 0; kk < kBK / 32; ++kk) {
+                frag fa[S::MT], fb[S::NT];
+#pragma unroll
+                for (int i = 0; i < S::MT; ++i) fa[i] = read_fragment<S::TM, A_ACROSS, frag>(sa, (wm * S::MT + i) * 16u, kk, lane);
+#pragma unroll
+                for (int j = 0; j < S::NT; ++j) fb[j] = read_fragment<S::TN, B_ACROSS, frag>(sb, (wn * S::NT + j) * 16u, kk, lane);
+#pragma unroll
+                for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < S::NT; ++j) acc[i][j] = H::mma(fb[j], fa[i], acc[i][j]);
+            }
+        }
+        // lane: row (lane & 15) of a 16 x 16 block, columns 4 * (lane / 16) + 0..3
+        const uint32_t row0 = tm * S::TM + wm * S::MT * 16u + (lane & 15u);
+        const uint32_t cl = tn * S::TN + wn * S::NT * 16u + (lane >> 4) * 4u;
+        if constexpr (EPI == EPI_LOSS || EPI == EPI_PROB) {
+            const float wsc = g.wsc ? *g.wsc : 1.f;
+            f32x4 h[S::NT];
+            uint32_t live[S::NT];  // bit r: column j, r exists
+#pragma unroll
+            for (int j = 0; j < S::NT; ++j) {
+                live[j] = 0;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const uint32_t c = cl + j * 16u + r;
+                    const bool in = c < g.n && !(g.keys && g.keys[c] == ~0ull);
+                    live[j] |= in ? 1u << r : 0u;
+                    h[j][r] = in ? (g.h ? g.h[c] * wsc : wsc) : 0.f;
+                }
+            }
+            if constexpr (EPI == EPI_LOSS) {
+                float2* red = reinterpret_cast<float2*>(lds + 2 * S::STAGE);
+#pragma unroll
+                for (int i = 0; i < S::MT; ++i) {
+                    const uint32_t row = row0 + i * 16u;
+                    const bool has = row < g.m;
+                    const float f = has ? g.zf[row] : 0.f;
+                    const int32_t lab = has ? g.label[row] - (int32_t)g.col0 : -1;
+                    float top = -__builtin_inff();
+#pragma unroll
+                    for (int j = 0; j < S::NT; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const float z = (live[j] >> r) & 1u ? acc[i][j][r] * (f * h[j][r]) : -__builtin_inff();
+                            acc[i][j][r] = z;
+                            if ((int32_t)(cl + j * 16u + r) == lab) g.zlab[row] = z;
+                            top = fmaxf(top, z);
+                        }
+                    top = fmaxf(top, __shfl_xor(top, 16));
+                    top = fmaxf(top, __shfl_xor(top, 32));
+                    float sum = 0.f;
+                    const float base = top == -__builtin_inff() ? 0.f : top;
+#pragma unroll
+                    for (int j = 0; j < S::NT; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) sum += exp2_fast(acc[i][j][r] - base);
+                    sum += __shfl_xor(sum, 16);
+                    sum += __shfl_xor(sum, 32);
+                    if (lane < 16) red[wn * S::TM + (wm * S::MT + i) * 16u + lane] = make_float2(top, sum);
+                }
+                __syncthreads();
+                for (uint32_t t = threadIdx.x; t < (uint32_t)S::TM; t += S::NW * 64) {
+                    const uint32_t row = tm * S::TM + t;
+                    if (row < g.m) {
+                        float2 a = red[t];
+#pragma unroll
+                        for (int x = 1; x < S::WN; ++x) a = join_sums(a, red[x * S::TM + t]);
+                        g.part[(size_t)row * g.part_ld + g.part0 + tn] = a;
+                    }
+                }
+                // (the next tile's writes to `red` come after its first step's barrier: these reads are done by then)
+            } else {
+                float ts[S::NT][4];
+                if (g.tpart) {
+#pragma unroll
+                    for (int j = 0; j < S::NT; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) ts[j][r] = 0.f;
+                }
+#pragma unroll
+                for (int i = 0; i < S::MT; ++i) {
+                    const uint32_t row = row0 + i * 16u;
+                    const bool has = row < g.m;
+                    const float f = has ? g.zf[row] : 0.f, l2 = has ? g.lse2[row] : 0.f, pf = has ? g.pf[row] : 0.f;
+                    const int32_t lab = has ? g.label[row] : -1;
+                    const bool on = lab >= 0;
+                    const float gr = g.tpart && on ? g.graw[row] : 0.f;
+#pragma unroll
+                    for (int j = 0; j < S::NT; ++j) {
+                        float v[4];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const uint32_t c = cl + j * 16u + r;
+                            const float z = acc[i][j][r] * (f * h[j][r]);
+                            float q = exp2_fast(z - l2);
+                            if ((int32_t)(c + g.col0) == lab) q -= 1.f;
+                            const bool in = on && ((live[j] >> r) & 1u);
+                            if (g.tpart) ts[j][r] += in ? q * z * gr : 0.f;
+                            v[r] = in ? q * pf * (g.h ? h[j][r] : 1.f) : 0.f;
+                        }
+                        const uint32_t c = cl + j * 16u;
+                        if (has && c < g.prob_ld) {  // (prob_ld: n rounded up to 8, so a lane's four columns are in or out together)
+                            uint16_t* to = g.prob + (uint64_t)row * g.prob_ld + c;
+                            ushort4 hi;
+                            hi.x = to_half<BF16>(v[0]), hi.y = to_half<BF16>(v[1]), hi.z = to_half<BF16>(v[2]), hi.w = to_half<BF16>(v[3]);
+                            *reinterpret_cast<ushort4*>(to) = hi;
+                            if (g.prob_planes > 1) {
+                                ushort4 lo;
+                                lo.x = to_half<BF16>(v[0] - from_half<BF16>(hi.x)), lo.y = to_half<BF16>(v[1] - from_half<BF16>(hi.y));
+                                lo.z = to_half<BF16>(v[2] - from_half<BF16>(hi.z)), lo.w = to_half<BF16>(v[3] - from_half<BF16>(hi.w));
+                                *reinterpret_cast<ushort4*>(to + g.prob_plane) = lo;
+                            }
+                        }
+                    }
+                }
+                if (g.tpart) {
+#pragma unroll
+                    for (int j = 0; j < S::NT; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            float t = ts[j][r];
+                            t += __shfl_xor(t, 1);
+                            t += __shfl_xor(t, 2);
+                            t += __shfl_xor(t, 4);
+                            t += __shfl_xor(t, 8);
+                            const uint32_t c = cl + j * 16u + r;
+                            if ((lane & 15u) == 0 && c < g.n) g.tpart[(size_t)(tm * S::WM + wm) * g.n + c] = t;
+                        }
+                }
+            }
+        } else if constexpr (EPI == EPI_PART) {
+            float* to = g.out_part + (size_t)sp * g.m * g.n;
+#pragma unroll
+            for (int i = 0; i < S::MT; ++i) {
+                const uint32_t row = row0 + i * 16u;
+#pragma unroll
+                for (int j = 0; j < S::NT; ++j) {
+                    const uint32_t c = cl + j * 16u;
+                    if (row < g.m && c < g.n) *reinterpret_cast<f32x4*>(to + (size_t)row * g.n + c) = acc[i][j];  // (n: a multiple of 4)
+                }
+            }
+        } else {
+            const float wf = g.wf ? *g.wf : 1.f;
+#pragma unroll
+            for (int i = 0; i < S::MT; ++i) {
+                const uint32_t row = row0 + i * 16u;
+                if (row < g.m) {
+                    const float rf = g.rf ? g.rf[row] * wf : wf;
+                    const float tc = g.tcoef ? g.tcoef[row] : 0.f, ti = g.tcoef ? g.tinv[row] : 0.f;
+#pragma unroll
+                    for (int j = 0; j < S::NT; ++j) {
+                        const uint32_t c = cl + j * 16u;
+                        if (c < g.n) {
+                            f32x4 v = acc[i][j] * rf;
+                            if (tc != 0.f) {
+#pragma unroll
+                                for (int r = 0; r < 4; ++r)
+                                    if (c + r < g.n) v[r] -= tc * (load_scalar(g.raw, g.raw_scalar, (uint64_t)row * g.raw_ld + c + r) * ti);
+                            }
+                            store4(g.out, g.out_scalar, (uint64_t)row * g.out_ld + c, v, g.n - c);
+                        }
+                    }
+                }
+            }
+        }
+    }
+}
+
+}  // namespace learn
+}  // namespace vs

@@ -45,6 +45,11 @@ class _GraphInfo(C.Structure):
                 ("entry_slot", C.c_uint32), ("connectivity", C.c_size_t), ("connectivity_base", C.c_size_t)]
 
 
+class _RowView(C.Structure):
+    _fields_ = [("d_rows", C.c_void_p), ("d_inverse_norms", C.c_void_p), ("d_keys", C.c_void_p), ("slots", C.c_size_t), ("removed", C.c_size_t),
+                ("dimensions", C.c_size_t), ("stride_bytes", C.c_size_t), ("metric", C.c_int), ("quantization", C.c_int), ("device", C.c_int)]
+
+
 def lib_path() -> str:
     # VS_HNSW_LIB: an instrumented build of the engine alone; VS_LIB_DIR: a directory with instrumented builds of every library (development)
     return os.environ.get("VS_HNSW_LIB") or os.path.join(os.environ.get("VS_LIB_DIR") or _HERE, "libvs_hnsw.so")
@@ -117,6 +122,9 @@ def lib():
     L.vs_hnsw_graph_info_get.argtypes = [vp, C.POINTER(_GraphInfo)]
     L.vs_hnsw_export_graph.argtypes = [vp, vp, vp, vp, vp, vp, vp]
     L.vs_hnsw_import_graph.argtypes = [vp, sz, vp, vp, vp, vp, vp, vp, sz, C.c_int32, C.c_uint32]
+    if hasattr(L, "vs_hnsw_rows"):
+        L.vs_hnsw_rows.argtypes = [vp, C.POINTER(_RowView)]
+        L.vs_hnsw_slots.argtypes = [vp, vp, sz, vp]
     L.vs_topk_merge_device.argtypes = [vp, vp, sz, sz, sz, vp, vp, vp, vp]
     L.vs_topk_merge_packed_device.argtypes = [vp, sz, sz, sz, sz, vp, vp, vp, vp]
     L.vs_f32_to_b1x8.argtypes = [vp, sz, vp]
@@ -396,6 +404,19 @@ class HipUsearchIndex:
         gi = _GraphInfo()
         _check(self.L.vs_hnsw_graph_info_get(self.h, C.byref(gi)))
         return {f[0]: getattr(gi, f[0]) for f in _GraphInfo._fields_}
+
+    def slots(self, primary_ids) -> np.ndarray:
+        """Slot numbers of members (-1: not a member): what `learn` calls number an index's rows by."""
+        keys = np.ascontiguousarray(primary_ids, dtype=np.uint64)
+        out = np.full(keys.shape, -1, dtype=np.int64)
+        _check(self.L.vs_hnsw_slots(self.h, _p(keys), keys.size, _p(out)))
+        return out
+
+    def rows(self) -> dict:
+        """Where the stored rows lie in HBM (include/vs_hnsw.h: vs_hnsw_rows); valid until the next add / remove / reserve."""
+        v = _RowView()
+        _check(self.L.vs_hnsw_rows(self.h, C.byref(v)))
+        return {f[0]: getattr(v, f[0]) for f in _RowView._fields_}
 
     def export_graph(self, vectors_out=None) -> dict:
         gi = self.graph_info()
