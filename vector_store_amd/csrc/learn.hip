@@ -193,8 +193,12 @@ __global__ __launch_bounds__(256) void rows_top_kernel(RowPrep a) {
             if (x < __builtin_inff()) top = fmaxf(top, x);
         }
     }
+    __shared__ float red[4];
     top = wave_max(top);
-    if (lane == 0 && top > 0.f) atomicMax(a.top, __float_as_uint(top));  // (a maximum: the same bits whatever the order)
+    if (lane == 0) red[threadIdx.x >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    if (threadIdx.x == 0 && top > 0.f) atomicMax(a.top, __float_as_uint(top));  // (a maximum: the same bits whatever the order)
 }
 // one wave per row of the piece
 __global__ __launch_bounds__(256) void rows_planes_kernel(RowPrep a) {
@@ -314,7 +318,7 @@ static void run_product(const ProductArgs& g, hipStream_t st) {
     hip_ok(allowed, "shared memory of the product");
     const uint64_t tiles = (uint64_t)g.tiles_m * g.tiles_n * g.splits;
     if (tiles >= (1ull << 31)) fail(VS_ERR_UNSUPPORTED, "too many tiles");
-    constexpr uint32_t resident = 256u * (S::LDS > 80 * 1024 ? 1u : 3u);
+    constexpr uint32_t resident = 256u * (160u * 1024u / S::LDS);
     hipLaunchKernelGGL((product_kernel<S, FORM, EPI, BF>), dim3((uint32_t)std::min<uint64_t>(tiles, resident)), dim3(S::NW * 64), S::LDS, st, g);
     launched("product");
 }
@@ -465,7 +469,7 @@ static Plan plan(const vs_rows* rows, const vs_softmax* q, bool grad_q, bool gra
     const size_t dn = (d + 3u) & ~3u;
     const uint32_t ksteps = (uint32_t)std::max<size_t>(1, (piece + 63) / 64);
     if (grad_q && n) {
-        size_t s = std::max<size_t>(1, (p.large_q ? 256 : 768) / qtiles);
+        size_t s = std::max<size_t>(1, (p.large_q ? 256 : 512) / qtiles);
         s = std::min<size_t>(s, std::max<size_t>(1, kSplitBytes / (n * dn * 4)));
         s = std::min<size_t>(s, std::max<uint32_t>(1, ksteps / 4));
         p.qsteps = (uint32_t)((ksteps + s - 1) / s);
@@ -577,7 +581,7 @@ struct Call {  // what the two calls share
         a.wsc = at<float>(p.o_wsc) + x;
         a.inv = p.cosine && !p.raw ? at<float>(p.o_inv) + first : nullptr;
         if (!p.raw && !p.cosine) {
-            hipLaunchKernelGGL(rows_top_kernel, dim3(std::min<uint32_t>(2048, (count + 3) / 4)), dim3(256), 0, st, a);
+            hipLaunchKernelGGL(rows_top_kernel, dim3(std::min<uint32_t>(512, (count + 3) / 4)), dim3(256), 0, st, a);
             launched("rows");
         }
         hipLaunchKernelGGL(rows_planes_kernel, dim3((count + 3) / 4), dim3(256), 0, st, a);
@@ -687,7 +691,8 @@ static void loss_grad(const vs_rows* rows, const vs_softmax* q, const float* d_l
         g.prob_planes = p.np;
         g.tpart = d_gw && p.cosine ? c.at<float>(p.o_tpart) : nullptr;
         g.graw = d_g;
-        product<SCORES, EPI_PROB>(g, p.large_s, p.bf, st);
+        if (g.tpart) product<SCORES, EPI_PROB_ALONG>(g, p.large_s, p.bf, st);
+        else product<SCORES, EPI_PROB>(g, p.large_s, p.bf, st);
         const Operand prob{(const char*)g.prob, g.prob_plane * 2, (uint64_t)g.prob_ld * 2, p.n, g.prob_ld};
         if (d_gq) {
             ProductArgs b = {};

@@ -38,6 +38,12 @@ __device__ __forceinline__ void store_scalar(void* p, int scalar, uint64_t i, fl
     if (scalar == SC_F32) reinterpret_cast<float*>(p)[i] = v;
     else reinterpret_cast<uint16_t*>(p)[i] = scalar == SC_F16 ? to_half<false>(v) : to_half<true>(v);
 }
+__device__ __forceinline__ ushort4 to_half4(int scalar, f32x4 v) {
+    ushort4 o;
+    if (scalar == SC_F16) o.x = to_half<false>(v[0]), o.y = to_half<false>(v[1]), o.z = to_half<false>(v[2]), o.w = to_half<false>(v[3]);
+    else o.x = to_half<true>(v[0]), o.y = to_half<true>(v[1]), o.z = to_half<true>(v[2]), o.w = to_half<true>(v[3]);
+    return o;
+}
 // up to four consecutive elements (`left` of them exist), one wide store where the address allows it
 __device__ __forceinline__ void store4(void* p, int scalar, uint64_t i, f32x4 v, uint32_t left) {
     if (scalar == SC_F32) {
@@ -49,10 +55,7 @@ __device__ __forceinline__ void store4(void* p, int scalar, uint64_t i, f32x4 v,
     } else {
         uint16_t* to = reinterpret_cast<uint16_t*>(p) + i;
         if (left >= 4 && ((uintptr_t)to & 7u) == 0) {
-            ushort4 o;
-            if (scalar == SC_F16) o.x = to_half<false>(v[0]), o.y = to_half<false>(v[1]), o.z = to_half<false>(v[2]), o.w = to_half<false>(v[3]);
-            else o.x = to_half<true>(v[0]), o.y = to_half<true>(v[1]), o.z = to_half<true>(v[2]), o.w = to_half<true>(v[3]);
-            *reinterpret_cast<ushort4*>(to) = o;
+            *reinterpret_cast<ushort4*>(to) = to_half4(scalar, v);
             return;
         }
     }

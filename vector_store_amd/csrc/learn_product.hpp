@@ -25,7 +25,7 @@ namespace vs {
 namespace learn {
 
 enum : int { SCORES = 0, DQ = 1, DW = 2 };
-enum : int { EPI_LOSS = 0, EPI_PROB = 1, EPI_PART = 2, EPI_ROWS = 3 };
+enum : int { EPI_LOSS = 0, EPI_PROB = 1, EPI_PART = 2, EPI_ROWS = 3, EPI_PROB_ALONG = 4 };  // (.._ALONG: cosine, with the sums of c z per column)
 
 struct Operand {
     const char* p;
@@ -59,8 +59,8 @@ struct ProductArgs {
     uint16_t* prob;
     uint64_t prob_plane;         // elements
     uint32_t prob_ld, prob_planes;
-    float* tpart;                // nullptr, or [row halves of tiles][n]: sums over rows of c z (cosine)
-    const float* graw;           // dloss per row for tpart
+    float* tpart;                // EPI_PROB_ALONG: [wave rows of tiles][n]: sums over rows of dloss c z
+    const float* graw;           // dloss per row
     // EPI_PART
     float* out_part;             // [splits][m][n]
     // EPI_ROWS
@@ -135,24 +135,74 @@ struct Loader {
     }
 };
 
-// Fragment of 16 output rows / columns x 32 k (eight k per lane: k = kk * 32 + 8 * (lane / 16) + 0..7).
-template <int X, bool ACROSS, class Frag>
+// Fragment of 16 output rows / columns x 32 k (eight k per lane: k = kk * 32 + 8 * (lane / 16) + 0..7), operand along k.
+template <class Frag>
 __device__ __forceinline__ Frag read_fragment(const char* lds, uint32_t x, uint32_t kk, uint32_t lane) {
+    const uint32_t row = x + (lane & 15u), kc = kk * 4u + (lane >> 4);
+    return *reinterpret_cast<const Frag*>(lds + row * 128u + ((kc ^ swz_row(row)) << 4));
+}
+// The same, operand across k: two transposing reads per fragment.  Lane i of 16 names 8 bytes of k row (i / 4), columns 4 * (i % 4), and gets
+// column i of four k.  swz_k is the same for every kk and for both halves of a fragment, so one address per fragment and immediate offsets do.
+// Written out, with their wait in the same block: behind the builtin the compiler waits for the LDS loads in flight (the next stage's).
+template <int X>
+__device__ __forceinline__ uint32_t across_address(uint32_t x, uint32_t lane) {
+    const uint32_t i = lane & 15u, k = (lane >> 4) * 8u + (i >> 2);
+    return k * (X * 2u) + (((x >> 4) ^ swz_k<X>(k)) << 5) + (i & 3u) * 8u;
+}
+using s16x4 = __attribute__((ext_vector_type(4))) short;
+using s16x8 = __attribute__((ext_vector_type(8))) short;
+template <int X, int KK>
+__device__ __forceinline__ void read_across4(const uint32_t* a, s16x8* f) {
+    s16x4 l0, h0, l1, h1, l2, h2, l3, h3;
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(l0), "=&v"(h0), "=&v"(l1), "=&v"(h1), "=&v"(l2), "=&v"(h2), "=&v"(l3), "=&v"(h3)
+        : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(KK * 64 * X), "n"(KK * 64 * X + 8 * X)
+        : "memory");
+    f[0] = __builtin_shufflevector(l0, h0, 0, 1, 2, 3, 4, 5, 6, 7);
+    f[1] = __builtin_shufflevector(l1, h1, 0, 1, 2, 3, 4, 5, 6, 7);
+    f[2] = __builtin_shufflevector(l2, h2, 0, 1, 2, 3, 4, 5, 6, 7);
+    f[3] = __builtin_shufflevector(l3, h3, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+template <int X, int KK>
+__device__ __forceinline__ void read_across2(const uint32_t* a, s16x8* f) {
+    s16x4 l0, h0, l1, h1;
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %4 offset:%6\n\tds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
+        "ds_read_b64_tr_b16 %2, %5 offset:%6\n\tds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(l0), "=&v"(h0), "=&v"(l1), "=&v"(h1)
+        : "v"(a[0]), "v"(a[1]), "n"(KK * 64 * X), "n"(KK * 64 * X + 8 * X)
+        : "memory");
+    f[0] = __builtin_shufflevector(l0, h0, 0, 1, 2, 3, 4, 5, 6, 7);
+    f[1] = __builtin_shufflevector(l1, h1, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+// T fragments of one operand; at: LDS byte address of its stage
+template <int X, int T, bool ACROSS, int KK, class Frag>
+__device__ __forceinline__ void read_fragments(const char* lds, uint32_t at, uint32_t x, uint32_t lane, const uint32_t* addr, Frag* f) {
     if constexpr (ACROSS) {
-        using s4 = __attribute__((ext_vector_type(4))) short;
-        using s8 = __attribute__((ext_vector_type(8))) short;
-        const uint32_t i = lane & 15u, k = kk * 32u + (lane >> 4) * 8u + (i >> 2);
-        const uint32_t u = x >> 4;
-        const auto at = [&](uint32_t kr) {
-            return (__attribute__((address_space(3))) s4*)(lds + kr * (X * 2u) + ((u ^ swz_k<X>(kr)) << 5) + (i & 3u) * 8u);
-        };
-        const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(k));
-        const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(k + 4u));
-        const s8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        return __builtin_bit_cast(Frag, v);
+        uint32_t a[T];
+        s16x8 v[T];
+#pragma unroll
+        for (int i = 0; i < T; ++i) a[i] = addr[i] + at;
+        if constexpr (T == 8) {
+            read_across4<X, KK>(a, v);
+            read_across4<X, KK>(a + 4, v + 4);
+        } else if constexpr (T == 4) {
+            read_across4<X, KK>(a, v);
+        } else {
+            static_assert(T == 2, "fragments per wave");
+            read_across2<X, KK>(a, v);
+        }
+#pragma unroll
+        for (int i = 0; i < T; ++i) f[i] = __builtin_bit_cast(Frag, v[i]);
     } else {
-        const uint32_t row = x + (lane & 15u), kc = kk * 4u + (lane >> 4);
-        return *reinterpret_cast<const Frag*>(lds + row * 128u + ((kc ^ swz_row(row)) << 4));
+#pragma unroll
+        for (int i = 0; i < T; ++i) f[i] = read_fragment<Frag>(lds, x + i * 16u, KK, lane);
     }
 }
 
@@ -167,17 +217,37 @@ struct Half<true> {
     static __device__ __forceinline__ f32x4 mma(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 
+// 16 rows x 64 columns of 16-bit values, four consecutive columns of a row per lane and block, to memory as whole 128-byte lines: straight
+// from the registers a store instruction would touch 16 rows in 32-byte pieces (measured: 850 us for 268 MB of probabilities; so 255 us).
+// cols (a multiple of 8) bounds the columns; 16-byte aligned rows.  scratch: 2 KiB of the wave's own.
+__device__ __forceinline__ void store_lines(char* scratch, const ushort4 (&v)[4], uint16_t* to, uint64_t ld, uint32_t row, uint32_t rows, uint32_t col, uint32_t cols,
+                                            uint32_t lane) {
+    const uint32_t r = lane & 15u, q = lane >> 4;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the last block has been read)
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) *reinterpret_cast<ushort4*>(scratch + r * 128u + (((j * 2u + (q >> 1)) ^ (r & 7u)) << 4) + (q & 1u) * 8u) = v[j];
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+        const uint32_t rr = h * 8u + (lane >> 3), c = lane & 7u;
+        const uint4 x = *reinterpret_cast<const uint4*>(scratch + rr * 128u + ((c ^ (rr & 7u)) << 4));
+        if (row + rr < rows && col + c * 8u < cols) *reinterpret_cast<uint4*>(to + (uint64_t)(row + rr) * ld + col + c * 8u) = x;
+    }
+    __builtin_amdgcn_wave_barrier();
+}
+
 // WM x WN waves, each MT x NT blocks of 16 x 16.
 template <int TM_, int TN_, int WM_, int WN_>
 struct Shape {
     static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, NW = WM_ * WN_;
     static constexpr int MT = TM_ / WM_ / 16, NT = TN_ / WN_ / 16;
     static constexpr int A_BYTES = TM_ * 128, B_BYTES = TN_ * 128, STAGE = A_BYTES + B_BYTES;
-    static constexpr int EPI_BYTES = WN_ * TM_ * 8;  // EPI_LOSS: (maximum, sum) per wave column and row
+    static constexpr int EPI_BYTES = WN_ * TM_ * 8 > NW * 2048 ? WN_ * TM_ * 8 : NW * 2048;  // EPI_LOSS: (maximum, sum) per wave column and row; else 2 KiB per wave
     static constexpr int LDS = 2 * STAGE + EPI_BYTES;
 };
-using Large = Shape<256, 256, 2, 4>;   // one workgroup per CU, 136 KiB of LDS
-using Small = Shape<64, 128, 2, 2>;    // 50 KiB: three workgroups per CU
+using Large = Shape<256, 256, 2, 4>;   // one workgroup per CU, 144 KiB of LDS
+using Small = Shape<64, 128, 2, 2>;    // 56 KiB: two workgroups per CU
 
 template <class S, int FORM, int EPI, bool BF16>
 __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
@@ -201,6 +271,12 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
     Loader<S::TN, S::NW, B_ACROSS> lb;
     la.init(g.a.ld, w, lane);
     lb.init(g.b.ld, w, lane);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+    uint32_t aa[S::MT], ab[S::NT];  // (across) the fragments' addresses within a stage
+#pragma unroll
+    for (int i = 0; i < S::MT; ++i) aa[i] = A_ACROSS ? across_address<S::TM>((wm * S::MT + i) * 16u, lane) : 0u;
+#pragma unroll
+    for (int j = 0; j < S::NT; ++j) ab[j] = B_ACROSS ? across_address<S::TN>((wn * S::NT + j) * 16u, lane) : 0u;
     const uint32_t steps = g.ksteps * g.segs;
     const uint32_t my_tiles = (tiles - 1u - blockIdx.x) / gridDim.x + 1u;
     const uint32_t total = my_tiles * steps;
@@ -236,25 +312,28 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
             __builtin_amdgcn_s_barrier();  // stage `at` is whole; nobody reads stage at - 1 any more
             asm volatile("" ::: "memory");
             if (p < total) prefetch();
-            const char* sa = lds + (at & 1u) * S::STAGE;
+            const uint32_t stage = (at & 1u) * S::STAGE;
+            const char* sa = lds + stage;
             const char* sb = sa + S::A_BYTES;
+            frag fa[S::MT], fb[S::NT];
+            read_fragments<S::TM, S::MT, A_ACROSS, 0>(sa, lds0 + stage, wm * S::MT * 16u, lane, aa, fa);
+            read_fragments<S::TN, S::NT, B_ACROSS, 0>(sb, lds0 + stage + S::A_BYTES, wn * S::NT * 16u, lane, ab, fb);
 #pragma unroll
-            for (uint32_t kk = 0; kk < kBK / 32; ++kk) {
-                frag fa[S::MT], fb[S::NT];
+            for (int i = 0; i < S::MT; ++i)
 #pragma unroll
-                for (int i = 0; i < S::MT; ++i) fa[i] = read_fragment<S::TM, A_ACROSS, frag>(sa, (wm * S::MT + i) * 16u, kk, lane);
+                for (int j = 0; j < S::NT; ++j) acc[i][j] = H::mma(fb[j], fa[i], acc[i][j]);
+            read_fragments<S::TM, S::MT, A_ACROSS, 1>(sa, lds0 + stage, wm * S::MT * 16u, lane, aa, fa);
+            read_fragments<S::TN, S::NT, B_ACROSS, 1>(sb, lds0 + stage + S::A_BYTES, wn * S::NT * 16u, lane, ab, fb);
 #pragma unroll
-                for (int j = 0; j < S::NT; ++j) fb[j] = read_fragment<S::TN, B_ACROSS, frag>(sb, (wn * S::NT + j) * 16u, kk, lane);
+            for (int i = 0; i < S::MT; ++i)
 #pragma unroll
-                for (int i = 0; i < S::MT; ++i)
-#pragma unroll
-                    for (int j = 0; j < S::NT; ++j) acc[i][j] = H::mma(fb[j], fa[i], acc[i][j]);
-            }
+                for (int j = 0; j < S::NT; ++j) acc[i][j] = H::mma(fb[j], fa[i], acc[i][j]);
         }
         // lane: row (lane & 15) of a 16 x 16 block, columns 4 * (lane / 16) + 0..3
         const uint32_t row0 = tm * S::TM + wm * S::MT * 16u + (lane & 15u);
-        const uint32_t cl = tn * S::TN + wn * S::NT * 16u + (lane >> 4) * 4u;
-        if constexpr (EPI == EPI_LOSS || EPI == EPI_PROB) {
+        const uint32_t c0 = tn * S::TN + wn * S::NT * 16u, cl = c0 + (lane >> 4) * 4u;
+        char* scratch = lds + 2 * S::STAGE + w * 2048u;
+        if constexpr (EPI == EPI_LOSS || EPI == EPI_PROB || EPI == EPI_PROB_ALONG) {
             const float wsc = g.wsc ? *g.wsc : 1.f;
             f32x4 h[S::NT];
             uint32_t live[S::NT];  // bit r: column j, r exists
@@ -311,50 +390,28 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                 }
                 // (the next tile's writes to `red` come after its first step's barrier: these reads are done by then)
             } else {
-                float ts[S::NT][4];
-                if (g.tpart) {
+                if constexpr (EPI == EPI_PROB_ALONG) {
+                    // (a pass of its own: its sums and the probabilities' stores together do not fit the registers)
+                    float ts[S::NT][4] = {};
 #pragma unroll
-                    for (int j = 0; j < S::NT; ++j)
+                    for (int i = 0; i < S::MT; ++i) {
+                        const uint32_t row = row0 + i * 16u;
+                        const int32_t lab = row < g.m ? g.label[row] : -1;
+                        const bool on = lab >= 0;
+                        float f = on ? g.zf[row] : 0.f;
+                        const float l2 = on ? g.lse2[row] : 0.f, gr = on ? g.graw[row] : 0.f;
+                        asm volatile("" : "+v"(f));  // (or the compiler keeps all 128 probabilities for the next pass)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) ts[j][r] = 0.f;
-                }
+                        for (int j = 0; j < S::NT; ++j)
 #pragma unroll
-                for (int i = 0; i < S::MT; ++i) {
-                    const uint32_t row = row0 + i * 16u;
-                    const bool has = row < g.m;
-                    const float f = has ? g.zf[row] : 0.f, l2 = has ? g.lse2[row] : 0.f, pf = has ? g.pf[row] : 0.f;
-                    const int32_t lab = has ? g.label[row] : -1;
-                    const bool on = lab >= 0;
-                    const float gr = g.tpart && on ? g.graw[row] : 0.f;
-#pragma unroll
-                    for (int j = 0; j < S::NT; ++j) {
-                        float v[4];
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const uint32_t c = cl + j * 16u + r;
-                            const float z = acc[i][j][r] * (f * h[j][r]);
-                            float q = exp2_fast(z - l2);
-                            if ((int32_t)(c + g.col0) == lab) q -= 1.f;
-                            const bool in = on && ((live[j] >> r) & 1u);
-                            if (g.tpart) ts[j][r] += in ? q * z * gr : 0.f;
-                            v[r] = in ? q * pf * (g.h ? h[j][r] : 1.f) : 0.f;
-                        }
-                        const uint32_t c = cl + j * 16u;
-                        if (has && c < g.prob_ld) {  // (prob_ld: n rounded up to 8, so a lane's four columns are in or out together)
-                            uint16_t* to = g.prob + (uint64_t)row * g.prob_ld + c;
-                            ushort4 hi;
-                            hi.x = to_half<BF16>(v[0]), hi.y = to_half<BF16>(v[1]), hi.z = to_half<BF16>(v[2]), hi.w = to_half<BF16>(v[3]);
-                            *reinterpret_cast<ushort4*>(to) = hi;
-                            if (g.prob_planes > 1) {
-                                ushort4 lo;
-                                lo.x = to_half<BF16>(v[0] - from_half<BF16>(hi.x)), lo.y = to_half<BF16>(v[1] - from_half<BF16>(hi.y));
-                                lo.z = to_half<BF16>(v[2] - from_half<BF16>(hi.z)), lo.w = to_half<BF16>(v[3] - from_half<BF16>(hi.w));
-                                *reinterpret_cast<ushort4*>(to + g.prob_plane) = lo;
+                            for (int r = 0; r < 4; ++r) {
+                                const float z = acc[i][j][r] * (f * h[j][r]);
+                                float q = exp2_fast(z - l2);
+                                if ((int32_t)(cl + j * 16u + r + g.col0) == lab) q -= 1.f;
+                                ts[j][r] += on && ((live[j] >> r) & 1u) ? q * z * gr : 0.f;
                             }
-                        }
+                        __builtin_amdgcn_sched_barrier(0);
                     }
-                }
-                if (g.tpart) {
 #pragma unroll
                     for (int j = 0; j < S::NT; ++j)
 #pragma unroll
@@ -367,6 +424,37 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                             const uint32_t c = cl + j * 16u + r;
                             if ((lane & 15u) == 0 && c < g.n) g.tpart[(size_t)(tm * S::WM + wm) * g.n + c] = t;
                         }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int i = 0; i < S::MT; ++i) {
+                    const uint32_t row = row0 + i * 16u;
+                    const bool has = row < g.m;
+                    const float f = has ? g.zf[row] : 0.f, l2 = has ? g.lse2[row] : 0.f, pf = has ? g.pf[row] : 0.f;
+                    const int32_t lab = has ? g.label[row] : -1;
+                    const bool on = lab >= 0;
+                    ushort4 hi[S::NT], lo[S::NT];
+#pragma unroll
+                    for (int j = 0; j < S::NT; ++j) {
+                        float v[4];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const uint32_t c = cl + j * 16u + r;
+                            const float z = acc[i][j][r] * (f * h[j][r]);
+                            float q = exp2_fast(z - l2);
+                            if ((int32_t)(c + g.col0) == lab) q -= 1.f;
+                            const bool in = on && ((live[j] >> r) & 1u);
+                            v[r] = in ? q * pf * (g.h ? h[j][r] : 1.f) : 0.f;
+                        }
+                        hi[j].x = to_half<BF16>(v[0]), hi[j].y = to_half<BF16>(v[1]), hi[j].z = to_half<BF16>(v[2]), hi[j].w = to_half<BF16>(v[3]);
+                        if (g.prob_planes > 1) {
+                            lo[j].x = to_half<BF16>(v[0] - from_half<BF16>(hi[j].x)), lo[j].y = to_half<BF16>(v[1] - from_half<BF16>(hi[j].y));
+                            lo[j].z = to_half<BF16>(v[2] - from_half<BF16>(hi[j].z)), lo[j].w = to_half<BF16>(v[3] - from_half<BF16>(hi[j].w));
+                        }
+                    }
+                    store_lines(scratch, hi, g.prob, g.prob_ld, row0 - (lane & 15u) + i * 16u, g.m, c0, g.prob_ld, lane);
+                    if (g.prob_planes > 1) store_lines(scratch, lo, g.prob + g.prob_plane, g.prob_ld, row0 - (lane & 15u) + i * 16u, g.m, c0, g.prob_ld, lane);
+                    __builtin_amdgcn_sched_barrier(0);  // one block of rows at a time: interleaved, they do not fit the registers
                 }
             }
         } else if constexpr (EPI == EPI_PART) {
@@ -382,26 +470,27 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
             }
         } else {
             const float wf = g.wf ? *g.wf : 1.f;
+            const bool lines = g.out_scalar != SC_F32 && g.n % 8u == 0 && g.out_ld % 8u == 0 && ((uintptr_t)g.out & 15u) == 0;
 #pragma unroll
             for (int i = 0; i < S::MT; ++i) {
                 const uint32_t row = row0 + i * 16u;
-                if (row < g.m) {
-                    const float rf = g.rf ? g.rf[row] * wf : wf;
-                    const float tc = g.tcoef ? g.tcoef[row] : 0.f, ti = g.tcoef ? g.tinv[row] : 0.f;
+                const bool has = row < g.m;
+                const float rf = has && g.rf ? g.rf[row] * wf : wf;
+                const float tc = has && g.tcoef ? g.tcoef[row] : 0.f, ti = has && g.tcoef ? g.tinv[row] : 0.f;
+                ushort4 o[S::NT];
 #pragma unroll
-                    for (int j = 0; j < S::NT; ++j) {
-                        const uint32_t c = cl + j * 16u;
-                        if (c < g.n) {
-                            f32x4 v = acc[i][j] * rf;
-                            if (tc != 0.f) {
+                for (int j = 0; j < S::NT; ++j) {
+                    const uint32_t c = cl + j * 16u;
+                    f32x4 v = acc[i][j] * rf;
+                    if (tc != 0.f) {
 #pragma unroll
-                                for (int r = 0; r < 4; ++r)
-                                    if (c + r < g.n) v[r] -= tc * (load_scalar(g.raw, g.raw_scalar, (uint64_t)row * g.raw_ld + c + r) * ti);
-                            }
-                            store4(g.out, g.out_scalar, (uint64_t)row * g.out_ld + c, v, g.n - c);
-                        }
+                        for (int r = 0; r < 4; ++r)
+                            if (c + r < g.n) v[r] -= tc * (load_scalar(g.raw, g.raw_scalar, (uint64_t)row * g.raw_ld + c + r) * ti);
                     }
+                    if (lines) o[j] = to_half4(g.out_scalar, v);
+                    else if (has && c < g.n) store4(g.out, g.out_scalar, (uint64_t)row * g.out_ld + c, v, g.n - c);
                 }
+                if (lines) store_lines(scratch, o, (uint16_t*)g.out, g.out_ld, row0 - (lane & 15u) + i * 16u, g.m, c0, g.n, lane);
             }
         }
     }
