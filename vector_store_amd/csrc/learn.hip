@@ -51,11 +51,11 @@ struct QueryPrep {
     uint32_t nplanes;
     uint64_t plane;
     int32_t* label;
-    float* zf;
+    float4* row;  // the products' factors: (zf, lse2, pf, label)
     // backward (g != nullptr)
     const float* g;
     const float* lse;
-    float *lse2, *pf, *df, *inv;
+    float *df, *inv;
     int32_t *ge, *xe;
 };
 
@@ -107,25 +107,27 @@ __global__ __launch_bounds__(256) void query_prep_kernel(QueryPrep a) {
     if (y < 0 || y >= (int64_t)a.rows || (a.keys && a.keys[y] == ~0ull)) y = -1;
     a.label[i] = (int32_t)y;
     const float s2 = a.scale * kLog2e;
-    a.zf[i] = a.raw ? s2 * inv : a.cosine ? s2 * 0x1p-26f : ldexpf(s2, e - 13);
-    if (!a.g) return;
-    a.lse2[i] = a.lse[i] * kLog2e;
-    a.inv[i] = inv;
-    const float g = y >= 0 ? a.g[i] : 0.f;
-    if (a.bf) {
-        a.pf[i] = g * inv * a.scale;
-        a.df[i] = y >= 0 ? 1.f : 0.f;
-        a.ge[i] = 0;
-        a.xe[i] = 0;
-        return;
+    float4 row = make_float4(a.raw ? s2 * inv : a.cosine ? s2 * 0x1p-26f : ldexpf(s2, e - 13), 0.f, 0.f, __int_as_float((int32_t)y));
+    if (a.g) {
+        row.y = a.lse[i] * kLog2e;
+        a.inv[i] = inv;
+        const float g = y >= 0 ? a.g[i] : 0.f;
+        if (a.bf) {
+            row.z = g * inv * a.scale;
+            a.df[i] = y >= 0 ? 1.f : 0.f;
+            a.ge[i] = 0;
+            a.xe[i] = 0;
+        } else {
+            // f16 probabilities: (p - [label]) * m * 2^13 with g = m * 2^x, 1/2 <= |m| < 1: below 2^13, and full precision down to p = 2^-26
+            int x = 0;
+            const float m = frexpf(g, &x);
+            row.z = m * 8192.f;
+            a.df[i] = y >= 0 ? ldexpf(a.scale * (a.cosine ? inv * 0x1p-13f : 1.f), x - 13) : 0.f;
+            a.ge[i] = x;
+            a.xe[i] = y < 0 || !(g != 0.f) ? kNoExponent : x + exponent_of(a.cosine ? top * inv : top);
+        }
     }
-    // f16 probabilities: (p - [label]) * m * 2^13 with g = m * 2^x, 1/2 <= |m| < 1: below 2^13, and full precision down to p = 2^-26
-    int x = 0;
-    const float m = frexpf(g, &x);
-    a.pf[i] = m * 8192.f;
-    a.df[i] = y >= 0 ? ldexpf(a.scale * (a.cosine ? inv * 0x1p-13f : 1.f), x - 13) : 0.f;
-    a.ge[i] = x;
-    a.xe[i] = y < 0 || !(g != 0.f) ? kNoExponent : x + exponent_of(a.cosine ? top * inv : top);
+    a.row[i] = row;
 }
 
 // The queries as an operand of dw = P^T q: rows of padding are zero whatever they held, and (f16) every row carries the power of two of its
@@ -319,7 +321,7 @@ static void run_product(const ProductArgs& g, hipStream_t st) {
     const uint64_t tiles = (uint64_t)g.tiles_m * g.tiles_n * g.splits;
     if (tiles >= (1ull << 31)) fail(VS_ERR_UNSUPPORTED, "too many tiles");
     constexpr uint32_t resident = 256u * (160u * 1024u / S::LDS);
-    hipLaunchKernelGGL((product_kernel<S, FORM, EPI, BF>), dim3((uint32_t)std::min<uint64_t>(tiles, resident)), dim3(S::NW * 64), S::LDS, st, g);
+    hipLaunchKernelGGL((product_kernel<S, FORM, EPI, BF>), dim3((uint32_t)std::min<uint64_t>((tiles + 7) / 8 * 8, resident)), dim3(S::NW * 64), S::LDS, st, g);
     launched("product");
 }
 template <int FORM, int EPI>
@@ -414,8 +416,8 @@ struct Plan {
     uint32_t piece = 0, pieces = 0;
     bool large_s = false, large_q = false, large_w = false;
     uint32_t splits = 1, qsteps = 1, tiles_v = 0, trows = 0;
-    size_t o_label, o_zf, o_qplanes, o_top, o_wsc, o_inv, o_wplanes, o_part, o_zlab;
-    size_t o_lse2, o_pf, o_df, o_qinv, o_ge, o_xe, o_exp, o_gplanes, o_prob, o_tpart, o_coef, o_qpart, o_qacc;
+    size_t o_label, o_row, o_qplanes, o_top, o_wsc, o_inv, o_wplanes, o_part, o_zlab;
+    size_t o_df, o_qinv, o_ge, o_xe, o_exp, o_gplanes, o_prob, o_tpart, o_coef, o_qpart, o_qacc;
     size_t bytes = 0;
 };
 
@@ -480,7 +482,7 @@ static Plan plan(const vs_rows* rows, const vs_softmax* q, bool grad_q, bool gra
     p.trows = (n + stm - 1) / stm * 2;  // (both shapes have two wave rows)
     Layout l;
     p.o_label = l.take((size_t)n * 4);
-    p.o_zf = l.take((size_t)n * 4);
+    p.o_row = l.take((size_t)n * 16);
     p.o_qplanes = l.take(p.q_in_place ? 0 : (size_t)p.nq * n * p.dp * 2);
     p.o_top = l.take((size_t)p.pieces * 4);
     p.o_wsc = l.take((size_t)p.pieces * 4);
@@ -490,8 +492,6 @@ static Plan plan(const vs_rows* rows, const vs_softmax* q, bool grad_q, bool gra
         p.o_part = l.take((size_t)n * p.tiles_v * 8);
         p.o_zlab = l.take((size_t)n * 4);
     } else {
-        p.o_lse2 = l.take((size_t)n * 4);
-        p.o_pf = l.take((size_t)n * 4);
         p.o_df = l.take((size_t)n * 4);
         p.o_qinv = l.take((size_t)n * 4);
         p.o_ge = l.take((size_t)n * 4);
@@ -541,11 +541,11 @@ struct Call {  // what the two calls share
         a.nplanes = p.nq;
         a.plane = (uint64_t)p.n * p.dp;
         a.label = at<int32_t>(p.o_label);
-        a.zf = at<float>(p.o_zf);
+        a.row = at<float4>(p.o_row);
         if (g) {
             a.g = g;
             a.lse = lse;
-            a.lse2 = at<float>(p.o_lse2), a.pf = at<float>(p.o_pf), a.df = at<float>(p.o_df), a.inv = at<float>(p.o_qinv);
+            a.df = at<float>(p.o_df), a.inv = at<float>(p.o_qinv);
             a.ge = at<int32_t>(p.o_ge), a.xe = at<int32_t>(p.o_xe);
         }
         hipLaunchKernelGGL(query_prep_kernel, dim3((p.n + 3) / 4), dim3(256), 0, st, a);
@@ -599,11 +599,10 @@ struct Call {  // what the two calls share
         g.splits = 1;
         g.ksteps = (g.k + 63) / 64;
         plane_pairs(g, p.nq, p.nw, true);
-        g.zf = at<float>(p.o_zf);
+        g.row = at<float4>(p.o_row);
         g.h = h() ? h() + first : nullptr;
         g.wsc = p.raw || p.cosine ? nullptr : at<float>(p.o_wsc) + x;
         g.keys = p.w.keys ? p.w.keys + first : nullptr;
-        g.label = at<int32_t>(p.o_label);
         g.col0 = first;
         return g;
     }
@@ -683,8 +682,6 @@ static void loss_grad(const vs_rows* rows, const vs_softmax* q, const float* d_l
         const uint32_t first = x * p.piece, count = std::min(p.piece, p.v - first);
         const Operand w = c.rows(x, first, count);
         ProductArgs g = c.scores(w, x, first, count);
-        g.lse2 = c.at<float>(p.o_lse2);
-        g.pf = c.at<float>(p.o_pf);
         g.prob = c.at<uint16_t>(p.o_prob);
         g.prob_ld = (count + 7u) & ~7u;
         g.prob_plane = (uint64_t)p.n * g.prob_ld;

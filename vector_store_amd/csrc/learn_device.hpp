@@ -29,6 +29,19 @@ __device__ __forceinline__ float2 join_sums(float2 a, float2 b) {
     return make_float2(m, a.y * exp2_fast(a.x - m) + b.y * exp2_fast(b.x - m));
 }
 
+// a and b hold one value per lane of two rows of blocks; N = 32: the halves of the wave are joined, lanes 0..31 end up with a's sums and lanes
+// 32..63 with b's; N = 16: the same for the odd and even sixteens (a in rows 0 and 2, b in rows 1 and 3)
+template <int N>
+__device__ __forceinline__ float2 join_swapped(float2 a, float2 b) {
+    using u2 = __attribute__((ext_vector_type(2))) unsigned int;
+    const auto swap = [](float x, float y) {
+        if constexpr (N == 32) return __builtin_bit_cast(u2, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false));
+        else return __builtin_bit_cast(u2, __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false));
+    };
+    const u2 m = swap(a.x, b.x), s = swap(a.y, b.y);
+    return join_sums(make_float2(__uint_as_float(m[0]), __uint_as_float(s[0])), make_float2(__uint_as_float(m[1]), __uint_as_float(s[1])));
+}
+
 __device__ __forceinline__ float load_scalar(const void* p, int scalar, uint64_t i) {
     if (scalar == SC_F32) return reinterpret_cast<const float*>(p)[i];
     const uint16_t h = reinterpret_cast<const uint16_t*>(p)[i];

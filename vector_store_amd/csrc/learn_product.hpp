@@ -42,20 +42,17 @@ struct ProductArgs {
     uint32_t splits, ksteps;     // slices of k and 64-deep steps per slice
     uint32_t segs;               // plane pairs
     uint32_t seg_a, seg_b;       // 4 bits each: the planes of pair s
-    // EPI_LOSS / EPI_PROB: z2 = acc * zf[row] * wsc * h[col] (base-2 exponent units)
-    const float* zf;
+    // EPI_LOSS / EPI_PROB: z2 = acc * zf * wsc * h[col] (base-2 exponent units); per row (zf, lse2, pf, label as bits)
+    const float4* row;
     const float* h;              // nullptr: 1
     const float* wsc;            // nullptr: 1
     const uint64_t* keys;        // nullptr, or per column: ~0 = not a member
-    const int32_t* label;        // per row: column of the whole table, -1 = ignored
-    uint32_t col0;               // first column of this piece
+    uint32_t col0;               // first column of this piece (labels are columns of the whole table, -1 = ignored)
     // EPI_LOSS
     float2* part;                // [m][part_ld] (maximum, sum of 2^(z2 - maximum)) per column tile
     uint32_t part_ld, part0;
     float* zlab;                 // z2 at the label
     // EPI_PROB: P = (2^(z2 - lse2) - [label]) * pf[row] * h[col]
-    const float* lse2;
-    const float* pf;
     uint16_t* prob;
     uint64_t prob_plane;         // elements
     uint32_t prob_ld, prob_planes;
@@ -243,11 +240,13 @@ struct Shape {
     static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, NW = WM_ * WN_;
     static constexpr int MT = TM_ / WM_ / 16, NT = TN_ / WN_ / 16;
     static constexpr int A_BYTES = TM_ * 128, B_BYTES = TN_ * 128, STAGE = A_BYTES + B_BYTES;
-    static constexpr int EPI_BYTES = WN_ * TM_ * 8 > NW * 2048 ? WN_ * TM_ * 8 : NW * 2048;  // EPI_LOSS: (maximum, sum) per wave column and row; else 2 KiB per wave
+    // row factors, then EPI_LOSS: (maximum, sum) per wave column and row; else 2 KiB per wave
+    static constexpr int ROW_BYTES = TM_ * 16;
+    static constexpr int EPI_BYTES = ROW_BYTES + (WN_ * TM_ * 8 > NW * 2048 ? WN_ * TM_ * 8 : NW * 2048);
     static constexpr int LDS = 2 * STAGE + EPI_BYTES;
 };
-using Large = Shape<256, 256, 2, 4>;   // one workgroup per CU, 144 KiB of LDS
-using Small = Shape<64, 128, 2, 2>;    // 56 KiB: two workgroups per CU
+using Large = Shape<256, 256, 2, 4>;   // one workgroup per CU, 148 KiB of LDS
+using Small = Shape<64, 128, 2, 2>;    // 57 KiB: two workgroups per CU
 
 template <class S, int FORM, int EPI, bool BF16>
 __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
@@ -256,16 +255,24 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
     using frag = typename H::frag;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const uint32_t lane = threadIdx.x & 63u, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = w / S::WN, wn = w % S::WN;
-    const uint32_t per_split = g.tiles_m * g.tiles_n, tiles = per_split * g.splits;
-    if (blockIdx.x >= tiles) return;
-    // blocks b, b + 8, b + 16 ... share an XCD and its L2: they take the row tiles of the same column tile one after the other
+    // Blocks b, b + 8, b + 16 ... share an XCD and its L2: each XCD takes a contiguous share of the tiles, ordered so that the tiles in
+    // flight on its 32 CUs are a compact patch (8 row tiles by 4 column tiles of the scores; all column tiles of a row tile of the gradients):
+    // an operand's stage is fetched once per XCD and read by the others from L2.
+    constexpr uint32_t GROUP = FORM == SCORES ? 4u : 8u;
+    const uint32_t per_split = g.tiles_m * g.tiles_n, all = per_split * g.splits;
+    const uint32_t share = (all + 7u) / 8u, first = (blockIdx.x & 7u) * share;
+    const uint32_t mine = first < all ? (all - first < share ? all - first : share) : 0u;  // tiles of this XCD
+    const uint32_t step = gridDim.x >> 3;                                                  // (the grid: a multiple of 8)
+    const uint32_t tile0 = blockIdx.x >> 3;
+    if (tile0 >= mine) return;
     const auto place = [&](uint32_t t, uint32_t& tm, uint32_t& tn, uint32_t& sp) {
+        t += first;
         sp = t / per_split;
         const uint32_t r = t - sp * per_split;
-        const uint32_t group = r / (8u * g.tiles_m), in = r - group * 8u * g.tiles_m;
-        const uint32_t left = g.tiles_n - group * 8u, width = left < 8u ? left : 8u;
+        const uint32_t group = r / (GROUP * g.tiles_m), in = r - group * GROUP * g.tiles_m;
+        const uint32_t left = g.tiles_n - group * GROUP, width = left < GROUP ? left : GROUP;
         tm = in / width;
-        tn = group * 8u + in % width;
+        tn = group * GROUP + in % width;
     };
     Loader<S::TM, S::NW, A_ACROSS> la;
     Loader<S::TN, S::NW, B_ACROSS> lb;
@@ -278,9 +285,8 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
 #pragma unroll
     for (int j = 0; j < S::NT; ++j) ab[j] = B_ACROSS ? across_address<S::TN>((wn * S::NT + j) * 16u, lane) : 0u;
     const uint32_t steps = g.ksteps * g.segs;
-    const uint32_t my_tiles = (tiles - 1u - blockIdx.x) / gridDim.x + 1u;
-    const uint32_t total = my_tiles * steps;
-    uint32_t p = 0, p_tile = blockIdx.x, p_seg = 0, p_ks = 0, p_tm, p_tn, p_sp;
+    const uint32_t total = ((mine - 1u - tile0) / step + 1u) * steps;
+    uint32_t p = 0, p_tile = tile0, p_seg = 0, p_ks = 0, p_tm, p_tn, p_sp;
     place(p_tile, p_tm, p_tn, p_sp);
     const auto prefetch = [&]() {
         char* st = lds + (p & 1u) * S::STAGE;
@@ -292,16 +298,22 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
             p_ks = 0;
             if (++p_seg == g.segs) {
                 p_seg = 0;
-                p_tile += gridDim.x;
-                if (p_tile < tiles) place(p_tile, p_tm, p_tn, p_sp);
+                p_tile += step;
+                if (p_tile < mine) place(p_tile, p_tm, p_tn, p_sp);
             }
         }
     };
     prefetch();
     uint32_t at = 0;
-    for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    for (uint32_t tile = tile0; tile < mine; tile += step) {
         uint32_t tm, tn, sp;
         place(tile, tm, tn, sp);
+        // the tile's row factors travel while the product runs
+        constexpr bool SOFTMAX = FORM == SCORES;
+        float4 factors = make_float4(0.f, 0.f, 0.f, __int_as_float(-1));
+        if constexpr (SOFTMAX) {
+            if (threadIdx.x < (uint32_t)S::TM && tm * S::TM + threadIdx.x < g.m) factors = g.row[tm * S::TM + threadIdx.x];
+        }
         f32x4 acc[S::MT][S::NT];
 #pragma unroll
         for (int i = 0; i < S::MT; ++i)
@@ -332,51 +344,78 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
         // lane: row (lane & 15) of a 16 x 16 block, columns 4 * (lane / 16) + 0..3
         const uint32_t row0 = tm * S::TM + wm * S::MT * 16u + (lane & 15u);
         const uint32_t c0 = tn * S::TN + wn * S::NT * 16u, cl = c0 + (lane >> 4) * 4u;
-        char* scratch = lds + 2 * S::STAGE + w * 2048u;
-        if constexpr (EPI == EPI_LOSS || EPI == EPI_PROB || EPI == EPI_PROB_ALONG) {
+        char* scratch = lds + 2 * S::STAGE + S::ROW_BYTES + w * 2048u;
+        if constexpr (SOFTMAX) {
+            float4* rows = reinterpret_cast<float4*>(lds + 2 * S::STAGE);
+            if (threadIdx.x < (uint32_t)S::TM) rows[threadIdx.x] = factors;
             const float wsc = g.wsc ? *g.wsc : 1.f;
+            // columns that all exist and have no factor of their own: the common case, with fewer instructions per score (the epilogue's
+            // vector instructions are what a product of short rows waits for: 128 scores per lane)
+            const bool plain = !g.h && !g.keys && c0 + S::NT * 16u <= g.n;
             f32x4 h[S::NT];
             uint32_t live[S::NT];  // bit r: column j, r exists
+            if (!plain) {
 #pragma unroll
-            for (int j = 0; j < S::NT; ++j) {
-                live[j] = 0;
+                for (int j = 0; j < S::NT; ++j) {
+                    live[j] = 0;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const uint32_t c = cl + j * 16u + r;
-                    const bool in = c < g.n && !(g.keys && g.keys[c] == ~0ull);
-                    live[j] |= in ? 1u << r : 0u;
-                    h[j][r] = in ? (g.h ? g.h[c] * wsc : wsc) : 0.f;
+                    for (int r = 0; r < 4; ++r) {
+                        const uint32_t c = cl + j * 16u + r;
+                        const bool in = c < g.n && !(g.keys && g.keys[c] == ~0ull);
+                        live[j] |= in ? 1u << r : 0u;
+                        h[j][r] = in ? (g.h ? g.h[c] : 1.f) : 0.f;
+                    }
                 }
             }
+            __syncthreads();
             if constexpr (EPI == EPI_LOSS) {
-                float2* red = reinterpret_cast<float2*>(lds + 2 * S::STAGE);
+                float2* red = reinterpret_cast<float2*>(lds + 2 * S::STAGE + S::ROW_BYTES);
+                float2 ms[S::MT];  // of this lane's 16 columns
 #pragma unroll
                 for (int i = 0; i < S::MT; ++i) {
-                    const uint32_t row = row0 + i * 16u;
-                    const bool has = row < g.m;
-                    const float f = has ? g.zf[row] : 0.f;
-                    const int32_t lab = has ? g.label[row] - (int32_t)g.col0 : -1;
-                    float top = -__builtin_inff();
+                    const float4 rf = rows[(wm * S::MT + i) * 16u + (lane & 15u)];
+                    const float f = rf.x * wsc;
+                    const uint32_t lab = (uint32_t)(__float_as_int(rf.w) - (int32_t)g.col0) - cl;
+                    float top = -__builtin_inff(), sum = 0.f;
+                    if (plain) {
 #pragma unroll
-                    for (int j = 0; j < S::NT; ++j)
+                        for (int j = 0; j < S::NT; ++j) acc[i][j] *= f;
+                    } else {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const float z = (live[j] >> r) & 1u ? acc[i][j][r] * (f * h[j][r]) : -__builtin_inff();
-                            acc[i][j][r] = z;
-                            if ((int32_t)(cl + j * 16u + r) == lab) g.zlab[row] = z;
-                            top = fmaxf(top, z);
-                        }
-                    top = fmaxf(top, __shfl_xor(top, 16));
-                    top = fmaxf(top, __shfl_xor(top, 32));
-                    float sum = 0.f;
+                        for (int j = 0; j < S::NT; ++j)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) acc[i][j][r] = (live[j] >> r) & 1u ? acc[i][j][r] * (f * h[j][r]) : -__builtin_inff();
+                    }
+#pragma unroll
+                    for (int j = 0; j < S::NT; ++j) top = fmaxf(fmaxf(fmaxf(top, acc[i][j][0]), fmaxf(acc[i][j][1], acc[i][j][2])), acc[i][j][3]);
+                    if (__any(lab < S::NT * 16u)) {  // a label of these rows lies in the wave's columns
+#pragma unroll
+                        for (int j = 0; j < S::NT; ++j)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                if (lab == j * 16u + r) g.zlab[row0 + i * 16u] = acc[i][j][r];
+                    }
                     const float base = top == -__builtin_inff() ? 0.f : top;
 #pragma unroll
                     for (int j = 0; j < S::NT; ++j)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) sum += exp2_fast(acc[i][j][r] - base);
-                    sum += __shfl_xor(sum, 16);
-                    sum += __shfl_xor(sum, 32);
-                    if (lane < 16) red[wn * S::TM + (wm * S::MT + i) * 16u + lane] = make_float2(top, sum);
+                    ms[i] = make_float2(top, sum);
+                }
+                // the four lanes of a row: block pairs swap halves, so that a join serves two blocks of rows at once
+                if constexpr (S::MT == 8) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) ms[i] = join_swapped<32>(ms[2 * i], ms[2 * i + 1]);
+                    ms[0] = join_swapped<16>(ms[0], ms[1]);
+                    ms[1] = join_swapped<16>(ms[2], ms[3]);
+                    const uint32_t q = lane >> 4, i = (q & 1u) * 2u + (q >> 1);
+                    red[wn * S::TM + (wm * S::MT + i) * 16u + (lane & 15u)] = ms[0];
+                    red[wn * S::TM + (wm * S::MT + 4u + i) * 16u + (lane & 15u)] = ms[1];
+                } else {
+                    static_assert(S::MT == 2, "row blocks per wave");
+                    float2 a = join_swapped<32>(ms[0], ms[1]);
+                    a = join_sums(a, make_float2(__shfl_xor(a.x, 16), __shfl_xor(a.y, 16)));
+                    if (!(lane & 16u)) red[wn * S::TM + (wm * S::MT + (lane >> 5)) * 16u + (lane & 15u)] = a;
                 }
                 __syncthreads();
                 for (uint32_t t = threadIdx.x; t < (uint32_t)S::TM; t += S::NW * 64) {
@@ -388,68 +427,87 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                         g.part[(size_t)row * g.part_ld + g.part0 + tn] = a;
                     }
                 }
-                // (the next tile's writes to `red` come after its first step's barrier: these reads are done by then)
+                // (the next tile's writes here come after its first step's barrier: these reads are done by then)
             } else {
                 if constexpr (EPI == EPI_PROB_ALONG) {
-                    // (a pass of its own: its sums and the probabilities' stores together do not fit the registers)
-                    float ts[S::NT][4] = {};
+                    // (a pass of its own, four columns at a time: its sums and the probabilities' stores together do not fit the registers)
+                    float gr[S::MT];
 #pragma unroll
-                    for (int i = 0; i < S::MT; ++i) {
-                        const uint32_t row = row0 + i * 16u;
-                        const int32_t lab = row < g.m ? g.label[row] : -1;
-                        const bool on = lab >= 0;
-                        float f = on ? g.zf[row] : 0.f;
-                        const float l2 = on ? g.lse2[row] : 0.f, gr = on ? g.graw[row] : 0.f;
-                        asm volatile("" : "+v"(f));  // (or the compiler keeps all 128 probabilities for the next pass)
+                    for (int i = 0; i < S::MT; ++i) gr[i] = row0 + i * 16u < g.m ? g.graw[row0 + i * 16u] : 0.f;
 #pragma unroll
-                        for (int j = 0; j < S::NT; ++j)
+                    for (int j = 0; j < S::NT; ++j) {
+                        f32x4 t = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int i = 0; i < S::MT; ++i) {
+                            const float4 rf = rows[(wm * S::MT + i) * 16u + (lane & 15u)];
+                            const uint32_t lab = (uint32_t)(__float_as_int(rf.w) - (int32_t)g.col0) - cl - j * 16u;
+                            float f = rf.x * wsc;
+                            asm volatile("" : "+v"(f));  // (or the compiler keeps all 128 probabilities for the next pass)
 #pragma unroll
                             for (int r = 0; r < 4; ++r) {
-                                const float z = acc[i][j][r] * (f * h[j][r]);
-                                float q = exp2_fast(z - l2);
-                                if ((int32_t)(cl + j * 16u + r + g.col0) == lab) q -= 1.f;
-                                ts[j][r] += on && ((live[j] >> r) & 1u) ? q * z * gr : 0.f;
+                                const float z = acc[i][j][r] * (plain ? f : f * h[j][r]);
+                                const float q = exp2_fast(z - rf.y) - (lab == (uint32_t)r ? 1.f : 0.f);
+                                t[r] += __float_as_int(rf.w) >= 0 && (plain || ((live[j] >> r) & 1u)) ? q * z * gr[i] : 0.f;
                             }
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-#pragma unroll
-                    for (int j = 0; j < S::NT; ++j)
+                        }
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            float t = ts[j][r];
-                            t += __shfl_xor(t, 1);
-                            t += __shfl_xor(t, 2);
-                            t += __shfl_xor(t, 4);
-                            t += __shfl_xor(t, 8);
+                            t[r] += __shfl_xor(t[r], 1);
+                            t[r] += __shfl_xor(t[r], 2);
+                            t[r] += __shfl_xor(t[r], 4);
+                            t[r] += __shfl_xor(t[r], 8);
                             const uint32_t c = cl + j * 16u + r;
-                            if ((lane & 15u) == 0 && c < g.n) g.tpart[(size_t)(tm * S::WM + wm) * g.n + c] = t;
+                            if ((lane & 15u) == 0 && c < g.n) g.tpart[(size_t)(tm * S::WM + wm) * g.n + c] = t[r];
                         }
-                    __builtin_amdgcn_sched_barrier(0);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
                 }
 #pragma unroll
                 for (int i = 0; i < S::MT; ++i) {
-                    const uint32_t row = row0 + i * 16u;
-                    const bool has = row < g.m;
-                    const float f = has ? g.zf[row] : 0.f, l2 = has ? g.lse2[row] : 0.f, pf = has ? g.pf[row] : 0.f;
-                    const int32_t lab = has ? g.label[row] : -1;
-                    const bool on = lab >= 0;
+                    const float4 rf = rows[(wm * S::MT + i) * 16u + (lane & 15u)];
+                    const float f = rf.x * wsc;
+                    const int32_t label = __float_as_int(rf.w);
+                    const uint32_t lab = (uint32_t)(label - (int32_t)g.col0) - cl;
+                    float v[S::NT][4];
+                    if (plain) {
+#pragma unroll
+                        for (int j = 0; j < S::NT; ++j)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) v[j][r] = exp2_fast(fmaf(acc[i][j][r], f, -rf.y));
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < S::NT; ++j)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) v[j][r] = (live[j] >> r) & 1u ? exp2_fast(acc[i][j][r] * (f * h[j][r]) - rf.y) : 0.f;
+                    }
+                    if (__any(lab < S::NT * 16u)) {
+#pragma unroll
+                        for (int j = 0; j < S::NT; ++j)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                if (lab == j * 16u + r) v[j][r] -= 1.f;
+                    }
+                    if (g.h) {
+#pragma unroll
+                        for (int j = 0; j < S::NT; ++j)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) v[j][r] *= h[j][r];
+                    }
+                    if (__any(label < 0)) {  // padding: whatever its query holds
+#pragma unroll
+                        for (int j = 0; j < S::NT; ++j)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) v[j][r] = label < 0 ? 0.f : v[j][r];
+                    }
                     ushort4 hi[S::NT], lo[S::NT];
 #pragma unroll
                     for (int j = 0; j < S::NT; ++j) {
-                        float v[4];
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const uint32_t c = cl + j * 16u + r;
-                            const float z = acc[i][j][r] * (f * h[j][r]);
-                            float q = exp2_fast(z - l2);
-                            if ((int32_t)(c + g.col0) == lab) q -= 1.f;
-                            const bool in = on && ((live[j] >> r) & 1u);
-                            v[r] = in ? q * pf * (g.h ? h[j][r] : 1.f) : 0.f;
-                        }
-                        hi[j].x = to_half<BF16>(v[0]), hi[j].y = to_half<BF16>(v[1]), hi[j].z = to_half<BF16>(v[2]), hi[j].w = to_half<BF16>(v[3]);
+                        for (int r = 0; r < 4; ++r) v[j][r] *= rf.z;
+                        hi[j].x = to_half<BF16>(v[j][0]), hi[j].y = to_half<BF16>(v[j][1]), hi[j].z = to_half<BF16>(v[j][2]), hi[j].w = to_half<BF16>(v[j][3]);
                         if (g.prob_planes > 1) {
-                            lo[j].x = to_half<BF16>(v[0] - from_half<BF16>(hi[j].x)), lo[j].y = to_half<BF16>(v[1] - from_half<BF16>(hi[j].y));
-                            lo[j].z = to_half<BF16>(v[2] - from_half<BF16>(hi[j].z)), lo[j].w = to_half<BF16>(v[3] - from_half<BF16>(hi[j].w));
+                            lo[j].x = to_half<BF16>(v[j][0] - from_half<BF16>(hi[j].x)), lo[j].y = to_half<BF16>(v[j][1] - from_half<BF16>(hi[j].y));
+                            lo[j].z = to_half<BF16>(v[j][2] - from_half<BF16>(hi[j].z)), lo[j].w = to_half<BF16>(v[j][3] - from_half<BF16>(hi[j].w));
                         }
                     }
                     store_lines(scratch, hi, g.prob, g.prob_ld, row0 - (lane & 15u) + i * 16u, g.m, c0, g.prob_ld, lane);
