@@ -81,12 +81,16 @@ __device__ __forceinline__ uint32_t swz_k(uint32_t k) {
     return ((k & 3u) | (((k >> 3) & 1u) << 2)) & (COLS / 16 - 1u);
 }
 
-// One operand's stage: 64 deep, X output rows / columns wide (X * 128 bytes of LDS), brought in by NW waves in pieces of 1 KiB.
+// One operand's stages: 64 deep, X output rows / columns wide (X * 128 bytes of LDS), brought in by NW waves in pieces of 1 KiB.  Between
+// two steps only a scalar moves; the instructions between a step's barrier and its first MFMA are what every wave of the CU waits for
+// (a descriptor computed per step cost 190 of 800 us at 4,096 x 131,072 x 768).
 template <int X, int NW, bool ACROSS>
 struct Loader {
     static constexpr int PIECES = X / 8 / NW;
     static_assert(X % (8 * NW) == 0, "whole pieces per wave");
     uint32_t off[PIECES];
+    const char* base;       // of the tile's first row / column (along), of the step (across)
+    uint32_t limit, full;   // bytes behind base that belong to the operand; across: of a step 64 deep
     __device__ __forceinline__ void init(uint64_t ld, uint32_t w, uint32_t lane) {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
@@ -101,36 +105,50 @@ struct Loader {
             }
         }
     }
-    // x0: first output row / column of the tile; k0: first k of the step; kend: end of k (a multiple of 8 along k)
-    __device__ __forceinline__ void stage(const Operand& o, uint32_t plane, uint32_t x0, uint32_t k0, uint32_t kend, char* lds, uint32_t w, uint32_t lane) const {
-        const char* base;
-        uint64_t bytes = 0;
+    static __device__ __forceinline__ uint32_t clamped(uint64_t bytes) { return bytes > 0x7FFFF000ull ? 0x7FFFF000u : (uint32_t)bytes; }
+    // x0: first output row / column of the tile; k0: first k of the step; kend: end of k
+    __device__ __forceinline__ void open(const Operand& o, uint32_t plane, uint32_t x0, uint32_t k0, uint32_t kend) {
         if constexpr (ACROSS) {
             base = o.p + plane * o.plane + (uint64_t)k0 * o.ld + (uint64_t)x0 * 2u;
-            if (k0 < kend && x0 < o.cols) {
-                const uint32_t left = kend - k0 < (uint32_t)kBK ? kend - k0 : (uint32_t)kBK;
-                bytes = (uint64_t)(left - 1u) * o.ld + (uint64_t)(o.cols - x0) * 2u;
-            }
+            full = x0 < o.cols ? clamped((kBK - 1u) * o.ld + (uint64_t)(o.cols - x0) * 2u) : 0u;
+            depth(o, k0, kend);
         } else {
-            base = o.p + plane * o.plane + (uint64_t)x0 * o.ld + (uint64_t)k0 * 2u;
-            if (k0 < kend && x0 < o.rows) bytes = (uint64_t)(o.rows - x0) * o.ld - (uint64_t)k0 * 2u;
-        }
-        const uint32_t limit = bytes > 0x7FFFF000ull ? 0x7FFFF000u : (uint32_t)bytes;
-        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)limit, 0x00020000);
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            uint32_t v = off[i];
-            if constexpr (!ACROSS) {
-                if (k0 + kBK > kend) {  // the last step of a depth that is no multiple of 64: chunks beyond it read nothing
-                    const uint32_t row = (w * PIECES + i) * 8u + (lane >> 3);
-                    const uint32_t kc = ((lane & 7u) ^ swz_row(row)) * 8u;
-                    if (k0 + kc >= kend) v = 0x7FFFFFF0u;
-                }
-            }
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(lds + (w * PIECES + i) * 1024u), 16, v, 0, 0, 0);
+            base = o.p + plane * o.plane + (uint64_t)x0 * o.ld;
+            limit = x0 < o.rows ? clamped((uint64_t)(o.rows - x0) * o.ld) : 0u;
         }
     }
+    __device__ __forceinline__ void depth(const Operand& o, uint32_t k0, uint32_t kend) {
+        const uint32_t left = k0 < kend ? kend - k0 : 0u;
+        const uint32_t less = left < (uint32_t)kBK ? (kBK - left) * (uint32_t)o.ld : 0u;
+        limit = left && less < full ? full - less : 0u;
+    }
+    __device__ __forceinline__ void advance(const Operand& o, uint32_t k0, uint32_t kend) {  // to the next step, at k0
+        if constexpr (ACROSS) {
+            base += (uint64_t)kBK * o.ld;
+            depth(o, k0, kend);
+        }
+    }
+    __device__ __forceinline__ void piece(int i, bool more, uint32_t k0, uint32_t kend, char* lds, uint32_t w, uint32_t lane) const {
+        // (all of it the same in every lane: kept in scalar registers, or each load becomes a loop over the lanes' descriptors)
+        const uint32_t bytes = __builtin_amdgcn_readfirstlane(more ? limit : 0u), lo = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)base),
+                       hi = __builtin_amdgcn_readfirstlane((uint32_t)((uintptr_t)base >> 32));
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)((uintptr_t)hi << 32 | lo), 0, (int)bytes, 0x00020000);
+        const bool tail = !ACROSS && k0 + kBK > kend;  // the last step of a depth that is no multiple of 64: chunks beyond it read nothing
+        const uint32_t shift = ACROSS || tail ? 0u : k0 * 2u;
+        uint32_t v = off[i];
+        if (tail) {
+            const uint32_t row = (w * PIECES + i) * 8u + (lane >> 3);
+            const uint32_t kc = ((lane & 7u) ^ swz_row(row)) * 8u;
+            v = k0 + kc < kend ? v + k0 * 2u : 0x7FFFFFF0u;
+        }
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(lds + (w * PIECES + i) * 1024u), 16, v, shift, 0, 0);
+    }
 };
+
+__device__ __forceinline__ void stage_rows(const void* p, uint32_t bytes, uint32_t off, char* lds) {
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)bytes, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, off, 0, 0, 0);
+}
 
 // Fragment of 16 output rows / columns x 32 k (eight k per lane: k = kk * 32 + 8 * (lane / 16) + 0..7), operand along k.
 template <class Frag>
@@ -240,13 +258,13 @@ struct Shape {
     static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, NW = WM_ * WN_;
     static constexpr int MT = TM_ / WM_ / 16, NT = TN_ / WN_ / 16;
     static constexpr int A_BYTES = TM_ * 128, B_BYTES = TN_ * 128, STAGE = A_BYTES + B_BYTES;
-    // row factors, then EPI_LOSS: (maximum, sum) per wave column and row; else 2 KiB per wave
+    // row factors of two tiles, then EPI_LOSS: (maximum, sum) per wave column and row; else 2 KiB per wave
     static constexpr int ROW_BYTES = TM_ * 16;
-    static constexpr int EPI_BYTES = ROW_BYTES + (WN_ * TM_ * 8 > NW * 2048 ? WN_ * TM_ * 8 : NW * 2048);
+    static constexpr int EPI_BYTES = 2 * ROW_BYTES + (WN_ * TM_ * 8 > NW * 2048 ? WN_ * TM_ * 8 : NW * 2048);
     static constexpr int LDS = 2 * STAGE + EPI_BYTES;
 };
-using Large = Shape<256, 256, 2, 4>;   // one workgroup per CU, 148 KiB of LDS
-using Small = Shape<64, 128, 2, 2>;    // 57 KiB: two workgroups per CU
+using Large = Shape<256, 256, 2, 4>;   // one workgroup per CU, 152 KiB of LDS
+using Small = Shape<64, 128, 2, 2>;    // 58 KiB: two workgroups per CU
 
 template <class S, int FORM, int EPI, bool BF16>
 __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
@@ -286,34 +304,55 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
     for (int j = 0; j < S::NT; ++j) ab[j] = B_ACROSS ? across_address<S::TN>((wn * S::NT + j) * 16u, lane) : 0u;
     const uint32_t steps = g.ksteps * g.segs;
     const uint32_t total = ((mine - 1u - tile0) / step + 1u) * steps;
-    uint32_t p = 0, p_tile = tile0, p_seg = 0, p_ks = 0, p_tm, p_tn, p_sp;
-    place(p_tile, p_tm, p_tn, p_sp);
-    const auto prefetch = [&]() {
-        char* st = lds + (p & 1u) * S::STAGE;
-        const uint32_t k0 = (p_sp * g.ksteps + p_ks) * kBK;
-        la.stage(g.a, (g.seg_a >> (4u * p_seg)) & 15u, p_tm * S::TM, k0, g.k, st, w, lane);
-        lb.stage(g.b, (g.seg_b >> (4u * p_seg)) & 15u, p_tn * S::TN, k0, g.k, st + S::A_BYTES, w, lane);
-        ++p;
-        if (++p_ks == g.ksteps) {
-            p_ks = 0;
-            if (++p_seg == g.segs) {
-                p_seg = 0;
-                p_tile += step;
-                if (p_tile < mine) place(p_tile, p_tm, p_tn, p_sp);
+    constexpr bool SOFTMAX = FORM == SCORES;
+    char* const row_buffers = lds + 2 * S::STAGE;  // SOFTMAX: the row factors of two tiles
+    uint32_t p = 0, p_tile = tile0, p_seg = 0, p_ks = 0, p_tm, p_tn, p_sp, p_k0, p_parity = 0;
+    const auto open = [&]() {
+        p_k0 = p_sp * g.ksteps * kBK;
+        la.open(g.a, (g.seg_a >> (4u * p_seg)) & 15u, p_tm * S::TM, p_k0, g.k);
+        lb.open(g.b, (g.seg_b >> (4u * p_seg)) & 15u, p_tn * S::TN, p_k0, g.k);
+    };
+    const auto prefetch_rows = [&]() {
+        // (beyond the last step the operands have no bytes: the loads bring zeros nobody reads)
+        if (SOFTMAX) {
+            if (p_ks == 0 && p_seg == 0 && w < (uint32_t)S::TM / 64u) {  // (rows beyond the last: zeros)
+                const uint32_t r0 = p_tm * S::TM;
+                stage_rows(g.row + r0, (g.m - r0) * 16u, w * 1024u + lane * 16u, row_buffers + p_parity * S::ROW_BYTES + w * 1024u);
             }
         }
     };
-    prefetch();
-    uint32_t at = 0;
-    for (uint32_t tile = tile0; tile < mine; tile += step) {
+    const auto advance = [&]() {
+        ++p;
+        if (++p_ks < g.ksteps) {
+            p_k0 += kBK;
+            la.advance(g.a, p_k0, g.k);
+            lb.advance(g.b, p_k0, g.k);
+            return;
+        }
+        p_ks = 0;
+        if (++p_seg == g.segs) {
+            p_seg = 0;
+            p_parity ^= 1u;
+            p_tile += step;
+            if (p_tile < mine) place(p_tile, p_tm, p_tn, p_sp);  // (beyond the last tile: the last one's operands, of no bytes)
+        }
+        open();
+    };
+    constexpr int PA = decltype(la)::PIECES, P = PA + decltype(lb)::PIECES;
+    place(p_tile, p_tm, p_tn, p_sp);
+    open();
+    prefetch_rows();
+#pragma unroll
+    for (int x = 0; x < P; ++x) {
+        if (x < PA) la.piece(x, p < total, p_k0, g.k, lds, w, lane);
+        else lb.piece(x - PA, p < total, p_k0, g.k, lds + S::A_BYTES, w, lane);
+    }
+    advance();
+    const float wsc = SOFTMAX && g.wsc ? *g.wsc : 1.f;
+    uint32_t at = 0, parity = 0;
+    for (uint32_t tile = tile0; tile < mine; tile += step, parity ^= 1u) {
         uint32_t tm, tn, sp;
         place(tile, tm, tn, sp);
-        // the tile's row factors travel while the product runs
-        constexpr bool SOFTMAX = FORM == SCORES;
-        float4 factors = make_float4(0.f, 0.f, 0.f, __int_as_float(-1));
-        if constexpr (SOFTMAX) {
-            if (threadIdx.x < (uint32_t)S::TM && tm * S::TM + threadIdx.x < g.m) factors = g.row[tm * S::TM + threadIdx.x];
-        }
         f32x4 acc[S::MT][S::NT];
 #pragma unroll
         for (int i = 0; i < S::MT; ++i)
@@ -323,32 +362,42 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();  // stage `at` is whole; nobody reads stage at - 1 any more
             asm volatile("" ::: "memory");
-            if (p < total) prefetch();
+            if (p < total) prefetch_rows();
             const uint32_t stage = (at & 1u) * S::STAGE;
             const char* sa = lds + stage;
             const char* sb = sa + S::A_BYTES;
+            char* next = lds + (S::STAGE - stage);
+            // The next stage's loads go out one by one between the MFMAs of the step's first half: issued in a row they fill the queue of the
+            // load unit (16 cycles each, 64 of them per CU), and every wave stands in front of its first MFMA until its own are through.
             frag fa[S::MT], fb[S::NT];
             read_fragments<S::TM, S::MT, A_ACROSS, 0>(sa, lds0 + stage, wm * S::MT * 16u, lane, aa, fa);
             read_fragments<S::TN, S::NT, B_ACROSS, 0>(sb, lds0 + stage + S::A_BYTES, wn * S::NT * 16u, lane, ab, fb);
 #pragma unroll
-            for (int i = 0; i < S::MT; ++i)
+            for (int i = 0; i < S::MT; ++i) {
 #pragma unroll
                 for (int j = 0; j < S::NT; ++j) acc[i][j] = H::mma(fb[j], fa[i], acc[i][j]);
+                __builtin_amdgcn_sched_barrier(0x104);  // (scalar instructions and LDS reads may pass)
+#pragma unroll
+                for (int x = i * P / S::MT; x < (i + 1) * P / S::MT; ++x) {
+                    if (x < PA) la.piece(x, p < total, p_k0, g.k, next, w, lane);
+                    else lb.piece(x - PA, p < total, p_k0, g.k, next + S::A_BYTES, w, lane);
+                }
+                __builtin_amdgcn_sched_barrier(0x104);
+            }
             read_fragments<S::TM, S::MT, A_ACROSS, 1>(sa, lds0 + stage, wm * S::MT * 16u, lane, aa, fa);
             read_fragments<S::TN, S::NT, B_ACROSS, 1>(sb, lds0 + stage + S::A_BYTES, wn * S::NT * 16u, lane, ab, fb);
 #pragma unroll
             for (int i = 0; i < S::MT; ++i)
 #pragma unroll
                 for (int j = 0; j < S::NT; ++j) acc[i][j] = H::mma(fb[j], fa[i], acc[i][j]);
+            if (p < total) advance();
         }
         // lane: row (lane & 15) of a 16 x 16 block, columns 4 * (lane / 16) + 0..3
         const uint32_t row0 = tm * S::TM + wm * S::MT * 16u + (lane & 15u);
         const uint32_t c0 = tn * S::TN + wn * S::NT * 16u, cl = c0 + (lane >> 4) * 4u;
-        char* scratch = lds + 2 * S::STAGE + S::ROW_BYTES + w * 2048u;
+        char* scratch = lds + 2 * S::STAGE + 2 * S::ROW_BYTES + w * 2048u;
         if constexpr (SOFTMAX) {
-            float4* rows = reinterpret_cast<float4*>(lds + 2 * S::STAGE);
-            if (threadIdx.x < (uint32_t)S::TM) rows[threadIdx.x] = factors;
-            const float wsc = g.wsc ? *g.wsc : 1.f;
+            const float4* rows = reinterpret_cast<const float4*>(row_buffers + parity * S::ROW_BYTES);
             // columns that all exist and have no factor of their own: the common case, with fewer instructions per score (the epilogue's
             // vector instructions are what a product of short rows waits for: 128 scores per lane)
             const bool plain = !g.h && !g.keys && c0 + S::NT * 16u <= g.n;
@@ -367,9 +416,8 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                     }
                 }
             }
-            __syncthreads();
             if constexpr (EPI == EPI_LOSS) {
-                float2* red = reinterpret_cast<float2*>(lds + 2 * S::STAGE + S::ROW_BYTES);
+                float2* red = reinterpret_cast<float2*>(lds + 2 * S::STAGE + 2 * S::ROW_BYTES);
                 float2 ms[S::MT];  // of this lane's 16 columns
 #pragma unroll
                 for (int i = 0; i < S::MT; ++i) {
@@ -393,7 +441,7 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                         for (int j = 0; j < S::NT; ++j)
 #pragma unroll
                             for (int r = 0; r < 4; ++r)
-                                if (lab == j * 16u + r) g.zlab[row0 + i * 16u] = acc[i][j][r];
+                                if (lab == j * 16u + r && row0 + i * 16u < g.m) g.zlab[row0 + i * 16u] = acc[i][j][r];
                     }
                     const float base = top == -__builtin_inff() ? 0.f : top;
 #pragma unroll
@@ -552,6 +600,7 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
             }
         }
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the loads beyond the last step: LDS is given back with nothing on its way into it)
 }
 
 }  // namespace learn
