@@ -47,6 +47,7 @@ struct QueryPrep {
     const uint64_t* keys;          // labels of removed members too
     float scale;
     uint32_t cosine, bf, raw;      // bf: bf16 operands; raw: planes hold the values themselves (bf16 or f16)
+    bool wide;                     // 16-byte aligned rows
     uint16_t* planes;              // nullptr: read in place
     uint32_t nplanes;
     uint64_t plane;
@@ -68,14 +69,37 @@ __device__ __forceinline__ int32_t exponent_of(float x) {  // x < 2^e (0, infini
     return e;
 }
 
-__device__ __forceinline__ void put_planes(uint16_t* to, uint64_t plane, uint32_t nplanes, bool bf, float x) {
-    if (bf) {
-        *to = to_half<true>(x);
-        return;
+// eight consecutive values of a row into its planes
+__device__ __forceinline__ void put_planes(uint16_t* to, uint64_t plane, uint32_t nplanes, bool bf, const float (&x)[8]) {
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        if (bf) {
+            hi[r] = (uint32_t)to_half<true>(x[2 * r]) | (uint32_t)to_half<true>(x[2 * r + 1]) << 16;
+            lo[r] = 0;
+        } else {
+            const uint16_t a = to_half<false>(x[2 * r]), b = to_half<false>(x[2 * r + 1]);
+            hi[r] = (uint32_t)a | (uint32_t)b << 16;
+            lo[r] = (uint32_t)to_half<false>(x[2 * r] - from_half<false>(a)) | (uint32_t)to_half<false>(x[2 * r + 1] - from_half<false>(b)) << 16;
+        }
     }
-    const uint16_t hi = to_half<false>(x);
-    *to = hi;
-    if (nplanes > 1) to[plane] = to_half<false>(x - from_half<false>(hi));
+    *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    if (nplanes > 1) *reinterpret_cast<uint4*>(to + plane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+}
+// sum of squares and largest |element| of a row, by a wave
+__device__ __forceinline__ void row_extent(const void* p, int scalar, uint64_t at, uint32_t d, bool wide, uint32_t lane, float& ss, float& top) {
+    ss = 0.f, top = 0.f;
+    for (uint32_t k = lane * 8u; k < d; k += 512) {
+        float x[8];
+        load8(p, scalar, at + k, d - k, wide, x);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            ss = fmaf(x[r], x[r], ss);
+            top = fmaxf(top, fabsf(x[r]));
+        }
+    }
+    ss = wave_sum(ss);
+    top = wave_max(top);
 }
 
 // one wave per query: its norm, largest element, factors, and its planes
@@ -83,22 +107,17 @@ __global__ __launch_bounds__(256) void query_prep_kernel(QueryPrep a) {
     const uint32_t lane = threadIdx.x & 63u, i = blockIdx.x * 4u + (threadIdx.x >> 6);
     if (i >= a.n) return;
     float ss = 0.f, top = 0.f;
-    if (a.cosine || !a.raw || a.g) {
-        for (uint32_t k = lane; k < a.d; k += 64) {
-            const float x = load_scalar(a.q, a.scalar, (uint64_t)i * a.ld + k);
-            ss = fmaf(x, x, ss);
-            top = fmaxf(top, fabsf(x));
-        }
-        ss = wave_sum(ss);
-        top = wave_max(top);
-    }
+    if (a.cosine || !a.raw || (a.g && !a.bf)) row_extent(a.q, a.scalar, (uint64_t)i * a.ld, a.d, a.wide, lane, ss, top);
     const float inv = !a.cosine ? 1.f : ss > 0.f ? 1.f / sqrtf(ss) : 0.f;
     const int32_t e = a.raw || a.cosine ? 0 : exponent_of(top);
-    const float mul = a.raw ? 1.f : a.cosine ? inv * 8192.f : ldexpf(1.f, 13 - e);
     if (a.planes) {
-        for (uint32_t k = lane; k < a.dp; k += 64) {
-            float x = k < a.d ? load_scalar(a.q, a.scalar, (uint64_t)i * a.ld + k) : 0.f;
-            if (!a.raw) x = a.cosine ? x * mul : ldexpf(x, 13 - e);
+        for (uint32_t k = lane * 8u; k < a.dp; k += 512) {
+            float x[8];
+            load8(a.q, a.scalar, (uint64_t)i * a.ld + k, k < a.d ? a.d - k : 0u, a.wide, x);
+            if (!a.raw) {
+#pragma unroll
+                for (int r = 0; r < 8; ++r) x[r] = a.cosine ? x[r] * (inv * 8192.f) : ldexpf(x[r], 13 - e);
+            }
             put_planes(a.planes + (uint64_t)i * a.dp + k, a.plane, a.nplanes, a.bf, x);
         }
     }
@@ -137,6 +156,7 @@ struct GradQueries {
     int scalar;
     uint64_t ld;
     uint32_t n, d, dp, cosine, bf, nplanes;
+    bool wide;
     const int32_t *label, *ge, *xe;
     const float* inv;
     float scale;
@@ -165,9 +185,13 @@ __global__ __launch_bounds__(256) void grad_queries_kernel(GradQueries a) {
     const bool on = a.label[i] >= 0 && a.xe[i] != kNoExponent;  // (padding, and queries whose loss nobody asks about)
     const int32_t up = a.bf ? 0 : a.ge[i] - a.top[0] + 13;
     const float inv = a.cosine && !a.bf ? a.inv[i] : 1.f;
-    for (uint32_t k = lane; k < a.dp; k += 64) {
-        float x = on && k < a.d ? load_scalar(a.q, a.scalar, (uint64_t)i * a.ld + k) : 0.f;
-        if (!a.bf) x = ldexpf(x * inv, up);
+    for (uint32_t k = lane * 8u; k < a.dp; k += 512) {
+        float x[8];
+        load8(a.q, a.scalar, (uint64_t)i * a.ld + k, on && k < a.d ? a.d - k : 0u, a.wide, x);
+        if (!a.bf) {
+#pragma unroll
+            for (int r = 0; r < 8; ++r) x[r] = ldexpf(x[r] * inv, up);
+        }
         put_planes(a.planes + (uint64_t)i * a.dp + k, a.plane, a.nplanes, a.bf, x);
     }
 }
@@ -179,20 +203,25 @@ struct RowPrep {
     uint32_t rows, d, dp;
     const uint64_t* keys;  // of the piece
     uint32_t cosine, bf, raw, nplanes;
+    bool wide;
     uint16_t* planes;
     uint64_t plane;
     uint32_t* top;   // bits of the largest |element| of the piece (inner product planes)
     float* wsc;      // 2^(e - 13)
     float* inv;      // 1 / |row|
 };
+template <int SC>
 __global__ __launch_bounds__(256) void rows_top_kernel(RowPrep a) {
     const uint32_t lane = threadIdx.x & 63u;
     float top = 0.f;
     for (uint32_t j = blockIdx.x * 4u + (threadIdx.x >> 6); j < a.rows; j += gridDim.x * 4u) {
         if (a.keys && a.keys[j] == ~0ull) continue;
-        for (uint32_t k = lane; k < a.d; k += 64) {
-            const float x = fabsf(load_scalar(a.w, a.scalar, (uint64_t)j * a.ld + k));
-            if (x < __builtin_inff()) top = fmaxf(top, x);
+        for (uint32_t k = lane * 8u; k < a.d; k += 512) {
+            float x[8];
+            load8(a.w, SC, (uint64_t)j * a.ld + k, a.d - k, a.wide, x);
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                if (fabsf(x[r]) < __builtin_inff()) top = fmaxf(top, fabsf(x[r]));
         }
     }
     __shared__ float red[4];
@@ -203,6 +232,7 @@ __global__ __launch_bounds__(256) void rows_top_kernel(RowPrep a) {
     if (threadIdx.x == 0 && top > 0.f) atomicMax(a.top, __float_as_uint(top));  // (a maximum: the same bits whatever the order)
 }
 // one wave per row of the piece
+template <int SC>
 __global__ __launch_bounds__(256) void rows_planes_kernel(RowPrep a) {
     const uint32_t lane = threadIdx.x & 63u, j = blockIdx.x * 4u + (threadIdx.x >> 6);
     const int32_t e = a.raw || a.cosine ? 0 : exponent_of(__uint_as_float(*a.top));
@@ -211,31 +241,27 @@ __global__ __launch_bounds__(256) void rows_planes_kernel(RowPrep a) {
     const bool live = !(a.keys && a.keys[j] == ~0ull);
     float inv = 1.f;
     if (a.cosine && !a.raw) {
-        float ss = 0.f;
-        for (uint32_t k = lane; k < a.d; k += 64) {
-            const float x = load_scalar(a.w, a.scalar, (uint64_t)j * a.ld + k);
-            ss = fmaf(x, x, ss);
-        }
-        ss = wave_sum(ss);
+        float ss, top;
+        row_extent(a.w, SC, (uint64_t)j * a.ld, a.d, a.wide, lane, ss, top);
         inv = live && ss > 0.f ? 1.f / sqrtf(ss) : 0.f;
         if (lane == 0) a.inv[j] = inv;
     }
-    for (uint32_t k = lane; k < a.dp; k += 64) {
-        float x = live && k < a.d ? load_scalar(a.w, a.scalar, (uint64_t)j * a.ld + k) : 0.f;
-        if (!a.raw) x = a.cosine ? x * (inv * 8192.f) : ldexpf(x, 13 - e);
+    for (uint32_t k = lane * 8u; k < a.dp; k += 512) {
+        float x[8];
+        load8(a.w, SC, (uint64_t)j * a.ld + k, live && k < a.d ? a.d - k : 0u, a.wide, x);
+        if (!a.raw) {
+#pragma unroll
+            for (int r = 0; r < 8; ++r) x[r] = a.cosine ? x[r] * (inv * 8192.f) : ldexpf(x[r], 13 - e);
+        }
         put_planes(a.planes + (uint64_t)j * a.dp + k, a.plane, a.nplanes, a.bf, x);
     }
 }
 // 1 / |row| of a table whose rows are used as they are
-__global__ __launch_bounds__(256) void rows_inverse_norm_kernel(const void* w, int scalar, uint64_t ld, uint32_t rows, uint32_t d, float* inv) {
+__global__ __launch_bounds__(256) void rows_inverse_norm_kernel(const void* w, int scalar, uint64_t ld, uint32_t rows, uint32_t d, bool wide, float* inv) {
     const uint32_t lane = threadIdx.x & 63u, j = blockIdx.x * 4u + (threadIdx.x >> 6);
     if (j >= rows) return;
-    float ss = 0.f;
-    for (uint32_t k = lane; k < d; k += 64) {
-        const float x = load_scalar(w, scalar, (uint64_t)j * ld + k);
-        ss = fmaf(x, x, ss);
-    }
-    ss = wave_sum(ss);
+    float ss, top;
+    row_extent(w, scalar, (uint64_t)j * ld, d, wide, lane, ss, top);
     if (lane == 0) inv[j] = ss > 0.f ? 1.f / sqrtf(ss) : 0.f;
 }
 __global__ void fill_words_kernel(uint32_t* p, uint32_t v, uint32_t n) {
@@ -281,7 +307,13 @@ __global__ __launch_bounds__(256) void query_join_kernel(QueryJoin a) {
     float dot = 0.f;
     for (uint32_t k = threadIdx.x; k < a.d; k += 256) {
         float s = 0.f;
-        for (uint32_t x = 0; x < a.splits; ++x) s += a.part[((size_t)x * a.n + i) * a.dn + k];
+        for (uint32_t x0 = 0; x0 < a.splits; x0 += 16) {  // (sixteen loads on their way at a time)
+            float v[16];
+#pragma unroll
+            for (uint32_t x = 0; x < 16; ++x) v[x] = x0 + x < a.splits ? a.part[((size_t)(x0 + x) * a.n + i) * a.dn + k] : 0.f;
+#pragma unroll
+            for (uint32_t x = 0; x < 16; ++x) s += v[x];
+        }
         s *= wsc;
         if (!a.first) s += a.acc[(size_t)i * a.dn + k];
         if (a.last && !a.cosine) {
@@ -537,6 +569,7 @@ struct Call {  // what the two calls share
         a.keys = p.w.keys;
         a.scale = q.scale;
         a.cosine = p.cosine, a.bf = p.bf, a.raw = p.raw;
+        a.wide = wide_rows(a.q, a.scalar, a.ld);
         a.planes = p.q_in_place ? nullptr : at<uint16_t>(p.o_qplanes);
         a.nplanes = p.nq;
         a.plane = (uint64_t)p.n * p.dp;
@@ -558,12 +591,21 @@ struct Call {  // what the two calls share
         }
         if (p.raw && p.inv_own) {
             hipLaunchKernelGGL(rows_inverse_norm_kernel, dim3((p.v + 3) / 4), dim3(256), 0, st, p.w.data, p.w.scalar, (uint64_t)p.w.ld, p.v, p.d,
-                               at<float>(p.o_inv));
+                               wide_rows(p.w.data, p.w.scalar, p.w.ld), at<float>(p.o_inv));
             launched("norms");
         }
     }
     const float* h() const { return !p.cosine || !p.raw ? nullptr : p.w.inv ? p.w.inv : at<float>(p.o_inv); }       // score factor of a column
     const float* inv() const { return p.raw && p.w.inv ? p.w.inv : at<float>(p.o_inv); }
+    template <int SC>
+    void launch_rows(const RowPrep& a, dim3 tops, dim3 all) const {
+        if (!p.raw && !p.cosine) {
+            hipLaunchKernelGGL((rows_top_kernel<SC>), tops, dim3(256), 0, st, a);
+            launched("rows");
+        }
+        hipLaunchKernelGGL((rows_planes_kernel<SC>), all, dim3(256), 0, st, a);
+        launched("rows");
+    }
     // the piece's rows as an operand
     Operand rows(uint32_t x, uint32_t first, uint32_t count) const {
         const char* data = p.w.data + (size_t)first * p.w.ld * size_of(p.w.scalar);
@@ -580,12 +622,13 @@ struct Call {  // what the two calls share
         a.top = at<uint32_t>(p.o_top) + x;
         a.wsc = at<float>(p.o_wsc) + x;
         a.inv = p.cosine && !p.raw ? at<float>(p.o_inv) + first : nullptr;
-        if (!p.raw && !p.cosine) {
-            hipLaunchKernelGGL(rows_top_kernel, dim3(std::min<uint32_t>(512, (count + 3) / 4)), dim3(256), 0, st, a);
-            launched("rows");
+        a.wide = wide_rows(a.w, a.scalar, a.ld);
+        const dim3 tops(std::min<uint32_t>(512, (count + 3) / 4)), all((count + 3) / 4);
+        switch (p.w.scalar) {
+            case VS_SCALAR_F32: launch_rows<SC_F32>(a, tops, all); break;
+            case VS_SCALAR_F16: launch_rows<SC_F16>(a, tops, all); break;
+            default: launch_rows<SC_BF16>(a, tops, all); break;
         }
-        hipLaunchKernelGGL(rows_planes_kernel, dim3((count + 3) / 4), dim3(256), 0, st, a);
-        launched("rows");
         return Operand{(const char*)a.planes, a.plane * 2, (uint64_t)p.dp * 2, count, p.dp};
     }
     // scores of all queries against a piece: operands and factors
@@ -665,6 +708,7 @@ static void loss_grad(const vs_rows* rows, const vs_softmax* q, const float* d_l
         a.scalar = q->scalar;
         a.ld = q->stride;
         a.n = p.n, a.d = p.d, a.dp = p.dp, a.cosine = p.cosine, a.bf = p.bf, a.nplanes = p.nqg;
+        a.wide = wide_rows(a.q, a.scalar, a.ld);
         a.label = c.at<int32_t>(p.o_label), a.ge = c.at<int32_t>(p.o_ge), a.xe = c.at<int32_t>(p.o_xe);
         a.inv = c.at<float>(p.o_qinv);
         a.scale = q->scale;

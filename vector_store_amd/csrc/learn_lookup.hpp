@@ -60,6 +60,31 @@ __device__ __forceinline__ void store8(void* p, int scalar, uint64_t i, uint32_t
     for (int r = 0; r < 8; ++r)
         if ((uint32_t)r < left) store_scalar(p, scalar, i + r, v[r]);
 }
+// eight values as they lie in memory
+template <int SC>
+__device__ __forceinline__ void unpack8(const uint4* raw, float (&v)[8]) {
+    if constexpr (SC == SC_F32) {
+        const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+#pragma unroll
+        for (int r = 0; r < 8; ++r) v[r] = __uint_as_float(w[r]);
+    } else {
+        const uint32_t w[4] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w};
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[2 * r] = from_half<SC == SC_BF16>((uint16_t)w[r]), v[2 * r + 1] = from_half<SC == SC_BF16>((uint16_t)(w[r] >> 16));
+    }
+}
+template <int SC>
+__device__ __forceinline__ void pack8(const float (&v)[8], uint4* raw) {
+    if constexpr (SC == SC_F32) {
+        raw[0] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+        raw[1] = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) w[r] = (uint32_t)to_half<SC == SC_BF16>(v[2 * r]) | (uint32_t)to_half<SC == SC_BF16>(v[2 * r + 1]) << 16;
+        raw[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
 inline bool wide_rows(const void* p, int scalar, uint64_t ld) {
     const uint64_t e = scalar == SC_F32 ? 4 : 2;
     return (uintptr_t)p % 16 == 0 && ld * e % 16 == 0;
@@ -118,71 +143,78 @@ inline void launch_zero_rows(void* out, int scalar, uint64_t ld, uint32_t n, uin
 }
 
 // ------------------------------------------------------------------------------------------------ stable sort of (id, t) by id
-// Least significant digit first, kDigit bits a pass.  A wave owns kWaveItems consecutive entries: it counts its digits (first kernel), the
-// counts of all waves are summed up digit by digit (second kernel, one workgroup), and it moves its entries to their places in order (third
-// kernel: entries of one digit keep their order because the lanes of a wave rank themselves by lane number and the waves by position).
-constexpr uint32_t kDigit = 9, kBins = 1u << kDigit, kWaveItems = 1024, kRun = 32;
+// Least significant digit first, up to 10 bits a pass.  A wave owns `items` consecutive entries (256, more beyond a million): it counts its digits (first kernel), a
+// wave per digit turns the counts of all waves into places within the digit (second kernel), and every wave moves its entries there in order
+// (third kernel, which sums the digits' totals up by itself; entries of one digit keep their order because the lanes of a wave rank
+// themselves by lane number and the waves by position).  Up to kSmallSort entries are sorted by one workgroup in one launch instead.
+constexpr uint32_t kMaxDigit = 10, kMaxBins = 1u << kMaxDigit, kRun = 16, kSmallSort = 4096;
 
 struct SortArgs {
     const void* ids;
     uint32_t id_bytes, n, rows;    // ids beyond the rows sort last as `rows`
-    uint32_t first, shift;         // first pass: keys come from ids
+    uint32_t first, shift, digit;  // first pass: keys come from ids
     const uint32_t *key_in, *pos_in;
     uint32_t *key_out, *pos_out;
-    uint32_t* counts;              // [kBins][waves]
-    uint32_t waves;
+    uint32_t* counts;              // [bins][waves], then [bins] totals
+    uint32_t waves, items;
 };
-__device__ __forceinline__ uint32_t sort_key(const SortArgs& a, uint32_t t) {
-    if (!a.first) return a.key_in[t];
-    const int64_t id = load_id(a.ids, a.id_bytes, t);
-    return id >= 0 && id < (int64_t)a.rows ? (uint32_t)id : a.rows;
+__device__ __forceinline__ uint32_t key_of(const void* ids, uint32_t id_bytes, uint32_t rows, uint32_t t) {
+    const int64_t id = load_id(ids, id_bytes, t);
+    return id >= 0 && id < (int64_t)rows ? (uint32_t)id : rows;
+}
+__device__ __forceinline__ uint32_t sort_key(const SortArgs& a, uint32_t t) { return a.first ? key_of(a.ids, a.id_bytes, a.rows, t) : a.key_in[t]; }
+// lanes (of `on`) whose digit is this lane's
+__device__ __forceinline__ uint64_t same_digit(uint32_t digit, uint32_t bits, uint64_t on) {
+    uint64_t same = on;
+    for (uint32_t b = 0; b < bits; ++b) {
+        const uint64_t m = __ballot((digit >> b) & 1u);
+        same &= (digit >> b) & 1u ? m : ~m;
+    }
+    return same;
+}
+__device__ __forceinline__ uint32_t wave_inclusive(uint32_t v, uint32_t lane) {
+    for (uint32_t o = 1; o < 64; o <<= 1) {
+        const uint32_t u = __shfl_up(v, o);
+        v += lane >= o ? u : 0u;
+    }
+    return v;
 }
 __global__ __launch_bounds__(64) void sort_count_kernel(SortArgs a) {
-    __shared__ uint32_t bins[kBins];
-    const uint32_t lane = threadIdx.x, t0 = blockIdx.x * kWaveItems, t1 = min(a.n, t0 + kWaveItems);
-    for (uint32_t b = lane; b < kBins; b += 64) bins[b] = 0;
+    __shared__ uint32_t bins[kMaxBins];
+    const uint32_t lane = threadIdx.x, t0 = blockIdx.x * a.items, t1 = min(a.n, t0 + a.items), nb = 1u << a.digit;
+    for (uint32_t b = lane; b < nb; b += 64) bins[b] = 0;
     __syncthreads();
-    for (uint32_t t = t0 + lane; t < t1; t += 64) atomicAdd(&bins[(sort_key(a, t) >> a.shift) & (kBins - 1)], 1u);
+    for (uint32_t t = t0 + lane; t < t1; t += 64) atomicAdd(&bins[(sort_key(a, t) >> a.shift) & (nb - 1)], 1u);  // (whole numbers: the order does not matter)
     __syncthreads();
-    for (uint32_t b = lane; b < kBins; b += 64) a.counts[(size_t)b * a.waves + blockIdx.x] = bins[b];
+    for (uint32_t b = lane; b < nb; b += 64) a.counts[(size_t)b * a.waves + blockIdx.x] = bins[b];
 }
-// exclusive sums of kBins * waves counts, in place
-__global__ __launch_bounds__(1024) void sort_sums_kernel(uint32_t* counts, uint32_t n) {
-    __shared__ uint32_t part[1024];
-    const uint32_t each = (n + 1023) / 1024, t0 = min(n, threadIdx.x * each), t1 = min(n, t0 + each);
-    uint32_t s = 0;
-    for (uint32_t t = t0; t < t1; ++t) s += counts[t];
-    part[threadIdx.x] = s;
-    __syncthreads();
-    for (uint32_t o = 1; o < 1024; o <<= 1) {
-        const uint32_t add = threadIdx.x >= o ? part[threadIdx.x - o] : 0;
-        __syncthreads();
-        part[threadIdx.x] += add;
-        __syncthreads();
+__global__ __launch_bounds__(256) void sort_places_kernel(SortArgs a) {
+    const uint32_t lane = threadIdx.x & 63u, b = blockIdx.x * 4u + (threadIdx.x >> 6), nb = 1u << a.digit;
+    if (b >= nb) return;
+    uint32_t* c = a.counts + (size_t)b * a.waves;
+    uint32_t at = 0;
+    for (uint32_t w = 0; w < a.waves; w += 64) {
+        const uint32_t v = w + lane < a.waves ? c[w + lane] : 0u, s = wave_inclusive(v, lane);
+        if (w + lane < a.waves) c[w + lane] = at + s - v;
+        at += __shfl(s, 63);
     }
-    uint32_t at = threadIdx.x ? part[threadIdx.x - 1] : 0;
-    for (uint32_t t = t0; t < t1; ++t) {
-        const uint32_t c = counts[t];
-        counts[t] = at;
-        at += c;
-    }
+    if (lane == 0) a.counts[(size_t)nb * a.waves + b] = at;
 }
 __global__ __launch_bounds__(64) void sort_move_kernel(SortArgs a) {
-    __shared__ uint32_t at[kBins];
-    const uint32_t lane = threadIdx.x, t0 = blockIdx.x * kWaveItems, t1 = min(a.n, t0 + kWaveItems);
-    for (uint32_t b = lane; b < kBins; b += 64) at[b] = a.counts[(size_t)b * a.waves + blockIdx.x];
+    __shared__ uint32_t at[kMaxBins];
+    const uint32_t lane = threadIdx.x, t0 = blockIdx.x * a.items, t1 = min(a.n, t0 + a.items), nb = 1u << a.digit;
+    uint32_t before = 0;
+    for (uint32_t b = 0; b < nb; b += 64) {  // (nb: 64 or more)
+        const uint32_t v = a.counts[(size_t)nb * a.waves + b + lane], s = wave_inclusive(v, lane);
+        at[b + lane] = before + s - v + a.counts[(size_t)(b + lane) * a.waves + blockIdx.x];
+        before += __shfl(s, 63);
+    }
     __syncthreads();
     for (uint32_t t = t0; t < t1; t += 64) {
         const bool on = t + lane < t1;
-        const uint32_t key = on ? sort_key(a, t + lane) : 0u, digit = (key >> a.shift) & (kBins - 1);
-        uint64_t same = __ballot(on);
-#pragma unroll
-        for (uint32_t b = 0; b < kDigit; ++b) {
-            const uint64_t m = __ballot((digit >> b) & 1u);
-            same &= (digit >> b) & 1u ? m : ~m;
-        }
-        const uint32_t rank = mbcnt(same);
-        const uint32_t to = on ? at[digit] + rank : 0u;
+        const uint32_t key = on ? sort_key(a, t + lane) : 0u, digit = (key >> a.shift) & (nb - 1);
+        const uint64_t same = same_digit(digit, a.digit, __ballot(on));
+        const uint32_t rank = mbcnt(same), to = on ? at[digit] + rank : 0u;
         __syncthreads();
         if (on && rank == 0) at[digit] += (uint32_t)__popcll(same);
         __syncthreads();
@@ -192,11 +224,90 @@ __global__ __launch_bounds__(64) void sort_move_kernel(SortArgs a) {
         }
     }
 }
+// n <= kSmallSort, one workgroup of 16 waves: the same, with everything in LDS; 4 bits a pass, so that a wave's counts are a lane's.
+// A wave owns 256 entries in 4 rounds of 64.
+struct SmallSortArgs {
+    const void* ids;
+    uint32_t id_bytes, n, rows, bits;
+    uint32_t *key_out, *pos_out;
+    // workgroups behind the first fill the output with zeros meanwhile (zero != 0)
+    uint32_t zero;
+    void* out;
+    int out_scalar;
+    uint64_t out_ld;
+    uint32_t dim, chunks;
+    bool wide_out;
+};
+__global__ __launch_bounds__(1024) void small_sort_kernel(SmallSortArgs a) {
+    __shared__ uint32_t key[2][kSmallSort], pos[2][kSmallSort / 2 + 16];  // (positions: 16 bits each)
+    __shared__ uint32_t count[16][17], base[16];
+    if (blockIdx.x) {
+        const uint64_t total = (uint64_t)a.rows * a.chunks;
+        const float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        for (uint64_t x = (uint64_t)(blockIdx.x - 1) * 1024u + threadIdx.x; x < total; x += (uint64_t)(gridDim.x - 1) * 1024u) {
+            const uint32_t t = (uint32_t)(x / a.chunks), k = (uint32_t)(x - (uint64_t)t * a.chunks) * 8u;
+            store8(a.out, a.out_scalar, (uint64_t)t * a.out_ld + k, a.dim - k, a.wide_out, v);
+        }
+        return;
+    }
+    const uint32_t lane = threadIdx.x & 63u, w = threadIdx.x >> 6;
+    const auto pos16 = [&](int x) { return reinterpret_cast<uint16_t*>(pos[x]); };
+    for (uint32_t t = threadIdx.x; t < a.n; t += 1024) {
+        key[0][t] = key_of(a.ids, a.id_bytes, a.rows, t);
+        pos16(0)[t] = (uint16_t)t;
+    }
+    int from = 0;
+    const uint32_t per = ((a.n + 15u) / 16u + 63u) & ~63u;  // entries of a wave, at most 256
+    const uint32_t t0 = min(a.n, w * per), t1 = min(a.n, t0 + per);
+    for (uint32_t shift = 0; shift < a.bits; shift += 4, from ^= 1) {
+        if (threadIdx.x < 256) count[threadIdx.x >> 4][threadIdx.x & 15u] = 0;
+        __syncthreads();
+        uint32_t rank[4], dig[4];
+#pragma unroll
+        for (uint32_t r = 0; r < 4; ++r) {
+            const uint32_t t = t0 + r * 64u + lane;
+            const bool on = t < t1;
+            dig[r] = on ? (key[from][t] >> shift) & 15u : 0u;
+            const uint64_t same = same_digit(dig[r], 4, __ballot(on));
+            rank[r] = 0;
+            if (on) rank[r] = count[w][dig[r]] + mbcnt(same);  // (the wave's own counters, one round after the other)
+            __builtin_amdgcn_wave_barrier();
+            if (on && mbcnt(same) == 0) count[w][dig[r]] += (uint32_t)__popcll(same);
+            __builtin_amdgcn_wave_barrier();
+        }
+        __syncthreads();
+        if (threadIdx.x < 16) {  // places of a digit's waves, then of the digits
+            uint32_t s = 0;
+            for (uint32_t x = 0; x < 16; ++x) {
+                const uint32_t c = count[x][threadIdx.x];
+                count[x][threadIdx.x] = s;
+                s += c;
+            }
+            base[threadIdx.x] = s;
+        }
+        __syncthreads();
+        uint32_t below = 0;
+        if (lane < 16)
+            for (uint32_t d = 0; d < lane; ++d) below += base[d];
+#pragma unroll
+        for (uint32_t r = 0; r < 4; ++r) {
+            const uint32_t t = t0 + r * 64u + lane;
+            const uint32_t b = __shfl(below, dig[r]);
+            if (t < t1) {
+                const uint32_t to = b + count[w][dig[r]] + rank[r];
+                key[from ^ 1][to] = key[from][t];
+                pos16(from ^ 1)[to] = pos16(from)[t];
+            }
+        }
+        __syncthreads();
+    }
+    for (uint32_t t = threadIdx.x; t < a.n; t += 1024) a.key_out[t] = key[from][t], a.pos_out[t] = pos16(from)[t];
+}
 
 // ------------------------------------------------------------------------------------------------ sums of the runs
 struct RunArgs {
     const uint32_t *key, *pos;
-    uint32_t n, rows, dim, chunks, runs;
+    uint32_t n, rows, dim, chunks;
     const void* grad;
     int grad_scalar;
     uint64_t grad_ld;
@@ -219,39 +330,64 @@ __device__ __forceinline__ void finish_row(const RunArgs& a, uint32_t row, uint3
     }
     store8(a.out, a.out_scalar, (uint64_t)row * a.out_ld + k, a.dim - k, a.wide_out, v);
 }
-// one workgroup per run; a thread owns 8 columns and goes through the run's entries
-__global__ __launch_bounds__(256) void run_sums_kernel(RunArgs a) {
-    __shared__ uint32_t key[kRun], pos[kRun];
-    __shared__ uint32_t before, after;  // ids on both sides of the run
-    const uint32_t t0 = blockIdx.x * kRun, m = min(kRun, a.n - t0);
-    if (threadIdx.x < m) key[threadIdx.x] = a.key[t0 + threadIdx.x], pos[threadIdx.x] = a.pos[t0 + threadIdx.x];
-    if (threadIdx.x == 64) before = t0 ? a.key[t0 - 1] : ~0u;
-    if (threadIdx.x == 65) after = t0 + m < a.n ? a.key[t0 + m] : ~0u;
-    __syncthreads();
-    for (uint32_t c = threadIdx.x; c < a.chunks; c += 256) {
+// A thread owns 8 columns of a run; its entries' rows are all asked for before the first is summed (a run of kRun rows in the registers: the
+// sums wait for memory once).  Short rows: several runs per workgroup.
+template <int SC>
+__global__ __launch_bounds__(256) void run_sums_kernel(RunArgs a, uint32_t runs, uint32_t per_group, uint32_t lanes) {
+    const uint32_t sub = threadIdx.x / lanes, run = blockIdx.x * per_group + sub;
+    if (sub >= per_group || run >= runs) return;
+    const uint32_t t0 = run * kRun, m = min(kRun, a.n - t0);
+    uint32_t key[kRun + 1], pos[kRun];
+#pragma unroll
+    for (uint32_t t = 0; t < kRun; ++t) key[t] = t < m ? a.key[t0 + t] : ~0u, pos[t] = t < m ? a.pos[t0 + t] : 0u;
+    key[kRun] = t0 + kRun < a.n ? a.key[t0 + kRun] : ~0u;
+    const uint32_t before = t0 ? a.key[t0 - 1] : ~0u;
+    for (uint32_t c = threadIdx.x - sub * lanes; c < a.chunks; c += lanes) {
         const uint32_t k = c * 8u;
-        float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        uint32_t from = 0;
-        for (uint32_t t = 0; t < m; ++t) {
-            const uint32_t id = key[t];
-            if (id >= a.rows) break;  // ids out of range sort last
-            float v[8];
-            load8(a.grad, a.grad_scalar, (uint64_t)pos[t] * a.grad_ld + k, a.dim - k, a.wide_in, v);
+        uint4 raw[kRun][SC == SC_F32 ? 2 : 1];
+        if (a.wide_in && a.dim - k >= 8) {
 #pragma unroll
-            for (int r = 0; r < 8; ++r) s[r] += v[r];
-            const uint32_t next = t + 1 < m ? key[t + 1] : after;
-            if (t + 1 < m && next == id) continue;
-            const bool began = from == 0 && before == id, goes_on = t + 1 == m && next == id;
-            if (began || goes_on) {
-                float* to = a.part + ((size_t)blockIdx.x * 2u + (began ? 0u : 1u)) * (a.chunks * 8u) + k;
-                reinterpret_cast<f32x4*>(to)[0] = f32x4{s[0], s[1], s[2], s[3]};
-                reinterpret_cast<f32x4*>(to)[1] = f32x4{s[4], s[5], s[6], s[7]};
-            } else {
-                finish_row(a, id, k, s);
+            for (uint32_t t = 0; t < kRun; ++t) {  // (ids out of range, and entries beyond the last: the first entry's row)
+                const uint64_t at = (uint64_t)pos[t] * a.grad_ld + k;
+                if constexpr (SC == SC_F32) {
+                    raw[t][0] = reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(a.grad) + at)[0];
+                    raw[t][1] = reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(a.grad) + at)[1];
+                } else {
+                    raw[t][0] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.grad) + at);
+                }
             }
-            from = t + 1;
+        } else {
 #pragma unroll
-            for (int r = 0; r < 8; ++r) s[r] = 0.f;
+            for (uint32_t t = 0; t < kRun; ++t) {
+                float v[8];
+                load8(a.grad, SC, (uint64_t)pos[t] * a.grad_ld + k, a.dim - k, false, v);
+                pack8<SC>(v, raw[t]);
+            }
+        }
+        float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        bool began = key[0] == before;  // the id at hand started in an earlier run
+#pragma unroll
+        for (uint32_t t = 0; t < kRun; ++t) {
+            if (key[t] < a.rows) {  // (ids out of range sort last)
+                const uint32_t id = key[t];
+                float v[8];
+                unpack8<SC>(raw[t], v);
+#pragma unroll
+                for (int r = 0; r < 8; ++r) s[r] += v[r];
+                const bool goes_on = key[t + 1] == id;
+                if (!goes_on || t + 1 == kRun) {
+                    if (began || goes_on) {
+                        float* to = a.part + ((size_t)run * 2u + (began ? 0u : 1u)) * (a.chunks * 8u) + k;
+                        reinterpret_cast<f32x4*>(to)[0] = f32x4{s[0], s[1], s[2], s[3]};
+                        reinterpret_cast<f32x4*>(to)[1] = f32x4{s[4], s[5], s[6], s[7]};
+                    } else {
+                        finish_row(a, id, k, s);
+                    }
+                    began = false;
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) s[r] = 0.f;
+                }
+            }
         }
     }
 }
@@ -262,24 +398,38 @@ __global__ __launch_bounds__(256) void run_join_kernel(RunArgs a) {
     const uint32_t id = a.key[t1 - 1], t0 = blockIdx.x * kRun;
     if (id >= a.rows || a.key[t1] != id) return;
     if (a.key[t0] == id && t0 && a.key[t0 - 1] == id) return;  // it began earlier: that run's workgroup adds up
-    for (uint32_t c = threadIdx.x; c < a.chunks; c += 256) {
+    // the last run the id reaches into: the first one that begins with another id (the keys are sorted) less one
+    uint32_t lo = blockIdx.x + 1, hi = (a.n + kRun - 1) / kRun;
+    while (hi - lo > 1) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (a.key[(size_t)mid * kRun] == id) lo = mid;
+        else hi = mid;
+    }
+    constexpr uint32_t AHEAD = 16;
+    for (uint32_t c = threadIdx.x; c < a.chunks; c += blockDim.x) {
         const uint32_t k = c * 8u, w = a.chunks * 8u;
         const float* p = a.part + ((size_t)blockIdx.x * 2u + 1u) * w + k;
-        float s[8];
+        f32x4 s0 = reinterpret_cast<const f32x4*>(p)[0], s1 = reinterpret_cast<const f32x4*>(p)[1];
+        for (uint32_t x = blockIdx.x + 1; x <= lo; x += AHEAD) {
+            f32x4 h[AHEAD][2];
 #pragma unroll
-        for (int r = 0; r < 8; ++r) s[r] = p[r];
-        for (uint32_t x = blockIdx.x + 1; x * kRun < a.n && a.key[x * kRun] == id; ++x) {
-            const float* h = a.part + (size_t)x * 2u * w + k;
+            for (uint32_t y = 0; y < AHEAD; ++y) {
+                const float* q = a.part + (size_t)min(x + y, lo) * 2u * w + k;
+                h[y][0] = reinterpret_cast<const f32x4*>(q)[0], h[y][1] = reinterpret_cast<const f32x4*>(q)[1];
+            }
 #pragma unroll
-            for (int r = 0; r < 8; ++r) s[r] += h[r];
+            for (uint32_t y = 0; y < AHEAD; ++y)
+                if (x + y <= lo) s0 += h[y][0], s1 += h[y][1];
         }
+        float s[8] = {s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3]};
         finish_row(a, id, k, s);
     }
 }
 
 struct LookupGradLayout {
     size_t key[2], pos[2], counts, part, bytes;
-    uint32_t waves, runs, passes;
+    uint32_t waves, items, runs, passes, digit, bits;
+    bool small;
 };
 inline LookupGradLayout lookup_grad_layout(size_t n, size_t rows, size_t dim) {
     LookupGradLayout l = {};
@@ -289,50 +439,71 @@ inline LookupGradLayout lookup_grad_layout(size_t n, size_t rows, size_t dim) {
         at += (b + 255) & ~(size_t)255;
         return r;
     };
-    l.waves = (uint32_t)((n + kWaveItems - 1) / kWaveItems);
+    l.small = n <= kSmallSort;
+    l.items = (uint32_t)std::max<size_t>(256, ((n + 4095) / 4096 + 63) / 64 * 64);
+    l.waves = (uint32_t)((n + l.items - 1) / l.items);
     l.runs = (uint32_t)((n + kRun - 1) / kRun);
-    uint32_t bits = 1;
-    while (bits < 31 && (rows >> bits)) ++bits;  // keys 0 .. rows
-    l.passes = (bits + kDigit - 1) / kDigit;
-    for (int x = 0; x < 2; ++x) l.key[x] = take(n * 4), l.pos[x] = take(n * 4);
-    l.counts = take((size_t)l.waves * kBins * 4);
+    l.bits = 1;
+    while (l.bits < 31 && (rows >> l.bits)) ++l.bits;  // keys 0 .. rows
+    l.passes = (l.bits + kMaxDigit - 1) / kMaxDigit;
+    l.digit = (l.bits + l.passes - 1) / l.passes;
+    if (l.digit < 6) l.digit = 6;  // (a wave looks at 64 digits at a time)
+    for (int x = 0; x < (l.small ? 1 : 2); ++x) l.key[x] = take(n * 4), l.pos[x] = take(n * 4);
+    l.counts = take(l.small ? 0 : ((size_t)l.waves + 1) * (1u << l.digit) * 4);
     l.part = take((size_t)l.runs * 2 * ((dim + 7) / 8 * 8) * 4);
     l.bytes = at;
     return l;
 }
 inline void launch_lookup_grad(const void* grad, int grad_scalar, uint64_t grad_ld, const void* ids, uint32_t id_bytes, uint32_t n, uint32_t rows, uint32_t dim, float scale,
                                bool accumulate, void* out, int out_scalar, uint64_t out_ld, const LookupGradLayout& l, char* work, hipStream_t st) {
-    if (!accumulate) launch_zero_rows(out, out_scalar, out_ld, rows, dim, st);
+    const uint32_t chunks = (dim + 7) / 8;
+    if (!accumulate && !(l.small && n)) launch_zero_rows(out, out_scalar, out_ld, rows, dim, st);
     if (!n) return;
-    SortArgs s = {};
-    s.ids = ids;
-    s.id_bytes = id_bytes;
-    s.n = n;
-    s.rows = rows;
-    s.counts = (uint32_t*)(work + l.counts);
-    s.waves = l.waves;
     uint32_t to = 0;
-    for (uint32_t pass = 0; pass < l.passes; ++pass, to ^= 1u) {
-        s.first = pass == 0;
-        s.shift = pass * kDigit;
-        s.key_in = (const uint32_t*)(work + l.key[to ^ 1u]), s.pos_in = (const uint32_t*)(work + l.pos[to ^ 1u]);
-        s.key_out = (uint32_t*)(work + l.key[to]), s.pos_out = (uint32_t*)(work + l.pos[to]);
-        hipLaunchKernelGGL(sort_count_kernel, dim3(l.waves), dim3(64), 0, st, s);
-        hipLaunchKernelGGL(sort_sums_kernel, dim3(1), dim3(1024), 0, st, s.counts, l.waves * kBins);
-        hipLaunchKernelGGL(sort_move_kernel, dim3(l.waves), dim3(64), 0, st, s);
+    if (l.small) {
+        SmallSortArgs s = {ids, id_bytes, n, rows, l.bits, (uint32_t*)(work + l.key[0]), (uint32_t*)(work + l.pos[0]), accumulate ? 0u : 1u, out, out_scalar, out_ld, dim, chunks,
+                           wide_rows(out, out_scalar, out_ld)};
+        const uint64_t blocks = ((uint64_t)rows * chunks + 1023) / 1024;
+        hipLaunchKernelGGL(small_sort_kernel, dim3(accumulate ? 1u : 1u + (uint32_t)(blocks < 2048 ? blocks : 2048)), dim3(1024), 0, st, s);
+    } else {
+        SortArgs s = {};
+        s.ids = ids;
+        s.id_bytes = id_bytes;
+        s.n = n;
+        s.rows = rows;
+        s.counts = (uint32_t*)(work + l.counts);
+        s.waves = l.waves;
+        s.items = l.items;
+        s.digit = l.digit;
+        for (uint32_t pass = 0; pass < l.passes; ++pass, to ^= 1u) {
+            s.first = pass == 0;
+            s.shift = pass * l.digit;
+            s.key_in = (const uint32_t*)(work + l.key[to ^ 1u]), s.pos_in = (const uint32_t*)(work + l.pos[to ^ 1u]);
+            s.key_out = (uint32_t*)(work + l.key[to]), s.pos_out = (uint32_t*)(work + l.pos[to]);
+            hipLaunchKernelGGL(sort_count_kernel, dim3(l.waves), dim3(64), 0, st, s);
+            hipLaunchKernelGGL(sort_places_kernel, dim3((1u << l.digit) / 4), dim3(256), 0, st, s);
+            hipLaunchKernelGGL(sort_move_kernel, dim3(l.waves), dim3(64), 0, st, s);
+        }
+        to ^= 1u;
     }
-    to ^= 1u;
     RunArgs r = {};
     r.key = (const uint32_t*)(work + l.key[to]), r.pos = (const uint32_t*)(work + l.pos[to]);
-    r.n = n, r.rows = rows, r.dim = dim, r.chunks = (dim + 7) / 8, r.runs = l.runs;
+    r.n = n, r.rows = rows, r.dim = dim, r.chunks = chunks;
     r.grad = grad, r.grad_scalar = grad_scalar, r.grad_ld = grad_ld;
     r.scale = scale;
     r.accumulate = accumulate;
     r.out = out, r.out_scalar = out_scalar, r.out_ld = out_ld;
     r.part = (float*)(work + l.part);
     r.wide_in = wide_rows(grad, grad_scalar, grad_ld), r.wide_out = wide_rows(out, out_scalar, out_ld);
-    hipLaunchKernelGGL(run_sums_kernel, dim3(l.runs), dim3(256), 0, st, r);
-    hipLaunchKernelGGL(run_join_kernel, dim3(l.runs), dim3(256), 0, st, r);
+    // rows of up to 32 pieces share a workgroup of one wave, longer ones take 128 or 256 threads each
+    const uint32_t threads = chunks <= 64 ? 64 : chunks <= 128 ? 128 : 256, lanes = std::min(chunks, threads), group = threads / lanes;
+    const dim3 grid((l.runs + group - 1) / group);
+    switch (grad_scalar) {
+        case SC_F32: hipLaunchKernelGGL((run_sums_kernel<SC_F32>), grid, dim3(threads), 0, st, r, l.runs, group, lanes); break;
+        case SC_F16: hipLaunchKernelGGL((run_sums_kernel<SC_F16>), grid, dim3(threads), 0, st, r, l.runs, group, lanes); break;
+        default: hipLaunchKernelGGL((run_sums_kernel<SC_BF16>), grid, dim3(threads), 0, st, r, l.runs, group, lanes); break;
+    }
+    if (l.runs > 1) hipLaunchKernelGGL(run_join_kernel, dim3(l.runs - 1), dim3(threads), 0, st, r);
 }
 
 }  // namespace learn
