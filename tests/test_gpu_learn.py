@@ -73,19 +73,24 @@ def reference(q, w, y, gl, scale, cos, dead=None):
     fq, fw = (1 / nq, 1 / nw) if cos else (1.0, 1.0)
     dq, dw = scale * (c @ wu), scale * (c.t() @ qu)
     bq, bw = abs(scale) * (m @ wu.abs()), abs(scale) * (m.t() @ qu.abs())                   # sums of magnitudes
+    every = torch.where(on, gl.abs(), torch.zeros_like(gl))
+    floor = (abs(scale) * every[:, None] * wu.abs().sum(0) * fq, abs(scale) * (every @ qu.abs())[None, :] * (fw if cos else 1.0))  # ... if every p were 1
+    floor = tuple(torch.nan_to_num(x, 0.0, 0.0, 0.0) * (2 if cos else 1) for x in floor)
     eq, ew = abs(scale) * ((m * ep) @ wu.abs()), abs(scale) * ((m * ep).t() @ qu.abs())     # ... times the probabilities' errors
     if cos:
         dq, dw = (dq - qu * (qu * dq).sum(1, keepdim=True)) * fq, (dw - wu * (wu * dw).sum(1, keepdim=True)) * fw
         (dq, dw) = (torch.nan_to_num(x, 0.0, 0.0, 0.0) for x in (dq, dw))
         along = lambda u, b, f: torch.nan_to_num((b + u.abs() * (u.abs() * b).sum(1, keepdim=True)) * f, 0.0, 0.0, 0.0)  # noqa: E731
         bq, eq, bw, ew = along(qu, bq, fq), along(qu, eq, fq), along(wu, bw, fw), along(wu, ew, fw)
-    return loss, lse, dq, dw, e_loss, e_lse, (bq, eq), (bw, ew)
+    return loss, lse, dq, dw, e_loss, e_lse, (bq, eq, floor[0]), (bw, ew, floor[1])
 
 
-def grad_bound(b, e, want, dtype, terms):
-    """one rounding of the probability and one of each operand (two f16 where the result is f32), the f32 sum, the result's own rounding"""
+def grad_bound(b, e, want, dtype, terms, floor):
+    """one rounding of the probability and one of each operand (two f16 where the result is f32), the f32 sum, the result's own rounding.
+    A probability is held as p * m * 2^15 (1/2 <= m < 1) in f16, whose steps do not get smaller than 2^-24: half a step is 2^-25 * 2^-15 / m <=
+    2^-39 of the loss's gradient, whatever p is, and `floor` is what p = 1 everywhere would add up to."""
     u = 4 * 2.0 ** -22 if dtype == F32 else 3 * U[dtype]
-    return b * (u + min(terms, 4096) * 2.0 ** -24) + e + want.abs() * U[dtype] + 4 * TINY[dtype]
+    return b * (u + min(terms, 4096) * 2.0 ** -24) + e + want.abs() * U[dtype] + 4 * TINY[dtype] + floor * 2.0 ** -39
 
 
 def close(got, want, bound, what):
@@ -105,8 +110,8 @@ def check(q, w, y, gl, scale, metric, rows=None, dead=None):
     close(s1, lse, e_lse, "lse")
     close(l1, loss, e_loss, "loss")
     g1, g2 = learn.softmax_loss_grad(q, src, y, s1, gl, scale, m)
-    close(g1, dq, grad_bound(*bq, dq, q.dtype, w.shape[0]), "dq")
-    close(g2, dw, grad_bound(*bw, dw, w.dtype, q.shape[0]), "dw")
+    close(g1, dq, grad_bound(bq[0], bq[1], dq, q.dtype, w.shape[0], bq[2]), "dq")
+    close(g2, dw, grad_bound(bw[0], bw[1], dw, w.dtype, q.shape[0], bw[2]), "dw")
     a, none = learn.softmax_loss_grad(q, src, y, s1, gl, scale, m, grad_rows=False)
     assert none is None
     none, b = learn.softmax_loss_grad(q, src, y, s1, gl, scale, m, grad_queries=False)
@@ -114,8 +119,8 @@ def check(q, w, y, gl, scale, metric, rows=None, dead=None):
     if q.dtype == w.dtype:  # the same kernels on the same numbers: the same bits
         assert torch.equal(a, g1) and torch.equal(b, g2)
     else:
-        close(a, dq, grad_bound(*bq, dq, q.dtype, w.shape[0]), "dq alone")
-        close(b, dw, grad_bound(*bw, dw, w.dtype, q.shape[0]), "dw alone")
+        close(a, dq, grad_bound(bq[0], bq[1], dq, q.dtype, w.shape[0], bq[2]), "dq alone")
+        close(b, dw, grad_bound(bw[0], bw[1], dw, w.dtype, q.shape[0], bw[2]), "dw alone")
     return l1, s1, g1, g2
 
 

@@ -35,6 +35,10 @@ static void launched(const char* what) { hip_ok(hipGetLastError(), what); }
 // f32's accuracy at three times the f16 product's cost -- the matrix pipe's f32 product costs sixteen.  f16's narrow range is met by
 // powers of two: a query row, the rows of a piece of the table (inner product), or the normalised vector (cosine) is scaled so that its
 // largest element lies in [2^12, 2^13]; what is 2^-36 of the largest is lost.
+// The gradients' products are f16 for every type: the probabilities are numbers this code rounds itself, and in bf16 their rounding would be
+// as large as the result's (measured at 4,096 x 131,072 x 768: 0.0025 of the gradient against 0.0017 for one rounding of the exact one).  One
+// f16 (2^-11) under a bf16 result, two under f16 and f32 ones (the second times 2^11: a probability below f16's normal range keeps its bits);
+// bf16 rows and queries are exact in a scaled f16.
 
 struct QueryPrep {
     const void* q;
@@ -52,11 +56,11 @@ struct QueryPrep {
     uint32_t nplanes;
     uint64_t plane;
     int32_t* label;
-    float4* row;  // the products' factors: (zf, lse2, pf, label)
+    float4* row;  // the products' factors: (zf, lse2, pf 2^-lo, label)
     // backward (g != nullptr)
     const float* g;
     const float* lse;
-    float *df, *inv;
+    float *df, *inv, *lo;
     int32_t *ge, *xe;
 };
 
@@ -107,7 +111,7 @@ __global__ __launch_bounds__(256) void query_prep_kernel(QueryPrep a) {
     const uint32_t lane = threadIdx.x & 63u, i = blockIdx.x * 4u + (threadIdx.x >> 6);
     if (i >= a.n) return;
     float ss = 0.f, top = 0.f;
-    if (a.cosine || !a.raw || (a.g && !a.bf)) row_extent(a.q, a.scalar, (uint64_t)i * a.ld, a.d, a.wide, lane, ss, top);
+    if (a.cosine || !a.raw || a.g) row_extent(a.q, a.scalar, (uint64_t)i * a.ld, a.d, a.wide, lane, ss, top);
     const float inv = !a.cosine ? 1.f : ss > 0.f ? 1.f / sqrtf(ss) : 0.f;
     const int32_t e = a.raw || a.cosine ? 0 : exponent_of(top);
     if (a.planes) {
@@ -128,34 +132,31 @@ __global__ __launch_bounds__(256) void query_prep_kernel(QueryPrep a) {
     const float s2 = a.scale * kLog2e;
     float4 row = make_float4(a.raw ? s2 * inv : a.cosine ? s2 * 0x1p-26f : ldexpf(s2, e - 13), 0.f, 0.f, __int_as_float((int32_t)y));
     if (a.g) {
-        row.y = a.lse[i] * kLog2e;
+        // lse in base-2 units, in two parts: row.y and what its rounding lost, which goes into the factor
+        const float lse = a.lse[i];
+        row.y = lse * kLog2e;
+        const float lo = fabsf(row.y) < __builtin_inff() ? fmaf(lse, kLog2e, -row.y) + lse * kLog2eLo : 0.f;
+        a.lo[i] = lo;
         a.inv[i] = inv;
         const float g = y >= 0 ? a.g[i] : 0.f;
-        if (a.bf) {
-            row.z = g * inv * a.scale;
-            a.df[i] = y >= 0 ? 1.f : 0.f;
-            a.ge[i] = 0;
-            a.xe[i] = 0;
-        } else {
-            // f16 probabilities: (p - [label]) * m * 2^13 with g = m * 2^x, 1/2 <= |m| < 1: below 2^13, and full precision down to p = 2^-26
-            int x = 0;
-            const float m = frexpf(g, &x);
-            row.z = m * 8192.f;
-            a.df[i] = y >= 0 ? ldexpf(a.scale * (a.cosine ? inv * 0x1p-13f : 1.f), x - 13) : 0.f;
-            a.ge[i] = x;
-            a.xe[i] = y < 0 || !(g != 0.f) ? kNoExponent : x + exponent_of(a.cosine ? top * inv : top);
-        }
+        // f16 probabilities: (p - [label]) * m * 2^15 with g = m * 2^x, 1/2 <= |m| < 1: below 2^15, off by at most 2^-11 of themselves or 2^-39
+        int x = 0;
+        const float m = frexpf(g, &x);
+        row.z = m * 32768.f * exp2f(-lo);
+        a.df[i] = y >= 0 ? ldexpf(a.scale * (a.cosine ? inv * 0x1p-13f : 1.f), x - 15) : 0.f;
+        a.ge[i] = x;
+        a.xe[i] = y < 0 || !(g != 0.f) ? kNoExponent : x + exponent_of(a.cosine ? top * inv : top);
     }
     a.row[i] = row;
 }
 
-// The queries as an operand of dw = P^T q: rows of padding are zero whatever they held, and (f16) every row carries the power of two of its
-// loss gradient, relative to the largest.  out: [0] the factor that undoes it.
+// The queries as an operand of dw = P^T q, in f16: rows of padding are zero whatever they held, every other row carries the power of two of its
+// loss gradient, relative to the largest; *wf undoes it.
 struct GradQueries {
     const void* q;
     int scalar;
     uint64_t ld;
-    uint32_t n, d, dp, cosine, bf, nplanes;
+    uint32_t n, d, dp, cosine, nplanes;
     bool wide;
     const int32_t *label, *ge, *xe;
     const float* inv;
@@ -176,23 +177,21 @@ __global__ __launch_bounds__(1024) void grad_exponent_kernel(GradQueries a) {
         for (int x = 1; x < 16; ++x) top = max(top, red[x]);
         if (top == kNoExponent) top = 0;
         a.top[0] = top;
-        a.wf[0] = ldexpf(a.scale, top - 26);
+        a.wf[0] = ldexpf(a.scale, top - 28);
     }
 }
 __global__ __launch_bounds__(256) void grad_queries_kernel(GradQueries a) {
     const uint32_t lane = threadIdx.x & 63u, i = blockIdx.x * 4u + (threadIdx.x >> 6);
     if (i >= a.n) return;
     const bool on = a.label[i] >= 0 && a.xe[i] != kNoExponent;  // (padding, and queries whose loss nobody asks about)
-    const int32_t up = a.bf ? 0 : a.ge[i] - a.top[0] + 13;
-    const float inv = a.cosine && !a.bf ? a.inv[i] : 1.f;
+    const int32_t up = a.ge[i] - a.top[0] + 13;
+    const float inv = a.cosine ? a.inv[i] : 1.f;
     for (uint32_t k = lane * 8u; k < a.dp; k += 512) {
         float x[8];
         load8(a.q, a.scalar, (uint64_t)i * a.ld + k, on && k < a.d ? a.d - k : 0u, a.wide, x);
-        if (!a.bf) {
 #pragma unroll
-            for (int r = 0; r < 8; ++r) x[r] = ldexpf(x[r] * inv, up);
-        }
-        put_planes(a.planes + (uint64_t)i * a.dp + k, a.plane, a.nplanes, a.bf, x);
+        for (int r = 0; r < 8; ++r) x[r] = ldexpf(x[r] * inv, up);
+        put_planes(a.planes + (uint64_t)i * a.dp + k, a.plane, a.nplanes, false, x);
     }
 }
 
@@ -244,7 +243,7 @@ __global__ __launch_bounds__(256) void rows_planes_kernel(RowPrep a) {
         float ss, top;
         row_extent(a.w, SC, (uint64_t)j * a.ld, a.d, a.wide, lane, ss, top);
         inv = live && ss > 0.f ? 1.f / sqrtf(ss) : 0.f;
-        if (lane == 0) a.inv[j] = inv;
+        if (lane == 0 && a.inv) a.inv[j] = inv;
     }
     for (uint32_t k = lane * 8u; k < a.dp; k += 512) {
         float x[8];
@@ -281,9 +280,16 @@ __global__ __launch_bounds__(256) void loss_join_kernel(const float2* part, uint
     __syncthreads();
     if (threadIdx.x) return;
     for (int x = 1; x < 4; ++x) a = join_sums(a, red[x]);
-    const float l2 = a.x + log2f(a.y);
-    lse[i] = l2 * kLn2;
-    loss[i] = label[i] >= 0 ? (l2 - zlab[i]) * kLn2 : 0.f;
+    if (label[i] < 0) {
+        lse[i] = (a.x + log2f(a.y)) * kLn2;
+        loss[i] = 0.f;
+        return;
+    }
+    // a: all columns but the label's
+    const float zy = zlab[i], apart = a.x - zy;
+    const float2 all = join_sums(a, make_float2(zy, 1.f));
+    lse[i] = (all.x + log2f(all.y)) * kLn2;
+    loss[i] = apart < 64.f ? log1pf(a.y * exp2f(apart)) : (apart + log2f(a.y)) * kLn2;
 }
 
 // dq of one query: slices of k in order, pieces in order; after the last piece its factor, the way through the normalisation, the cast
@@ -361,13 +367,15 @@ static void product(ProductArgs g, bool large, bool bf, hipStream_t st) {
     const uint32_t tm = large ? Large::TM : Small::TM, tn = large ? Large::TN : Small::TN;
     g.tiles_m = (g.m + tm - 1) / tm;
     g.tiles_n = (g.n + tn - 1) / tn;
-    if (large) {
-        if (bf) run_product<Large, FORM, EPI, true>(g, st);
-        else run_product<Large, FORM, EPI, false>(g, st);
-    } else {
-        if (bf) run_product<Small, FORM, EPI, true>(g, st);
-        else run_product<Small, FORM, EPI, false>(g, st);
+    if constexpr (FORM == SCORES) {  // (the gradients' products are f16 whatever the types)
+        if (bf) {
+            if (large) run_product<Large, FORM, EPI, true>(g, st);
+            else run_product<Small, FORM, EPI, true>(g, st);
+            return;
+        }
     }
+    if (large) run_product<Large, FORM, EPI, false>(g, st);
+    else run_product<Small, FORM, EPI, false>(g, st);
 }
 // The large tile where it fills the chip: it reads an operand byte per 256 outputs where the small one reads it per 64 / 128.
 static bool use_large(uint64_t m, uint64_t n) { return m > 64 && ((m + 255) / 256) * ((n + 255) / 256) >= 192; }
@@ -444,12 +452,13 @@ struct Plan {
     uint32_t n = 0, v = 0, d = 0, dp = 0;
     bool cosine = false, bf = false, raw = false, q_in_place = false, w_in_place = false, inv_own = false;
     bool grad_q = false, grad_w = false;
-    uint32_t nq = 1, nw = 1, np = 1, nqg = 1;  // planes of the queries, the rows, the probabilities, the queries of dw
+    bool regrow = false;                                // the rows of dq are laid out apart from those of the scores
+    uint32_t nq = 1, nw = 1, np = 1, nqg = 1, nwg = 1;  // planes of the queries, the rows, the probabilities, the queries of dw, the rows of dq
     uint32_t piece = 0, pieces = 0;
     bool large_s = false, large_q = false, large_w = false;
     uint32_t splits = 1, qsteps = 1, tiles_v = 0, trows = 0;
-    size_t o_label, o_row, o_qplanes, o_top, o_wsc, o_inv, o_wplanes, o_part, o_zlab;
-    size_t o_df, o_qinv, o_ge, o_xe, o_exp, o_gplanes, o_prob, o_tpart, o_coef, o_qpart, o_qacc;
+    size_t o_label, o_row, o_qplanes, o_top, o_wsc, o_inv, o_wplanes, o_gwplanes, o_part, o_zlab;
+    size_t o_df, o_qinv, o_lo, o_ge, o_xe, o_exp, o_gplanes, o_prob, o_tpart, o_coef, o_qpart, o_qacc;
     size_t bytes = 0;
 };
 
@@ -482,10 +491,12 @@ static Plan plan(const vs_rows* rows, const vs_softmax* q, bool grad_q, bool gra
     p.grad_q = grad_q;
     p.grad_w = grad_w;
     const bool grad = grad_q || grad_w;
-    p.np = (grad_q && tq == VS_SCALAR_F32) || (grad_w && tw == VS_SCALAR_F32) ? 2 : 1;
-    p.nqg = !p.bf && tw == VS_SCALAR_F32 && p.nq > 1 ? 2 : 1;
+    p.np = (grad_q && tq != VS_SCALAR_BF16) || (grad_w && tw != VS_SCALAR_BF16) ? 2 : 1;
+    p.nqg = tw != VS_SCALAR_BF16 && (p.cosine || tq == VS_SCALAR_F32) ? 2 : 1;
+    p.regrow = p.bf && grad_q;
+    p.nwg = p.regrow ? 1 : p.nw;
     // pieces of the table: one, unless rows are re-laid or probabilities are kept for the two products that read them
-    const size_t per_row = (p.w_in_place ? 0 : (size_t)p.nw * p.dp * 2) + (grad ? (size_t)p.np * n * 2 : 0);
+    const size_t per_row = (p.w_in_place ? 0 : (size_t)p.nw * p.dp * 2) + (p.regrow ? (size_t)p.dp * 2 : 0) + (grad ? (size_t)p.np * n * 2 : 0);
     size_t piece = v;
     if (per_row) piece = std::min<size_t>(v, std::max<size_t>(2048, kPieceBytes / per_row));
     piece = std::min<size_t>(piece, 1u << 20);
@@ -520,12 +531,14 @@ static Plan plan(const vs_rows* rows, const vs_softmax* q, bool grad_q, bool gra
     p.o_wsc = l.take((size_t)p.pieces * 4);
     p.o_inv = l.take(p.inv_own ? (size_t)v * 4 : 0);
     p.o_wplanes = l.take(p.w_in_place ? 0 : (size_t)p.nw * piece * p.dp * 2);
+    p.o_gwplanes = l.take(p.regrow ? piece * p.dp * 2 : 0);
     if (!grad) {
         p.o_part = l.take((size_t)n * p.tiles_v * 8);
         p.o_zlab = l.take((size_t)n * 4);
     } else {
         p.o_df = l.take((size_t)n * 4);
         p.o_qinv = l.take((size_t)n * 4);
+        p.o_lo = l.take((size_t)n * 4);
         p.o_ge = l.take((size_t)n * 4);
         p.o_xe = l.take((size_t)n * 4);
         p.o_exp = l.take(8);
@@ -540,13 +553,14 @@ static Plan plan(const vs_rows* rows, const vs_softmax* q, bool grad_q, bool gra
     return p;
 }
 
+// Which planes are multiplied: (lo hi, hi lo, hi hi) of what there is -- the largest products last, so that the small ones are added to small
+// sums --, or hi hi alone.
 static void plane_pairs(ProductArgs& g, uint32_t na, uint32_t nb, bool all) {
-    // (hi hi, lo hi, hi lo) of what there is; one product only where the result is 16 bits wide
-    g.segs = 1;
+    g.segs = 0;
     g.seg_a = g.seg_b = 0;
-    if (!all) return;
-    if (na > 1) g.seg_a |= 1u << (4 * g.segs++);
-    if (nb > 1) g.seg_b |= 1u << (4 * g.segs++);
+    if (all && na > 1) g.seg_a |= 1u << (4 * g.segs++);
+    if (all && nb > 1) g.seg_b |= 1u << (4 * g.segs++);
+    ++g.segs;
 }
 
 struct Call {  // what the two calls share
@@ -578,14 +592,14 @@ struct Call {  // what the two calls share
         if (g) {
             a.g = g;
             a.lse = lse;
-            a.df = at<float>(p.o_df), a.inv = at<float>(p.o_qinv);
+            a.df = at<float>(p.o_df), a.inv = at<float>(p.o_qinv), a.lo = at<float>(p.o_lo);
             a.ge = at<int32_t>(p.o_ge), a.xe = at<int32_t>(p.o_xe);
         }
         hipLaunchKernelGGL(query_prep_kernel, dim3((p.n + 3) / 4), dim3(256), 0, st, a);
         launched("queries");
     }
     void tables() const {  // once per call, before the pieces
-        if (!p.raw && !p.cosine) {
+        if ((!p.raw || p.regrow) && !p.cosine) {
             hipLaunchKernelGGL(fill_words_kernel, dim3((p.pieces + 255) / 256), dim3(256), 0, st, at<uint32_t>(p.o_top), 0u, p.pieces);
             launched("fill");
         }
@@ -598,38 +612,43 @@ struct Call {  // what the two calls share
     const float* h() const { return !p.cosine || !p.raw ? nullptr : p.w.inv ? p.w.inv : at<float>(p.o_inv); }       // score factor of a column
     const float* inv() const { return p.raw && p.w.inv ? p.w.inv : at<float>(p.o_inv); }
     template <int SC>
-    void launch_rows(const RowPrep& a, dim3 tops, dim3 all) const {
-        if (!p.raw && !p.cosine) {
-            hipLaunchKernelGGL((rows_top_kernel<SC>), tops, dim3(256), 0, st, a);
+    void launch_rows(const RowPrep& a) const {
+        if (!a.raw && !p.cosine) {
+            hipLaunchKernelGGL((rows_top_kernel<SC>), dim3(std::min<uint32_t>(512, (a.rows + 3) / 4)), dim3(256), 0, st, a);
             launched("rows");
         }
-        hipLaunchKernelGGL((rows_planes_kernel<SC>), all, dim3(256), 0, st, a);
+        hipLaunchKernelGGL((rows_planes_kernel<SC>), dim3((a.rows + 3) / 4), dim3(256), 0, st, a);
         launched("rows");
     }
-    // the piece's rows as an operand
-    Operand rows(uint32_t x, uint32_t first, uint32_t count) const {
-        const char* data = p.w.data + (size_t)first * p.w.ld * size_of(p.w.scalar);
-        if (p.w_in_place) return Operand{data, 0, p.w.ld * 2, count, p.d};
+    // a piece's rows re-laid: as they are (raw: bf16 or f16), or as f16 planes
+    Operand relay(uint32_t x, uint32_t first, uint32_t count, size_t o_planes, uint32_t nplanes, bool raw) const {
         RowPrep a = {};
-        a.w = data;
+        a.w = p.w.data + (size_t)first * p.w.ld * size_of(p.w.scalar);
         a.scalar = p.w.scalar;
         a.ld = p.w.ld;
         a.rows = count, a.d = p.d, a.dp = p.dp;
         a.keys = p.w.keys ? p.w.keys + first : nullptr;
-        a.cosine = p.cosine, a.bf = p.bf, a.raw = p.raw, a.nplanes = p.nw;
-        a.planes = at<uint16_t>(p.o_wplanes);
+        a.cosine = p.cosine, a.raw = raw, a.bf = raw && p.bf, a.nplanes = nplanes;
+        a.wide = wide_rows(a.w, a.scalar, a.ld);
+        a.planes = at<uint16_t>(o_planes);
         a.plane = (uint64_t)p.piece * p.dp;
         a.top = at<uint32_t>(p.o_top) + x;
         a.wsc = at<float>(p.o_wsc) + x;
         a.inv = p.cosine && !p.raw ? at<float>(p.o_inv) + first : nullptr;
-        a.wide = wide_rows(a.w, a.scalar, a.ld);
-        const dim3 tops(std::min<uint32_t>(512, (count + 3) / 4)), all((count + 3) / 4);
         switch (p.w.scalar) {
-            case VS_SCALAR_F32: launch_rows<SC_F32>(a, tops, all); break;
-            case VS_SCALAR_F16: launch_rows<SC_F16>(a, tops, all); break;
-            default: launch_rows<SC_BF16>(a, tops, all); break;
+            case VS_SCALAR_F32: launch_rows<SC_F32>(a); break;
+            case VS_SCALAR_F16: launch_rows<SC_F16>(a); break;
+            default: launch_rows<SC_BF16>(a); break;
         }
         return Operand{(const char*)a.planes, a.plane * 2, (uint64_t)p.dp * 2, count, p.dp};
+    }
+    // the piece's rows as an operand of the scores; of dq
+    Operand rows(uint32_t x, uint32_t first, uint32_t count) const {
+        if (p.w_in_place) return Operand{p.w.data + (size_t)first * p.w.ld * size_of(p.w.scalar), 0, p.w.ld * 2, count, p.d};
+        return relay(x, first, count, p.o_wplanes, p.nw, p.raw);
+    }
+    Operand grad_rows(const Operand& scores, uint32_t x, uint32_t first, uint32_t count) const {
+        return p.regrow ? relay(x, first, count, p.o_gwplanes, 1, false) : scores;
     }
     // scores of all queries against a piece: operands and factors
     ProductArgs scores(const Operand& w, uint32_t x, uint32_t first, uint32_t count) const {
@@ -707,7 +726,7 @@ static void loss_grad(const vs_rows* rows, const vs_softmax* q, const float* d_l
         a.q = q->d_queries;
         a.scalar = q->scalar;
         a.ld = q->stride;
-        a.n = p.n, a.d = p.d, a.dp = p.dp, a.cosine = p.cosine, a.bf = p.bf, a.nplanes = p.nqg;
+        a.n = p.n, a.d = p.d, a.dp = p.dp, a.cosine = p.cosine, a.nplanes = p.nqg;
         a.wide = wide_rows(a.q, a.scalar, a.ld);
         a.label = c.at<int32_t>(p.o_label), a.ge = c.at<int32_t>(p.o_ge), a.xe = c.at<int32_t>(p.o_xe);
         a.inv = c.at<float>(p.o_qinv);
@@ -716,7 +735,7 @@ static void loss_grad(const vs_rows* rows, const vs_softmax* q, const float* d_l
         a.plane = (uint64_t)p.n * p.dp;
         a.top = c.at<int32_t>(p.o_exp);
         a.wf = c.at<float>(p.o_exp) + 1;
-        if (!p.bf) hipLaunchKernelGGL(grad_exponent_kernel, dim3(1), dim3(1024), 0, st, a);
+        hipLaunchKernelGGL(grad_exponent_kernel, dim3(1), dim3(1024), 0, st, a);
         hipLaunchKernelGGL(grad_queries_kernel, dim3((p.n + 3) / 4), dim3(256), 0, st, a);
         launched("queries");
         gq = Operand{(const char*)a.planes, a.plane * 2, (uint64_t)p.dp * 2, p.n, p.dp};
@@ -726,6 +745,7 @@ static void loss_grad(const vs_rows* rows, const vs_softmax* q, const float* d_l
         const uint32_t first = x * p.piece, count = std::min(p.piece, p.v - first);
         const Operand w = c.rows(x, first, count);
         ProductArgs g = c.scores(w, x, first, count);
+        g.lo = c.at<float>(p.o_lo);
         g.prob = c.at<uint16_t>(p.o_prob);
         g.prob_ld = (count + 7u) & ~7u;
         g.prob_plane = (uint64_t)p.n * g.prob_ld;
@@ -738,17 +758,18 @@ static void loss_grad(const vs_rows* rows, const vs_softmax* q, const float* d_l
         if (d_gq) {
             ProductArgs b = {};
             b.a = prob;
-            b.b = w;
+            b.b = c.grad_rows(w, x, first, count);
             b.m = p.n, b.n = dn, b.k = count;
             b.splits = p.splits;
             b.ksteps = p.qsteps;
-            plane_pairs(b, p.np, p.nw, q->scalar == VS_SCALAR_F32);
+            plane_pairs(b, p.np, p.nwg, q->scalar != VS_SCALAR_BF16);
+            b.lo_first = q->scalar != VS_SCALAR_BF16 && p.np > 1;
             b.out_part = c.at<float>(p.o_qpart);
-            product<DQ, EPI_PART>(b, p.large_q, p.bf, st);
+            product<DQ, EPI_PART>(b, p.large_q, false, st);
             QueryJoin j = {};
             j.part = b.out_part;
             j.splits = p.splits, j.n = p.n, j.d = p.d, j.dn = dn;
-            j.wsc = p.raw || p.cosine ? nullptr : c.at<float>(p.o_wsc) + x;
+            j.wsc = (p.raw && !p.regrow) || p.cosine ? nullptr : c.at<float>(p.o_wsc) + x;
             j.acc = c.at<float>(p.o_qacc);
             j.first = x == 0, j.last = x + 1 == p.pieces, j.cosine = p.cosine;
             j.df = c.at<float>(p.o_df), j.inv = c.at<float>(p.o_qinv);
@@ -770,18 +791,19 @@ static void loss_grad(const vs_rows* rows, const vs_softmax* q, const float* d_l
             b.m = count, b.n = p.d, b.k = p.n;
             b.splits = 1;
             b.ksteps = (p.n + 63) / 64;
-            plane_pairs(b, p.np, p.nqg, p.w.scalar == VS_SCALAR_F32);
+            plane_pairs(b, p.np, p.nqg, p.w.scalar != VS_SCALAR_BF16);
+            b.lo_first = p.w.scalar != VS_SCALAR_BF16 && p.np > 1;
             b.out = (char*)d_gw + (size_t)first * gw_ld * size_of(p.w.scalar);
             b.out_scalar = p.w.scalar;
             b.out_ld = gw_ld;
-            b.wf = p.bf ? nullptr : c.at<float>(p.o_exp) + 1;
-            b.rf = p.cosine && !p.raw ? c.inv() + first : nullptr;
+            b.wf = c.at<float>(p.o_exp) + 1;
+            b.rf = p.cosine ? c.inv() + first : nullptr;
             b.tcoef = p.cosine ? c.at<float>(p.o_coef) : nullptr;
             b.tinv = p.cosine ? c.inv() + first : nullptr;
             b.raw = p.w.data + (size_t)first * p.w.ld * size_of(p.w.scalar);
             b.raw_scalar = p.w.scalar;
             b.raw_ld = p.w.ld;
-            product<DW, EPI_ROWS>(b, p.large_w, p.bf, st);
+            product<DW, EPI_ROWS>(b, p.large_w, false, st);
         }
     }
 }

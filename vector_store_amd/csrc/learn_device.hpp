@@ -7,7 +7,8 @@ namespace learn {
 
 using f32x4 = __attribute__((ext_vector_type(4))) float;
 
-constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
+constexpr float kLog2e = 1.44269504088896340736f, kLog2eLo = 1.9259629911266175e-8f,  // log2(e) = their sum
+                kLn2 = 0.693147180559945309417f;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }  // one instruction; below 2^-126 it returns 0: such a term is nothing beside the 1 of the row's maximum
 

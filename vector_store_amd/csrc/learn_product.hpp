@@ -42,7 +42,8 @@ struct ProductArgs {
     uint32_t splits, ksteps;     // slices of k and 64-deep steps per slice
     uint32_t segs;               // plane pairs
     uint32_t seg_a, seg_b;       // 4 bits each: the planes of pair s
-    // EPI_LOSS / EPI_PROB: z2 = acc * zf * wsc * h[col] (base-2 exponent units); per row (zf, lse2, pf, label as bits)
+    uint32_t lo_first;           // the first pair's a is the probabilities' second plane, which is stored times 2^11
+    // EPI_LOSS / EPI_PROB: z2 = acc * zf * wsc * h[col] (base-2 exponent units); per row (zf, lse2, pf 2^-lo, label as bits)
     const float4* row;
     const float* h;              // nullptr: 1
     const float* wsc;            // nullptr: 1
@@ -52,7 +53,8 @@ struct ProductArgs {
     float2* part;                // [m][part_ld] (maximum, sum of 2^(z2 - maximum)) per column tile
     uint32_t part_ld, part0;
     float* zlab;                 // z2 at the label
-    // EPI_PROB: P = (2^(z2 - lse2) - [label]) * pf[row] * h[col]
+    // EPI_PROB: P = f16((2^(z2 - lse2 - lo) - [label]) * pf), and 2^11 times what that loses; lo: what lse2 lost when it was rounded
+    const float* lo;
     uint16_t* prob;
     uint64_t prob_plane;         // elements
     uint32_t prob_ld, prob_planes;
@@ -363,6 +365,14 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
             __builtin_amdgcn_s_barrier();  // stage `at` is whole; nobody reads stage at - 1 any more
             asm volatile("" ::: "memory");
             if (p < total) prefetch_rows();
+            if constexpr (FORM != SCORES) {
+                if (g.lo_first && s == g.ksteps) {
+#pragma unroll
+                    for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+                        for (int j = 0; j < S::NT; ++j) acc[i][j] *= 0x1p-11f;
+                }
+            }
             const uint32_t stage = (at & 1u) * S::STAGE;
             const char* sa = lds + stage;
             const char* sb = sa + S::A_BYTES;
@@ -424,30 +434,44 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                     const float4 rf = rows[(wm * S::MT + i) * 16u + (lane & 15u)];
                     const float f = rf.x * wsc;
                     const uint32_t lab = (uint32_t)(__float_as_int(rf.w) - (int32_t)g.col0) - cl;
+                    const bool here = __any(lab < S::NT * 16u);  // a label of these rows lies in the wave's columns
+                    // the sum leaves the label out: the loss is log(1 + the others' share), which keeps its accuracy when it is small.
+                    // 2^(acc f - top) in one rounding: what the score itself loses when it is rounded does not enter.
                     float top = -__builtin_inff(), sum = 0.f;
-                    if (plain) {
+                    if (plain && !here) {
+                        float most = acc[i][0][0], least = most;
 #pragma unroll
-                        for (int j = 0; j < S::NT; ++j) acc[i][j] *= f;
+                        for (int j = 0; j < S::NT; ++j)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) most = fmaxf(most, acc[i][j][r]), least = fminf(least, acc[i][j][r]);
+                        top = (f >= 0.f ? most : least) * f;
+                        const float base = top == -__builtin_inff() ? 0.f : top;
+#pragma unroll
+                        for (int j = 0; j < S::NT; ++j)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) sum += exp2_fast(fmaf(acc[i][j][r], f, -base));
                     } else {
 #pragma unroll
                         for (int j = 0; j < S::NT; ++j)
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) acc[i][j][r] = (live[j] >> r) & 1u ? acc[i][j][r] * (f * h[j][r]) : -__builtin_inff();
-                    }
-#pragma unroll
-                    for (int j = 0; j < S::NT; ++j) top = fmaxf(fmaxf(fmaxf(top, acc[i][j][0]), fmaxf(acc[i][j][1], acc[i][j][2])), acc[i][j][3]);
-                    if (__any(lab < S::NT * 16u)) {  // a label of these rows lies in the wave's columns
+                            for (int r = 0; r < 4; ++r) {
+                                const float fh = plain ? f : f * h[j][r], z = acc[i][j][r] * fh;
+                                bool in = plain || ((live[j] >> r) & 1u);
+                                if (lab == j * 16u + r) {
+                                    if (row0 + i * 16u < g.m) g.zlab[row0 + i * 16u] = z;
+                                    in = false;
+                                }
+                                top = in ? fmaxf(top, z) : top;
+                            }
+                        const float base = top == -__builtin_inff() ? 0.f : top;
 #pragma unroll
                         for (int j = 0; j < S::NT; ++j)
 #pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                if (lab == j * 16u + r && row0 + i * 16u < g.m) g.zlab[row0 + i * 16u] = acc[i][j][r];
+                            for (int r = 0; r < 4; ++r) {
+                                const float e = exp2_fast(fmaf(acc[i][j][r], plain ? f : f * h[j][r], -base));
+                                sum += (plain || ((live[j] >> r) & 1u)) && lab != j * 16u + r ? e : 0.f;
+                            }
                     }
-                    const float base = top == -__builtin_inff() ? 0.f : top;
-#pragma unroll
-                    for (int j = 0; j < S::NT; ++j)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) sum += exp2_fast(acc[i][j][r] - base);
                     ms[i] = make_float2(top, sum);
                 }
                 // the four lanes of a row: block pairs swap halves, so that a join serves two blocks of rows at once
@@ -479,9 +503,13 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
             } else {
                 if constexpr (EPI == EPI_PROB_ALONG) {
                     // (a pass of its own, four columns at a time: its sums and the probabilities' stores together do not fit the registers)
-                    float gr[S::MT];
+                    float gr[S::MT], lo[S::MT];
 #pragma unroll
-                    for (int i = 0; i < S::MT; ++i) gr[i] = row0 + i * 16u < g.m ? g.graw[row0 + i * 16u] : 0.f;
+                    for (int i = 0; i < S::MT; ++i) {
+                        const bool has = row0 + i * 16u < g.m;
+                        gr[i] = has ? g.graw[row0 + i * 16u] : 0.f;
+                        lo[i] = has ? g.lo[row0 + i * 16u] : 0.f;
+                    }
 #pragma unroll
                     for (int j = 0; j < S::NT; ++j) {
                         f32x4 t = {0.f, 0.f, 0.f, 0.f};
@@ -493,8 +521,8 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                             asm volatile("" : "+v"(f));  // (or the compiler keeps all 128 probabilities for the next pass)
 #pragma unroll
                             for (int r = 0; r < 4; ++r) {
-                                const float z = acc[i][j][r] * (plain ? f : f * h[j][r]);
-                                const float q = exp2_fast(z - rf.y) - (lab == (uint32_t)r ? 1.f : 0.f);
+                                const float fh = plain ? f : f * h[j][r], z = acc[i][j][r] * fh;
+                                const float q = exp2_fast(fmaf(acc[i][j][r], fh, -rf.y) - lo[i]) - (lab == (uint32_t)r ? 1.f : 0.f);
                                 t[r] += __float_as_int(rf.w) >= 0 && (plain || ((live[j] >> r) & 1u)) ? q * z * gr[i] : 0.f;
                             }
                         }
@@ -526,20 +554,15 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
 #pragma unroll
                         for (int j = 0; j < S::NT; ++j)
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) v[j][r] = (live[j] >> r) & 1u ? exp2_fast(acc[i][j][r] * (f * h[j][r]) - rf.y) : 0.f;
+                            for (int r = 0; r < 4; ++r) v[j][r] = (live[j] >> r) & 1u ? exp2_fast(fmaf(acc[i][j][r], f * h[j][r], -rf.y)) : 0.f;
                     }
                     if (__any(lab < S::NT * 16u)) {
+                        const float one = lab < S::NT * 16u && row0 + i * 16u < g.m ? exp2_fast(g.lo[row0 + i * 16u]) : 1.f;
 #pragma unroll
                         for (int j = 0; j < S::NT; ++j)
 #pragma unroll
                             for (int r = 0; r < 4; ++r)
-                                if (lab == j * 16u + r) v[j][r] -= 1.f;
-                    }
-                    if (g.h) {
-#pragma unroll
-                        for (int j = 0; j < S::NT; ++j)
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) v[j][r] *= h[j][r];
+                                if (lab == j * 16u + r) v[j][r] -= one;
                     }
                     if (__any(label < 0)) {  // padding: whatever its query holds
 #pragma unroll
@@ -552,10 +575,10 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                     for (int j = 0; j < S::NT; ++j) {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) v[j][r] *= rf.z;
-                        hi[j].x = to_half<BF16>(v[j][0]), hi[j].y = to_half<BF16>(v[j][1]), hi[j].z = to_half<BF16>(v[j][2]), hi[j].w = to_half<BF16>(v[j][3]);
+                        hi[j].x = to_half<false>(v[j][0]), hi[j].y = to_half<false>(v[j][1]), hi[j].z = to_half<false>(v[j][2]), hi[j].w = to_half<false>(v[j][3]);
                         if (g.prob_planes > 1) {
-                            lo[j].x = to_half<BF16>(v[j][0] - from_half<BF16>(hi[j].x)), lo[j].y = to_half<BF16>(v[j][1] - from_half<BF16>(hi[j].y));
-                            lo[j].z = to_half<BF16>(v[j][2] - from_half<BF16>(hi[j].z)), lo[j].w = to_half<BF16>(v[j][3] - from_half<BF16>(hi[j].w));
+                            lo[j].x = to_half<false>((v[j][0] - from_half<false>(hi[j].x)) * 2048.f), lo[j].y = to_half<false>((v[j][1] - from_half<false>(hi[j].y)) * 2048.f);
+                            lo[j].z = to_half<false>((v[j][2] - from_half<false>(hi[j].z)) * 2048.f), lo[j].w = to_half<false>((v[j][3] - from_half<false>(hi[j].w)) * 2048.f);
                         }
                     }
                     store_lines(scratch, hi, g.prob, g.prob_ld, row0 - (lane & 15u) + i * 16u, g.m, c0, g.prob_ld, lane);
