@@ -269,6 +269,8 @@ __global__ void fill_words_kernel(uint32_t* p, uint32_t v, uint32_t n) {
 }
 
 // ------------------------------------------------------------------------------------------------ joins
+// natural logarithm of 2^x y, rounded once
+__device__ __forceinline__ float log_sum(float2 a) { return (float)(((double)a.x + log2((double)a.y)) * 0.69314718055994530942); }
 __global__ __launch_bounds__(256) void loss_join_kernel(const float2* part, uint32_t part_ld, uint32_t n, const int32_t* label, const float* zlab,
                                                         float* loss, float* lse) {
     __shared__ float2 red[4];
@@ -281,14 +283,13 @@ __global__ __launch_bounds__(256) void loss_join_kernel(const float2* part, uint
     if (threadIdx.x) return;
     for (int x = 1; x < 4; ++x) a = join_sums(a, red[x]);
     if (label[i] < 0) {
-        lse[i] = (a.x + log2f(a.y)) * kLn2;
+        lse[i] = log_sum(a);
         loss[i] = 0.f;
         return;
     }
     // a: all columns but the label's
     const float zy = zlab[i], apart = a.x - zy;
-    const float2 all = join_sums(a, make_float2(zy, 1.f));
-    lse[i] = (all.x + log2f(all.y)) * kLn2;
+    lse[i] = log_sum(join_sums(a, make_float2(zy, 1.f)));
     loss[i] = apart < 64.f ? log1pf(a.y * exp2f(apart)) : (apart + log2f(a.y)) * kLn2;
 }
 
@@ -462,8 +463,27 @@ struct Plan {
     size_t bytes = 0;
 };
 
-constexpr size_t kPieceBytes = 256ull << 20;    // re-laid rows and probabilities of one piece: what the last-level cache holds
+// Re-laid rows and probabilities of one piece.  A step of 4,096 x 131,072 x 768 took 3.66 / 3.45 / 3.43 / 3.40 ms with 256 / 640 / 1,400 / 2,400 MiB:
+// larger pieces leave fewer CUs without a tile, and what the last-level cache (256 MiB) no longer holds costs about as much.
+constexpr size_t kPieceBytes = 640ull << 20;
 constexpr size_t kSplitBytes = 128ull << 20;    // f32 slices of dq
+
+// Rows per piece, at most `most`.  A workgroup per CU owns 256 x 256 outputs, so 257 tiles take as long as 512: of the sizes allowed, the one
+// whose products leave the fewest CUs idle (in steps of 64 k; a tile's epilogue counts 6, a piece's launches 10).
+static size_t piece_rows(uint64_t n, uint64_t v, uint64_t d, size_t most, bool grad_w) {
+    if (most >= v) return (v + 255) / 256 * 256;
+    const uint64_t tm = (n + 255) / 256, td = (d + 255) / 256, all = (v + 255) / 256;
+    const auto cost = [&](uint64_t c) {
+        return (tm * c + 255) / 256 * ((d + 63) / 64 + 6) + (grad_w ? (c * td + 255) / 256 * ((n + 63) / 64 + 6) : 0) + 10;
+    };
+    const uint64_t top = std::max<uint64_t>(1, most / 256);
+    uint64_t best = top, best_cost = ~0ull;
+    for (uint64_t c = std::max<uint64_t>(1, top / 3); c <= top; ++c) {
+        const uint64_t whole = all / c, rest = all % c, total = whole * cost(c) + (rest ? cost(rest) : 0);
+        if (total <= best_cost) best = c, best_cost = total;
+    }
+    return best * 256;
+}
 
 static Plan plan(const vs_rows* rows, const vs_softmax* q, bool grad_q, bool grad_w) {
     Plan p;
@@ -501,8 +521,7 @@ static Plan plan(const vs_rows* rows, const vs_softmax* q, bool grad_q, bool gra
     if (per_row) piece = std::min<size_t>(v, std::max<size_t>(2048, kPieceBytes / per_row));
     piece = std::min<size_t>(piece, 1u << 20);
     if (piece) {
-        const size_t pieces = (v + piece - 1) / piece;
-        piece = ((v + pieces - 1) / pieces + 255) / 256 * 256;
+        piece = piece_rows(n, v, d, piece, grad_w);
         p.pieces = (uint32_t)((v + piece - 1) / piece);
     }
     p.piece = (uint32_t)piece;

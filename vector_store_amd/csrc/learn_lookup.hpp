@@ -128,18 +128,39 @@ inline void launch_lookup(const void* rows, int scalar, uint64_t ld, uint32_t co
     hipLaunchKernelGGL(lookup_kernel, dim3((uint32_t)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st, a);
 }
 
-__global__ __launch_bounds__(256) void zero_rows_kernel(void* out, int scalar, uint64_t ld, uint32_t n, uint32_t dim, uint32_t chunks, bool wide) {
-    const uint64_t total = (uint64_t)n * chunks;
-    const float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (uint64_t x = (uint64_t)blockIdx.x * 256u + threadIdx.x; x < total; x += (uint64_t)gridDim.x * 256u) {
-        const uint32_t t = (uint32_t)(x / chunks), k = (uint32_t)(x - (uint64_t)t * chunks) * 8u;
-        store8(out, scalar, (uint64_t)t * ld + k, dim - k, wide, v);
+// Zeros.  Rows that follow each other without a gap are one stretch of memory, filled 16 bytes at a time (a division per piece of a row made
+// the fill three times as long); otherwise row by row.
+struct ZeroArgs {
+    void* out;
+    int scalar;
+    uint64_t ld;
+    uint32_t n, dim;
+};
+__device__ __forceinline__ void zero_rows(const ZeroArgs& a, uint64_t worker, uint64_t workers) {
+    const uint32_t e = a.scalar == SC_F32 ? 4u : 2u;
+    char* p = reinterpret_cast<char*>(a.out);
+    if (a.ld == a.dim) {
+        const uint64_t bytes = (uint64_t)a.n * a.dim * e, head = ((16u - ((uintptr_t)p & 15u)) & 15u) < bytes ? (16u - ((uintptr_t)p & 15u)) & 15u : bytes;
+        const uint64_t lines = (bytes - head) / 16u, tail = head + lines * 16u;
+        for (uint64_t x = worker; x < lines; x += workers) reinterpret_cast<uint4*>(p + head)[x] = make_uint4(0u, 0u, 0u, 0u);
+        if (worker < head / e) store_scalar(p, a.scalar, worker, 0.f);
+        if (worker < (bytes - tail) / e) store_scalar(p + tail, a.scalar, worker, 0.f);
+    } else {
+        const uint64_t total = (uint64_t)a.n * a.dim;
+        for (uint64_t x = worker; x < total; x += workers) {
+            const uint32_t t = (uint32_t)(x / a.dim), k = (uint32_t)(x - (uint64_t)t * a.dim);
+            store_scalar(a.out, a.scalar, (uint64_t)t * a.ld + k, 0.f);
+        }
     }
 }
+__global__ __launch_bounds__(256) void zero_rows_kernel(ZeroArgs a) { zero_rows(a, (uint64_t)blockIdx.x * 256u + threadIdx.x, (uint64_t)gridDim.x * 256u); }
+inline uint32_t zero_blocks(const ZeroArgs& a, uint32_t threads) {  // about four stores of 16 bytes per thread
+    const uint64_t per = (uint64_t)threads * 4u * 16u, bytes = (uint64_t)a.n * a.dim * (a.scalar == SC_F32 ? 4u : 2u), blocks = (bytes + per - 1) / per;
+    return (uint32_t)(blocks < 1 ? 1 : blocks < 16384 ? blocks : 16384);
+}
 inline void launch_zero_rows(void* out, int scalar, uint64_t ld, uint32_t n, uint32_t dim, hipStream_t st) {
-    const uint32_t chunks = (dim + 7) / 8;
-    const uint64_t blocks = ((uint64_t)n * chunks + 255) / 256;
-    hipLaunchKernelGGL(zero_rows_kernel, dim3((uint32_t)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st, out, scalar, ld, n, dim, chunks, wide_rows(out, scalar, ld));
+    const ZeroArgs a = {out, scalar, ld, n, dim};
+    hipLaunchKernelGGL(zero_rows_kernel, dim3(zero_blocks(a, 256)), dim3(256), 0, st, a);
 }
 
 // ------------------------------------------------------------------------------------------------ stable sort of (id, t) by id
@@ -230,24 +251,13 @@ struct SmallSortArgs {
     const void* ids;
     uint32_t id_bytes, n, rows, bits;
     uint32_t *key_out, *pos_out;
-    // workgroups behind the first fill the output with zeros meanwhile (zero != 0)
-    uint32_t zero;
-    void* out;
-    int out_scalar;
-    uint64_t out_ld;
-    uint32_t dim, chunks;
-    bool wide_out;
+    ZeroArgs zero;  // workgroups behind the first fill the output with zeros meanwhile
 };
 __global__ __launch_bounds__(1024) void small_sort_kernel(SmallSortArgs a) {
     __shared__ uint32_t key[2][kSmallSort], pos[2][kSmallSort / 2 + 16];  // (positions: 16 bits each)
     __shared__ uint32_t count[16][17], base[16];
     if (blockIdx.x) {
-        const uint64_t total = (uint64_t)a.rows * a.chunks;
-        const float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        for (uint64_t x = (uint64_t)(blockIdx.x - 1) * 1024u + threadIdx.x; x < total; x += (uint64_t)(gridDim.x - 1) * 1024u) {
-            const uint32_t t = (uint32_t)(x / a.chunks), k = (uint32_t)(x - (uint64_t)t * a.chunks) * 8u;
-            store8(a.out, a.out_scalar, (uint64_t)t * a.out_ld + k, a.dim - k, a.wide_out, v);
-        }
+        zero_rows(a.zero, (uint64_t)(blockIdx.x - 1) * 1024u + threadIdx.x, (uint64_t)(gridDim.x - 1) * 1024u);
         return;
     }
     const uint32_t lane = threadIdx.x & 63u, w = threadIdx.x >> 6;
@@ -461,10 +471,8 @@ inline void launch_lookup_grad(const void* grad, int grad_scalar, uint64_t grad_
     if (!n) return;
     uint32_t to = 0;
     if (l.small) {
-        SmallSortArgs s = {ids, id_bytes, n, rows, l.bits, (uint32_t*)(work + l.key[0]), (uint32_t*)(work + l.pos[0]), accumulate ? 0u : 1u, out, out_scalar, out_ld, dim, chunks,
-                           wide_rows(out, out_scalar, out_ld)};
-        const uint64_t blocks = ((uint64_t)rows * chunks + 1023) / 1024;
-        hipLaunchKernelGGL(small_sort_kernel, dim3(accumulate ? 1u : 1u + (uint32_t)(blocks < 2048 ? blocks : 2048)), dim3(1024), 0, st, s);
+        SmallSortArgs s = {ids, id_bytes, n, rows, l.bits, (uint32_t*)(work + l.key[0]), (uint32_t*)(work + l.pos[0]), {out, out_scalar, out_ld, rows, dim}};
+        hipLaunchKernelGGL(small_sort_kernel, dim3(accumulate ? 1u : 1u + std::min(4096u, zero_blocks(s.zero, 1024))), dim3(1024), 0, st, s);
     } else {
         SortArgs s = {};
         s.ids = ids;
