@@ -55,6 +55,8 @@ struct QueryPrep {
     uint16_t* planes;              // nullptr: read in place
     uint32_t nplanes;
     uint64_t plane;
+    uint32_t* tops;                // the pieces' largest elements, zeroed for rows_top_kernel
+    uint32_t pieces;
     int32_t* label;
     float4* row;  // the products' factors: (zf, lse2, pf 2^-lo, label)
     // backward (g != nullptr)
@@ -108,6 +110,8 @@ __device__ __forceinline__ void row_extent(const void* p, int scalar, uint64_t a
 
 // one wave per query: its norm, largest element, factors, and its planes
 __global__ __launch_bounds__(256) void query_prep_kernel(QueryPrep a) {
+    if (blockIdx.x == 0)
+        for (uint32_t x = threadIdx.x; x < a.pieces; x += 256) a.tops[x] = 0;
     const uint32_t lane = threadIdx.x & 63u, i = blockIdx.x * 4u + (threadIdx.x >> 6);
     if (i >= a.n) return;
     float ss = 0.f, top = 0.f;
@@ -166,25 +170,30 @@ struct GradQueries {
     int32_t* top;  // [1]
     float* wf;     // [1]
 };
-__global__ __launch_bounds__(1024) void grad_exponent_kernel(GradQueries a) {
+// (the largest exponent: every workgroup looks for itself where the queries are few, which saves a launch)
+constexpr uint32_t kOwnExponent = 8192;
+__device__ __forceinline__ int32_t grad_exponent(const GradQueries& a) {
     __shared__ int32_t red[16];
     int32_t top = kNoExponent;
-    for (uint32_t i = threadIdx.x; i < a.n; i += 1024) top = max(top, a.xe[i]);
+    for (uint32_t i = threadIdx.x; i < a.n; i += blockDim.x) top = max(top, a.xe[i]);
     for (int o = 32; o; o >>= 1) top = max(top, __shfl_xor(top, o));
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int x = 1; x < 16; ++x) top = max(top, red[x]);
-        if (top == kNoExponent) top = 0;
-        a.top[0] = top;
-        a.wf[0] = ldexpf(a.scale, top - 28);
-    }
+    top = red[0];
+    for (uint32_t x = 1; x < blockDim.x / 64; ++x) top = max(top, red[x]);
+    return top == kNoExponent ? 0 : top;
+}
+__global__ __launch_bounds__(1024) void grad_exponent_kernel(GradQueries a) {
+    const int32_t top = grad_exponent(a);
+    if (threadIdx.x == 0) a.top[0] = top;
 }
 __global__ __launch_bounds__(256) void grad_queries_kernel(GradQueries a) {
+    const int32_t top = a.n <= kOwnExponent ? grad_exponent(a) : a.top[0];
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.wf[0] = ldexpf(a.scale, top - 28);
     const uint32_t lane = threadIdx.x & 63u, i = blockIdx.x * 4u + (threadIdx.x >> 6);
     if (i >= a.n) return;
     const bool on = a.label[i] >= 0 && a.xe[i] != kNoExponent;  // (padding, and queries whose loss nobody asks about)
-    const int32_t up = a.ge[i] - a.top[0] + 13;
+    const int32_t up = a.ge[i] - top + 13;
     const float inv = a.cosine ? a.inv[i] : 1.f;
     for (uint32_t k = lane * 8u; k < a.dp; k += 512) {
         float x[8];
@@ -263,11 +272,6 @@ __global__ __launch_bounds__(256) void rows_inverse_norm_kernel(const void* w, i
     row_extent(w, scalar, (uint64_t)j * ld, d, wide, lane, ss, top);
     if (lane == 0) inv[j] = ss > 0.f ? 1.f / sqrtf(ss) : 0.f;
 }
-__global__ void fill_words_kernel(uint32_t* p, uint32_t v, uint32_t n) {
-    const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x;
-    if (i < n) p[i] = v;
-}
-
 // ------------------------------------------------------------------------------------------------ joins
 // natural logarithm of 2^x y, rounded once
 __device__ __forceinline__ float log_sum(float2 a) { return (float)(((double)a.x + log2((double)a.y)) * 0.69314718055994530942); }
@@ -606,6 +610,8 @@ struct Call {  // what the two calls share
         a.planes = p.q_in_place ? nullptr : at<uint16_t>(p.o_qplanes);
         a.nplanes = p.nq;
         a.plane = (uint64_t)p.n * p.dp;
+        a.tops = at<uint32_t>(p.o_top);
+        a.pieces = p.pieces;
         a.label = at<int32_t>(p.o_label);
         a.row = at<float4>(p.o_row);
         if (g) {
@@ -618,10 +624,6 @@ struct Call {  // what the two calls share
         launched("queries");
     }
     void tables() const {  // once per call, before the pieces
-        if ((!p.raw || p.regrow) && !p.cosine) {
-            hipLaunchKernelGGL(fill_words_kernel, dim3((p.pieces + 255) / 256), dim3(256), 0, st, at<uint32_t>(p.o_top), 0u, p.pieces);
-            launched("fill");
-        }
         if (p.raw && p.inv_own) {
             hipLaunchKernelGGL(rows_inverse_norm_kernel, dim3((p.v + 3) / 4), dim3(256), 0, st, p.w.data, p.w.scalar, (uint64_t)p.w.ld, p.v, p.d,
                                wide_rows(p.w.data, p.w.scalar, p.w.ld), at<float>(p.o_inv));
@@ -754,7 +756,7 @@ static void loss_grad(const vs_rows* rows, const vs_softmax* q, const float* d_l
         a.plane = (uint64_t)p.n * p.dp;
         a.top = c.at<int32_t>(p.o_exp);
         a.wf = c.at<float>(p.o_exp) + 1;
-        hipLaunchKernelGGL(grad_exponent_kernel, dim3(1), dim3(1024), 0, st, a);
+        if (p.n > kOwnExponent) hipLaunchKernelGGL(grad_exponent_kernel, dim3(1), dim3(1024), 0, st, a);
         hipLaunchKernelGGL(grad_queries_kernel, dim3((p.n + 3) / 4), dim3(256), 0, st, a);
         launched("queries");
         gq = Operand{(const char*)a.planes, a.plane * 2, (uint64_t)p.dp * 2, p.n, p.dp};

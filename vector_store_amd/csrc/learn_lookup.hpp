@@ -3,9 +3,9 @@
 // Forward: out[t] = scale * row[id[t]].  Bound by the memory: one 16-byte piece of a row per thread and load.
 //
 // Backward: sums over the t that read a row, in the order of t, without float atomics (two calls give the same bits).  The (id, t) pairs are
-// sorted by id -- stable, so t ascends within an id --, the sorted list is cut into runs of kRun entries, a workgroup sums each run: an id
+// sorted by id -- stable, so t ascends within an id --, the sorted list is cut into runs of 16 or 64 entries, a workgroup sums each run: an id
 // whose entries all lie in one run is written at once, the others leave a partial row at the run's head (the id began earlier) or tail
-// (it goes on), and a second kernel adds those up from the run where the id begins.  An id read n times costs n / kRun serial steps, not n.
+// (it goes on), and a second kernel adds those up from the run where the id begins.  An id read n times costs n / 64 serial steps, not n.
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -168,7 +168,7 @@ inline void launch_zero_rows(void* out, int scalar, uint64_t ld, uint32_t n, uin
 // wave per digit turns the counts of all waves into places within the digit (second kernel), and every wave moves its entries there in order
 // (third kernel, which sums the digits' totals up by itself; entries of one digit keep their order because the lanes of a wave rank
 // themselves by lane number and the waves by position).  Up to kSmallSort entries are sorted by one workgroup in one launch instead.
-constexpr uint32_t kMaxDigit = 10, kMaxBins = 1u << kMaxDigit, kRun = 16, kSmallSort = 4096;
+constexpr uint32_t kMaxDigit = 10, kMaxBins = 1u << kMaxDigit, kBatch = 16, kSmallSort = 4096;
 
 struct SortArgs {
     const void* ids;
@@ -317,7 +317,7 @@ __global__ __launch_bounds__(1024) void small_sort_kernel(SmallSortArgs a) {
 // ------------------------------------------------------------------------------------------------ sums of the runs
 struct RunArgs {
     const uint32_t *key, *pos;
-    uint32_t n, rows, dim, chunks;
+    uint32_t n, rows, dim, chunks, run;
     const void* grad;
     int grad_scalar;
     uint64_t grad_ld;
@@ -340,105 +340,135 @@ __device__ __forceinline__ void finish_row(const RunArgs& a, uint32_t row, uint3
     }
     store8(a.out, a.out_scalar, (uint64_t)row * a.out_ld + k, a.dim - k, a.wide_out, v);
 }
-// A thread owns 8 columns of a run; its entries' rows are all asked for before the first is summed (a run of kRun rows in the registers: the
-// sums wait for memory once).  Short rows: several runs per workgroup.
+// A thread owns 8 columns of a run of kBatch * batches entries; the rows of a batch are all asked for before the first is summed.  Short rows:
+// several runs per workgroup.
 template <int SC>
 __global__ __launch_bounds__(256) void run_sums_kernel(RunArgs a, uint32_t runs, uint32_t per_group, uint32_t lanes) {
     const uint32_t sub = threadIdx.x / lanes, run = blockIdx.x * per_group + sub;
     if (sub >= per_group || run >= runs) return;
-    const uint32_t t0 = run * kRun, m = min(kRun, a.n - t0);
-    uint32_t key[kRun + 1], pos[kRun];
-#pragma unroll
-    for (uint32_t t = 0; t < kRun; ++t) key[t] = t < m ? a.key[t0 + t] : ~0u, pos[t] = t < m ? a.pos[t0 + t] : 0u;
-    key[kRun] = t0 + kRun < a.n ? a.key[t0 + kRun] : ~0u;
-    const uint32_t before = t0 ? a.key[t0 - 1] : ~0u;
+    const uint32_t first = run * a.run, last = min(a.n, first + a.run);
+    const uint32_t before = first ? a.key[first - 1] : ~0u;
     for (uint32_t c = threadIdx.x - sub * lanes; c < a.chunks; c += lanes) {
         const uint32_t k = c * 8u;
-        uint4 raw[kRun][SC == SC_F32 ? 2 : 1];
-        if (a.wide_in && a.dim - k >= 8) {
+        float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        bool began = a.key[first] == before;  // the id at hand started in an earlier run
+        for (uint32_t t0 = first; t0 < last; t0 += kBatch) {
+            const uint32_t m = min(kBatch, a.n - t0);
+            uint32_t key[kBatch + 1], pos[kBatch];
 #pragma unroll
-            for (uint32_t t = 0; t < kRun; ++t) {  // (ids out of range, and entries beyond the last: the first entry's row)
-                const uint64_t at = (uint64_t)pos[t] * a.grad_ld + k;
-                if constexpr (SC == SC_F32) {
-                    raw[t][0] = reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(a.grad) + at)[0];
-                    raw[t][1] = reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(a.grad) + at)[1];
-                } else {
-                    raw[t][0] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.grad) + at);
+            for (uint32_t t = 0; t < kBatch; t += 4) {  // (the lists are laid out in whole batches; what lies behind the last entry is not used)
+                const uint4 x = *reinterpret_cast<const uint4*>(a.key + t0 + t), y = *reinterpret_cast<const uint4*>(a.pos + t0 + t);
+                key[t] = x.x, key[t + 1] = x.y, key[t + 2] = x.z, key[t + 3] = x.w;
+                pos[t] = y.x, pos[t + 1] = y.y, pos[t + 2] = y.z, pos[t + 3] = y.w;
+            }
+#pragma unroll
+            for (uint32_t t = 0; t < kBatch; ++t) {
+                if (t >= m) key[t] = ~0u, pos[t] = 0u;
+            }
+            key[kBatch] = t0 + kBatch < a.n ? a.key[t0 + kBatch] : ~0u;
+            const bool ends = t0 + kBatch >= last;
+            uint4 raw[kBatch][SC == SC_F32 ? 2 : 1];
+            if (a.wide_in && a.dim - k >= 8) {
+#pragma unroll
+                for (uint32_t t = 0; t < kBatch; ++t) {  // (ids out of range: their rows exist too, and are not summed)
+                    const uint64_t at = (uint64_t)pos[t] * a.grad_ld + k;
+                    if constexpr (SC == SC_F32) {
+                        raw[t][0] = reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(a.grad) + at)[0];
+                        raw[t][1] = reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(a.grad) + at)[1];
+                    } else {
+                        raw[t][0] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.grad) + at);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (uint32_t t = 0; t < kBatch; ++t) {
+                    float v[8];
+                    load8(a.grad, SC, (uint64_t)pos[t] * a.grad_ld + k, a.dim - k, false, v);
+                    pack8<SC>(v, raw[t]);
                 }
             }
-        } else {
 #pragma unroll
-            for (uint32_t t = 0; t < kRun; ++t) {
-                float v[8];
-                load8(a.grad, SC, (uint64_t)pos[t] * a.grad_ld + k, a.dim - k, false, v);
-                pack8<SC>(v, raw[t]);
-            }
-        }
-        float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        bool began = key[0] == before;  // the id at hand started in an earlier run
+            for (uint32_t t = 0; t < kBatch; ++t) {
+                if (key[t] < a.rows) {  // (ids out of range sort last)
+                    const uint32_t id = key[t];
+                    float v[8];
+                    unpack8<SC>(raw[t], v);
 #pragma unroll
-        for (uint32_t t = 0; t < kRun; ++t) {
-            if (key[t] < a.rows) {  // (ids out of range sort last)
-                const uint32_t id = key[t];
-                float v[8];
-                unpack8<SC>(raw[t], v);
+                    for (int r = 0; r < 8; ++r) s[r] += v[r];
+                    const bool goes_on = key[t + 1] == id;
+                    if (!goes_on || (ends && t + 1 == kBatch)) {
+                        if (began || goes_on) {
+                            float* to = a.part + ((size_t)run * 2u + (began ? 0u : 1u)) * (a.chunks * 8u) + k;
+                            reinterpret_cast<f32x4*>(to)[0] = f32x4{s[0], s[1], s[2], s[3]};
+                            reinterpret_cast<f32x4*>(to)[1] = f32x4{s[4], s[5], s[6], s[7]};
+                        } else {
+                            finish_row(a, id, k, s);
+                        }
+                        began = false;
 #pragma unroll
-                for (int r = 0; r < 8; ++r) s[r] += v[r];
-                const bool goes_on = key[t + 1] == id;
-                if (!goes_on || t + 1 == kRun) {
-                    if (began || goes_on) {
-                        float* to = a.part + ((size_t)run * 2u + (began ? 0u : 1u)) * (a.chunks * 8u) + k;
-                        reinterpret_cast<f32x4*>(to)[0] = f32x4{s[0], s[1], s[2], s[3]};
-                        reinterpret_cast<f32x4*>(to)[1] = f32x4{s[4], s[5], s[6], s[7]};
-                    } else {
-                        finish_row(a, id, k, s);
+                        for (int r = 0; r < 8; ++r) s[r] = 0.f;
                     }
-                    began = false;
-#pragma unroll
-                    for (int r = 0; r < 8; ++r) s[r] = 0.f;
                 }
             }
         }
     }
 }
-// the run whose last id began in it and goes on: tail + heads of the following runs
-__global__ __launch_bounds__(256) void run_join_kernel(RunArgs a) {
-    const uint32_t t1 = (blockIdx.x + 1) * kRun;
+// The run whose last id began in it and goes on: tail + heads of the following runs.  Groups of `lanes` threads take every per_group-th head,
+// sixteen on their way at a time; their sums are added in the groups' order.
+constexpr uint32_t kJoinThreads = 256;
+__global__ __launch_bounds__(kJoinThreads) void run_join_kernel(RunArgs a, uint32_t per_group, uint32_t lanes) {
+    __shared__ f32x4 sums[kJoinThreads][2];
+    const uint32_t t1 = (blockIdx.x + 1) * a.run;
     if (t1 >= a.n) return;
-    const uint32_t id = a.key[t1 - 1], t0 = blockIdx.x * kRun;
+    const uint32_t id = a.key[t1 - 1], t0 = blockIdx.x * a.run;
     if (id >= a.rows || a.key[t1] != id) return;
     if (a.key[t0] == id && t0 && a.key[t0 - 1] == id) return;  // it began earlier: that run's workgroup adds up
-    // the last run the id reaches into: the first one that begins with another id (the keys are sorted) less one
-    uint32_t lo = blockIdx.x + 1, hi = (a.n + kRun - 1) / kRun;
+    // the last run the id reaches into (the keys are sorted)
+    uint32_t lo = blockIdx.x + 1, hi = (a.n + a.run - 1) / a.run;
+    for (uint32_t s = 1; lo + s < hi; s *= 2) {  // (most reach into the next run only: in growing steps, then by halves)
+        if (a.key[(size_t)(lo + s) * a.run] != id) hi = lo + s;
+        else lo += s;
+    }
     while (hi - lo > 1) {
         const uint32_t mid = lo + (hi - lo) / 2;
-        if (a.key[(size_t)mid * kRun] == id) lo = mid;
+        if (a.key[(size_t)mid * a.run] == id) lo = mid;
         else hi = mid;
     }
     constexpr uint32_t AHEAD = 16;
-    for (uint32_t c = threadIdx.x; c < a.chunks; c += blockDim.x) {
-        const uint32_t k = c * 8u, w = a.chunks * 8u;
-        const float* p = a.part + ((size_t)blockIdx.x * 2u + 1u) * w + k;
-        f32x4 s0 = reinterpret_cast<const f32x4*>(p)[0], s1 = reinterpret_cast<const f32x4*>(p)[1];
-        for (uint32_t x = blockIdx.x + 1; x <= lo; x += AHEAD) {
-            f32x4 h[AHEAD][2];
+    const uint32_t sub = threadIdx.x / lanes, l = threadIdx.x - sub * lanes, w = a.chunks * 8u;
+    for (uint32_t c0 = 0; c0 < a.chunks; c0 += lanes) {
+        const uint32_t k = (c0 + l) * 8u;
+        const bool on = sub < per_group && c0 + l < a.chunks;
+        f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
+        if (on) {
+            for (uint32_t x = blockIdx.x + 1 + sub; x <= lo; x += AHEAD * per_group) {
+                f32x4 h[AHEAD][2];
 #pragma unroll
-            for (uint32_t y = 0; y < AHEAD; ++y) {
-                const float* q = a.part + (size_t)min(x + y, lo) * 2u * w + k;
-                h[y][0] = reinterpret_cast<const f32x4*>(q)[0], h[y][1] = reinterpret_cast<const f32x4*>(q)[1];
+                for (uint32_t y = 0; y < AHEAD; ++y) {
+                    const float* q = a.part + (size_t)min(x + y * per_group, lo) * 2u * w + k;
+                    h[y][0] = reinterpret_cast<const f32x4*>(q)[0], h[y][1] = reinterpret_cast<const f32x4*>(q)[1];
+                }
+#pragma unroll
+                for (uint32_t y = 0; y < AHEAD; ++y)
+                    if (x + y * per_group <= lo) s0 += h[y][0], s1 += h[y][1];
             }
-#pragma unroll
-            for (uint32_t y = 0; y < AHEAD; ++y)
-                if (x + y <= lo) s0 += h[y][0], s1 += h[y][1];
         }
-        float s[8] = {s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3]};
-        finish_row(a, id, k, s);
+        __syncthreads();
+        sums[threadIdx.x][0] = s0, sums[threadIdx.x][1] = s1;
+        __syncthreads();
+        if (on && sub == 0) {
+            const float* p = a.part + ((size_t)blockIdx.x * 2u + 1u) * w + k;
+            s0 = reinterpret_cast<const f32x4*>(p)[0], s1 = reinterpret_cast<const f32x4*>(p)[1];
+            for (uint32_t g = 0; g < per_group; ++g) s0 += sums[g * lanes + l][0], s1 += sums[g * lanes + l][1];
+            float s[8] = {s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3]};
+            finish_row(a, id, k, s);
+        }
     }
 }
 
 struct LookupGradLayout {
     size_t key[2], pos[2], counts, part, bytes;
-    uint32_t waves, items, runs, passes, digit, bits;
+    uint32_t waves, items, run, runs, passes, digit, bits;
     bool small;
 };
 inline LookupGradLayout lookup_grad_layout(size_t n, size_t rows, size_t dim) {
@@ -452,13 +482,15 @@ inline LookupGradLayout lookup_grad_layout(size_t n, size_t rows, size_t dim) {
     l.small = n <= kSmallSort;
     l.items = (uint32_t)std::max<size_t>(256, ((n + 4095) / 4096 + 63) / 64 * 64);
     l.waves = (uint32_t)((n + l.items - 1) / l.items);
-    l.runs = (uint32_t)((n + kRun - 1) / kRun);
+    // short runs keep few ids spread over the chip; long ones leave fewer sums to be joined (131k ids in runs of 16 / 64: 97 + 36 us / 98 + 12 us)
+    l.run = n <= 8192 ? kBatch : 4 * kBatch;
+    l.runs = (uint32_t)((n + l.run - 1) / l.run);
     l.bits = 1;
     while (l.bits < 31 && (rows >> l.bits)) ++l.bits;  // keys 0 .. rows
     l.passes = (l.bits + kMaxDigit - 1) / kMaxDigit;
     l.digit = (l.bits + l.passes - 1) / l.passes;
     if (l.digit < 6) l.digit = 6;  // (a wave looks at 64 digits at a time)
-    for (int x = 0; x < (l.small ? 1 : 2); ++x) l.key[x] = take(n * 4), l.pos[x] = take(n * 4);
+    for (int x = 0; x < (l.small ? 1 : 2); ++x) l.key[x] = take((size_t)l.runs * l.run * 4), l.pos[x] = take((size_t)l.runs * l.run * 4);
     l.counts = take(l.small ? 0 : ((size_t)l.waves + 1) * (1u << l.digit) * 4);
     l.part = take((size_t)l.runs * 2 * ((dim + 7) / 8 * 8) * 4);
     l.bytes = at;
@@ -496,7 +528,7 @@ inline void launch_lookup_grad(const void* grad, int grad_scalar, uint64_t grad_
     }
     RunArgs r = {};
     r.key = (const uint32_t*)(work + l.key[to]), r.pos = (const uint32_t*)(work + l.pos[to]);
-    r.n = n, r.rows = rows, r.dim = dim, r.chunks = chunks;
+    r.n = n, r.rows = rows, r.dim = dim, r.chunks = chunks, r.run = l.run;
     r.grad = grad, r.grad_scalar = grad_scalar, r.grad_ld = grad_ld;
     r.scale = scale;
     r.accumulate = accumulate;
@@ -511,7 +543,8 @@ inline void launch_lookup_grad(const void* grad, int grad_scalar, uint64_t grad_
         case SC_F16: hipLaunchKernelGGL((run_sums_kernel<SC_F16>), grid, dim3(threads), 0, st, r, l.runs, group, lanes); break;
         default: hipLaunchKernelGGL((run_sums_kernel<SC_BF16>), grid, dim3(threads), 0, st, r, l.runs, group, lanes); break;
     }
-    if (l.runs > 1) hipLaunchKernelGGL(run_join_kernel, dim3(l.runs - 1), dim3(threads), 0, st, r);
+    const uint32_t jl = std::min(chunks, kJoinThreads);
+    if (l.runs > 1) hipLaunchKernelGGL(run_join_kernel, dim3(l.runs - 1), dim3(kJoinThreads), 0, st, r, kJoinThreads / jl, jl);
 }
 
 }  // namespace learn
