@@ -236,37 +236,47 @@ struct Half<true> {
 
 // 16 rows x 64 columns of 16-bit values, four consecutive columns of a row per lane and block, to memory as whole 128-byte lines: straight
 // from the registers a store instruction would touch 16 rows in 32-byte pieces (measured: 850 us for 268 MB of probabilities; so 255 us).
-// cols (a multiple of 8) bounds the columns; 16-byte aligned rows.  scratch: 2 KiB of the wave's own.
+// cols (a multiple of 8) bounds the columns; 16-byte aligned rows.  scratch: the wave's own, for ROWS rows at a time.
+template <int ROWS>
 __device__ __forceinline__ void store_lines(char* scratch, const ushort4 (&v)[4], uint16_t* to, uint64_t ld, uint32_t row, uint32_t rows, uint32_t col, uint32_t cols,
                                             uint32_t lane) {
     const uint32_t r = lane & 15u, q = lane >> 4;
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the last block has been read)
 #pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) *reinterpret_cast<ushort4*>(scratch + r * 128u + (((j * 2u + (q >> 1)) ^ (r & 7u)) << 4) + (q & 1u) * 8u) = v[j];
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_wave_barrier();
+    for (uint32_t part = 0; part < 16u / ROWS; ++part) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the last block has been read)
+        if (ROWS == 16 || r / ROWS == part) {
 #pragma unroll
-    for (uint32_t h = 0; h < 2; ++h) {
-        const uint32_t rr = h * 8u + (lane >> 3), c = lane & 7u;
-        const uint4 x = *reinterpret_cast<const uint4*>(scratch + rr * 128u + ((c ^ (rr & 7u)) << 4));
-        if (row + rr < rows && col + c * 8u < cols) *reinterpret_cast<uint4*>(to + (uint64_t)(row + rr) * ld + col + c * 8u) = x;
+            for (uint32_t j = 0; j < 4; ++j)
+                *reinterpret_cast<ushort4*>(scratch + (r % ROWS) * 128u + (((j * 2u + (q >> 1)) ^ (r & 7u)) << 4) + (q & 1u) * 8u) = v[j];
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (uint32_t h = 0; h < ROWS / 8; ++h) {
+            const uint32_t in = h * 8u + (lane >> 3), rr = part * ROWS + in, c = lane & 7u;
+            const uint4 x = *reinterpret_cast<const uint4*>(scratch + in * 128u + ((c ^ (in & 7u)) << 4));
+            if (row + rr < rows && col + c * 8u < cols) *reinterpret_cast<uint4*>(to + (uint64_t)(row + rr) * ld + col + c * 8u) = x;
+        }
+        __builtin_amdgcn_wave_barrier();
     }
-    __builtin_amdgcn_wave_barrier();
 }
 
 // WM x WN waves, each MT x NT blocks of 16 x 16.
-template <int TM_, int TN_, int WM_, int WN_>
+template <int TM_, int TN_, int WM_, int WN_, int RING_>
 struct Shape {
+    static constexpr int RING = RING_;  // stages in LDS: the loads run RING - 1 steps ahead
     static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, NW = WM_ * WN_;
     static constexpr int MT = TM_ / WM_ / 16, NT = TN_ / WN_ / 16;
     static constexpr int A_BYTES = TM_ * 128, B_BYTES = TN_ * 128, STAGE = A_BYTES + B_BYTES;
-    // row factors of two tiles, then EPI_LOSS: (maximum, sum) per wave column and row; else 2 KiB per wave
+    // row factors of RING tiles, then EPI_LOSS: (maximum, sum) per wave column and row; else SCRATCH per wave
     static constexpr int ROW_BYTES = TM_ * 16;
-    static constexpr int EPI_BYTES = 2 * ROW_BYTES + (WN_ * TM_ * 8 > NW * 2048 ? WN_ * TM_ * 8 : NW * 2048);
-    static constexpr int LDS = 2 * STAGE + EPI_BYTES;
+    static constexpr int SCRATCH = RING_ * (STAGE + ROW_BYTES) + NW * 2048 <= 160 * 1024 ? 2048 : 1024;  // of a wave: 16 or 8 rows of 128 bytes
+    static constexpr int EPI_BYTES = RING_ * ROW_BYTES + (WN_ * TM_ * 8 > NW * SCRATCH ? WN_ * TM_ * 8 : NW * SCRATCH);
+    static constexpr int LDS = RING_ * STAGE + EPI_BYTES;
 };
-using Large = Shape<256, 256, 2, 4>;   // one workgroup per CU, 152 KiB of LDS
-using Small = Shape<64, 128, 2, 2>;    // 58 KiB: two workgroups per CU
+using Large = Shape<256, 256, 2, 4, 2>;   // one workgroup per CU, 152 KiB of LDS
+using Medium = Shape<128, 256, 2, 4, 3>;  // one workgroup per CU, 158 KiB
+using Small = Shape<64, 128, 2, 2, 2>;    // 58 KiB: two workgroups per CU
 
 template <class S, int FORM, int EPI, bool BF16>
 __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
@@ -307,7 +317,7 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
     const uint32_t steps = g.ksteps * g.segs;
     const uint32_t total = ((mine - 1u - tile0) / step + 1u) * steps;
     constexpr bool SOFTMAX = FORM == SCORES;
-    char* const row_buffers = lds + 2 * S::STAGE;  // SOFTMAX: the row factors of two tiles
+    char* const row_buffers = lds + S::RING * S::STAGE;  // SOFTMAX: the row factors of RING tiles (a tile may be one step)
     uint32_t p = 0, p_tile = tile0, p_seg = 0, p_ks = 0, p_tm, p_tn, p_sp, p_k0, p_parity = 0;
     const auto open = [&]() {
         p_k0 = p_sp * g.ksteps * kBK;
@@ -317,7 +327,7 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
     const auto prefetch_rows = [&]() {
         // (beyond the last step the operands have no bytes: the loads bring zeros nobody reads)
         if (SOFTMAX) {
-            if (p_ks == 0 && p_seg == 0 && w < (uint32_t)S::TM / 64u) {  // (rows beyond the last: zeros)
+            if (p < total && p_ks == 0 && p_seg == 0 && w < (uint32_t)S::TM / 64u) {  // (rows beyond the last: zeros)
                 const uint32_t r0 = p_tm * S::TM;
                 stage_rows(g.row + r0, (g.m - r0) * 16u, w * 1024u + lane * 16u, row_buffers + p_parity * S::ROW_BYTES + w * 1024u);
             }
@@ -334,7 +344,7 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
         p_ks = 0;
         if (++p_seg == g.segs) {
             p_seg = 0;
-            p_parity ^= 1u;
+            p_parity = p_parity + 1u < (uint32_t)S::RING ? p_parity + 1u : 0u;
             p_tile += step;
             if (p_tile < mine) place(p_tile, p_tm, p_tn, p_sp);  // (beyond the last tile: the last one's operands, of no bytes)
         }
@@ -344,15 +354,21 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
     place(p_tile, p_tm, p_tn, p_sp);
     open();
     prefetch_rows();
+    uint32_t next_at = 0;  // of the stage the next loads go to
 #pragma unroll
-    for (int x = 0; x < P; ++x) {
-        if (x < PA) la.piece(x, p < total, p_k0, g.k, lds, w, lane);
-        else lb.piece(x - PA, p < total, p_k0, g.k, lds + S::A_BYTES, w, lane);
+    for (int st = 0; st < S::RING - 1; ++st) {
+        if (st) prefetch_rows();
+#pragma unroll
+        for (int x = 0; x < P; ++x) {
+            if (x < PA) la.piece(x, p < total, p_k0, g.k, lds + next_at, w, lane);
+            else lb.piece(x - PA, p < total, p_k0, g.k, lds + next_at + S::A_BYTES, w, lane);
+        }
+        advance();
+        next_at += S::STAGE;
     }
-    advance();
     const float wsc = SOFTMAX && g.wsc ? *g.wsc : 1.f;
-    uint32_t at = 0, parity = 0;
-    for (uint32_t tile = tile0; tile < mine; tile += step, parity ^= 1u) {
+    uint32_t stage = 0, parity = 0;
+    for (uint32_t tile = tile0; tile < mine; tile += step, parity = parity + 1u < (uint32_t)S::RING ? parity + 1u : 0u) {
         uint32_t tm, tn, sp;
         place(tile, tm, tn, sp);
         f32x4 acc[S::MT][S::NT];
@@ -360,11 +376,12 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
         for (int i = 0; i < S::MT; ++i)
 #pragma unroll
             for (int j = 0; j < S::NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (uint32_t s = 0; s < steps; ++s, ++at) {
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();  // stage `at` is whole; nobody reads stage at - 1 any more
+        for (uint32_t s = 0; s < steps; ++s) {
+            // (a wave's loads arrive in order: what may still be on its way are the P pieces of the stages after this one)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S::RING - 2) * P) : "memory");
+            __builtin_amdgcn_s_barrier();  // the stage is whole; nobody reads the one before it any more
             asm volatile("" ::: "memory");
-            if (p < total) prefetch_rows();
+            prefetch_rows();
             if constexpr (FORM != SCORES) {
                 if (g.lo_first && s == g.ksteps) {
 #pragma unroll
@@ -373,10 +390,9 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                         for (int j = 0; j < S::NT; ++j) acc[i][j] *= 0x1p-11f;
                 }
             }
-            const uint32_t stage = (at & 1u) * S::STAGE;
             const char* sa = lds + stage;
             const char* sb = sa + S::A_BYTES;
-            char* next = lds + (S::STAGE - stage);
+            char* next = lds + next_at;
             // The next stage's loads go out one by one between the MFMAs of the step's first half: issued in a row they fill the queue of the
             // load unit (16 cycles each, 64 of them per CU), and every wave stands in front of its first MFMA until its own are through.
             frag fa[S::MT], fb[S::NT];
@@ -400,12 +416,14 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
             for (int i = 0; i < S::MT; ++i)
 #pragma unroll
                 for (int j = 0; j < S::NT; ++j) acc[i][j] = H::mma(fb[j], fa[i], acc[i][j]);
-            if (p < total) advance();
+            advance();
+            next_at = stage;
+            stage = stage + S::STAGE < S::RING * S::STAGE ? stage + S::STAGE : 0u;
         }
         // lane: row (lane & 15) of a 16 x 16 block, columns 4 * (lane / 16) + 0..3
         const uint32_t row0 = tm * S::TM + wm * S::MT * 16u + (lane & 15u);
         const uint32_t c0 = tn * S::TN + wn * S::NT * 16u, cl = c0 + (lane >> 4) * 4u;
-        char* scratch = lds + 2 * S::STAGE + 2 * S::ROW_BYTES + w * 2048u;
+        char* scratch = lds + S::RING * (S::STAGE + S::ROW_BYTES) + w * (uint32_t)S::SCRATCH;
         if constexpr (SOFTMAX) {
             const float4* rows = reinterpret_cast<const float4*>(row_buffers + parity * S::ROW_BYTES);
             // columns that all exist and have no factor of their own: the common case, with fewer instructions per score (the epilogue's
@@ -427,7 +445,7 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                 }
             }
             if constexpr (EPI == EPI_LOSS) {
-                float2* red = reinterpret_cast<float2*>(lds + 2 * S::STAGE + 2 * S::ROW_BYTES);
+                float2* red = reinterpret_cast<float2*>(lds + S::RING * (S::STAGE + S::ROW_BYTES));
                 float2 ms[S::MT];  // of this lane's 16 columns
 #pragma unroll
                 for (int i = 0; i < S::MT; ++i) {
@@ -483,6 +501,12 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                     const uint32_t q = lane >> 4, i = (q & 1u) * 2u + (q >> 1);
                     red[wn * S::TM + (wm * S::MT + i) * 16u + (lane & 15u)] = ms[0];
                     red[wn * S::TM + (wm * S::MT + 4u + i) * 16u + (lane & 15u)] = ms[1];
+                } else if constexpr (S::MT == 4) {
+                    ms[0] = join_swapped<32>(ms[0], ms[1]);
+                    ms[1] = join_swapped<32>(ms[2], ms[3]);
+                    ms[0] = join_swapped<16>(ms[0], ms[1]);
+                    const uint32_t q = lane >> 4, i = (q & 1u) * 2u + (q >> 1);
+                    red[wn * S::TM + (wm * S::MT + i) * 16u + (lane & 15u)] = ms[0];
                 } else {
                     static_assert(S::MT == 2, "row blocks per wave");
                     float2 a = join_swapped<32>(ms[0], ms[1]);
@@ -581,8 +605,8 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                             lo[j].z = to_half<false>((v[j][2] - from_half<false>(hi[j].z)) * 2048.f), lo[j].w = to_half<false>((v[j][3] - from_half<false>(hi[j].w)) * 2048.f);
                         }
                     }
-                    store_lines(scratch, hi, g.prob, g.prob_ld, row0 - (lane & 15u) + i * 16u, g.m, c0, g.prob_ld, lane);
-                    if (g.prob_planes > 1) store_lines(scratch, lo, g.prob + g.prob_plane, g.prob_ld, row0 - (lane & 15u) + i * 16u, g.m, c0, g.prob_ld, lane);
+                    store_lines<S::SCRATCH / 128>(scratch, hi, g.prob, g.prob_ld, row0 - (lane & 15u) + i * 16u, g.m, c0, g.prob_ld, lane);
+                    if (g.prob_planes > 1) store_lines<S::SCRATCH / 128>(scratch, lo, g.prob + g.prob_plane, g.prob_ld, row0 - (lane & 15u) + i * 16u, g.m, c0, g.prob_ld, lane);
                     __builtin_amdgcn_sched_barrier(0);  // one block of rows at a time: interleaved, they do not fit the registers
                 }
             }
@@ -619,7 +643,7 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                     if (lines) o[j] = to_half4(g.out_scalar, v);
                     else if (has && c < g.n) store4(g.out, g.out_scalar, (uint64_t)row * g.out_ld + c, v, g.n - c);
                 }
-                if (lines) store_lines(scratch, o, (uint16_t*)g.out, g.out_ld, row0 - (lane & 15u) + i * 16u, g.m, c0, g.n, lane);
+                if (lines) store_lines<S::SCRATCH / 128>(scratch, o, (uint16_t*)g.out, g.out_ld, row0 - (lane & 15u) + i * 16u, g.m, c0, g.n, lane);
             }
         }
     }
