@@ -367,23 +367,41 @@ static void run_product(const ProductArgs& g, hipStream_t st) {
     hipLaunchKernelGGL((product_kernel<S, FORM, EPI, BF>), dim3((uint32_t)std::min<uint64_t>((tiles + 7) / 8 * 8, resident)), dim3(S::NW * 64), S::LDS, st, g);
     launched("product");
 }
-template <int FORM, int EPI>
-static void product(ProductArgs g, bool large, bool bf, hipStream_t st) {
-    const uint32_t tm = large ? Large::TM : Small::TM, tn = large ? Large::TN : Small::TN;
-    g.tiles_m = (g.m + tm - 1) / tm;
-    g.tiles_n = (g.n + tn - 1) / tn;
-    if constexpr (FORM == SCORES) {  // (the gradients' products are f16 whatever the types)
-        if (bf) {
-            if (large) run_product<Large, FORM, EPI, true>(g, st);
-            else run_product<Small, FORM, EPI, true>(g, st);
-            return;
-        }
+enum : int { LARGE = 0, MEDIUM = 1, SMALL = 2 };
+constexpr uint32_t kTileM[3] = {Large::TM, Medium::TM, Small::TM}, kTileN[3] = {Large::TN, Medium::TN, Small::TN};
+template <int FORM, int EPI, bool BF>
+static void product_of(const ProductArgs& g, int shape, hipStream_t st) {
+    switch (shape) {
+        case LARGE: return run_product<Large, FORM, EPI, BF>(g, st);
+        case MEDIUM: return run_product<Medium, FORM, EPI, BF>(g, st);
+        default: return run_product<Small, FORM, EPI, BF>(g, st);
     }
-    if (large) run_product<Large, FORM, EPI, false>(g, st);
-    else run_product<Small, FORM, EPI, false>(g, st);
 }
-// The large tile where it fills the chip: it reads an operand byte per 256 outputs where the small one reads it per 64 / 128.
-static bool use_large(uint64_t m, uint64_t n) { return m > 64 && ((m + 255) / 256) * ((n + 255) / 256) >= 192; }
+template <int FORM, int EPI>
+static void product(ProductArgs g, int shape, bool bf, hipStream_t st) {
+    g.tiles_m = (g.m + kTileM[shape] - 1) / kTileM[shape];
+    g.tiles_n = (g.n + kTileN[shape] - 1) / kTileN[shape];
+    if constexpr (FORM == SCORES) {  // (the gradients' products are f16 whatever the types)
+        if (bf) return product_of<FORM, EPI, true>(g, shape, st);
+    }
+    product_of<FORM, EPI, false>(g, shape, st);
+}
+// The tile for m x n outputs: the one whose rounds over the chip take least.  A round of large tiles (256 workgroups) is 1, of medium ones
+// 0.62, of small ones (512) 0.44 -- measured over 64 .. 4,096 x 131,072 outputs, 768 and 1,536 deep: 256 x 32,768 in 26.6 / 19.5 / 23.7 us,
+// 300 x 131,072 in 89 / 79 / 91, 777 x 131,072 in 167 / 177 / 229, 64 x 131,072 in 52 / 36 / 32.  `whole`: k is sliced until the chip is
+// full, so only the outputs beyond m and n are waste.
+static int choose_shape(uint64_t m, uint64_t n, bool whole) {
+    const double round[3] = {1.0, 0.62, 0.44};
+    const uint64_t resident[3] = {256, 256, 512};
+    int best = SMALL;
+    double least = 1e300;
+    for (int x = 0; x < 3; ++x) {
+        const uint64_t tiles = ((m + kTileM[x] - 1) / kTileM[x]) * ((n + kTileN[x] - 1) / kTileN[x]);
+        const double cost = round[x] * (whole ? (double)tiles / resident[x] : (double)((tiles + resident[x] - 1) / resident[x]));
+        if (cost < least) best = x, least = cost;
+    }
+    return best;
+}
 
 struct Rows {  // vs_rows resolved
     const char* data = nullptr;
@@ -460,7 +478,7 @@ struct Plan {
     bool regrow = false;                                // the rows of dq are laid out apart from those of the scores
     uint32_t nq = 1, nw = 1, np = 1, nqg = 1, nwg = 1;  // planes of the queries, the rows, the probabilities, the queries of dw, the rows of dq
     uint32_t piece = 0, pieces = 0;
-    bool large_s = false, large_q = false, large_w = false;
+    int shape_s = LARGE, shape_q = LARGE, shape_w = LARGE;  // of the scores, dq, dw
     uint32_t splits = 1, qsteps = 1, tiles_v = 0, trows = 0;
     size_t o_label, o_row, o_qplanes, o_top, o_wsc, o_inv, o_wplanes, o_gwplanes, o_part, o_zlab;
     size_t o_df, o_qinv, o_lo, o_ge, o_xe, o_exp, o_gplanes, o_prob, o_tpart, o_coef, o_qpart, o_qacc;
@@ -529,23 +547,22 @@ static Plan plan(const vs_rows* rows, const vs_softmax* q, bool grad_q, bool gra
         p.pieces = (uint32_t)((v + piece - 1) / piece);
     }
     p.piece = (uint32_t)piece;
-    p.large_s = use_large(n, piece);
-    p.large_w = use_large(piece, d);
-    p.large_q = n > 64 && d > 128;
-    const uint32_t tm = p.large_q ? 256 : 64, tn = p.large_q ? 256 : 128;
-    const size_t qtiles = (size_t)((n + tm - 1) / tm) * ((d + tn - 1) / tn);
+    p.shape_s = choose_shape(n, piece, false);
+    p.shape_w = choose_shape(piece, d, false);
+    p.shape_q = choose_shape(n, d, true);
+    const size_t qtiles = (size_t)((n + kTileM[p.shape_q] - 1) / kTileM[p.shape_q]) * ((d + kTileN[p.shape_q] - 1) / kTileN[p.shape_q]);
     const size_t dn = (d + 3u) & ~3u;
     const uint32_t ksteps = (uint32_t)std::max<size_t>(1, (piece + 63) / 64);
     if (grad_q && n) {
-        size_t s = std::max<size_t>(1, (p.large_q ? 256 : 512) / qtiles);
+        size_t s = std::max<size_t>(1, (p.shape_q == SMALL ? 512 : 256) / qtiles);
         s = std::min<size_t>(s, std::max<size_t>(1, kSplitBytes / (n * dn * 4)));
         s = std::min<size_t>(s, std::max<uint32_t>(1, ksteps / 4));
         p.qsteps = (uint32_t)((ksteps + s - 1) / s);
         p.splits = (ksteps + p.qsteps - 1) / p.qsteps;
     }
-    const uint32_t stn = p.large_s ? Large::TN : Small::TN, stm = p.large_s ? Large::TM : Small::TM;
+    const uint32_t stn = kTileN[p.shape_s], stm = kTileM[p.shape_s];
     p.tiles_v = p.pieces ? (p.pieces - 1) * (p.piece / stn) + (uint32_t)((v - (size_t)(p.pieces - 1) * p.piece + stn - 1) / stn) : 0;
-    p.trows = (n + stm - 1) / stm * 2;  // (both shapes have two wave rows)
+    p.trows = (n + stm - 1) / stm * 2;  // (every shape has two wave rows)
     Layout l;
     p.o_label = l.take((size_t)n * 4);
     p.o_row = l.take((size_t)n * 16);
@@ -714,9 +731,8 @@ static void loss(const vs_rows* rows, const vs_softmax* q, float* d_loss, float*
         g.part_ld = p.tiles_v;
         g.part0 = tile;
         g.zlab = c.at<float>(p.o_zlab);
-        product<SCORES, EPI_LOSS>(g, p.large_s, p.bf, st);
-        const uint32_t tn = p.large_s ? Large::TN : Small::TN;
-        tile += (count + tn - 1) / tn;
+        product<SCORES, EPI_LOSS>(g, p.shape_s, p.bf, st);
+        tile += (count + kTileN[p.shape_s] - 1) / kTileN[p.shape_s];
     }
     hipLaunchKernelGGL(loss_join_kernel, dim3(p.n), dim3(256), 0, st, c.at<float2>(p.o_part), p.tiles_v, p.n, c.at<int32_t>(p.o_label),
                        c.at<float>(p.o_zlab), d_loss, d_lse);
@@ -773,8 +789,8 @@ static void loss_grad(const vs_rows* rows, const vs_softmax* q, const float* d_l
         g.prob_planes = p.np;
         g.tpart = d_gw && p.cosine ? c.at<float>(p.o_tpart) : nullptr;
         g.graw = d_g;
-        if (g.tpart) product<SCORES, EPI_PROB_ALONG>(g, p.large_s, p.bf, st);
-        else product<SCORES, EPI_PROB>(g, p.large_s, p.bf, st);
+        if (g.tpart) product<SCORES, EPI_PROB_ALONG>(g, p.shape_s, p.bf, st);
+        else product<SCORES, EPI_PROB>(g, p.shape_s, p.bf, st);
         const Operand prob{(const char*)g.prob, g.prob_plane * 2, (uint64_t)g.prob_ld * 2, p.n, g.prob_ld};
         if (d_gq) {
             ProductArgs b = {};
@@ -786,7 +802,7 @@ static void loss_grad(const vs_rows* rows, const vs_softmax* q, const float* d_l
             plane_pairs(b, p.np, p.nwg, q->scalar != VS_SCALAR_BF16);
             b.lo_first = q->scalar != VS_SCALAR_BF16 && p.np > 1;
             b.out_part = c.at<float>(p.o_qpart);
-            product<DQ, EPI_PART>(b, p.large_q, false, st);
+            product<DQ, EPI_PART>(b, p.shape_q, false, st);
             QueryJoin j = {};
             j.part = b.out_part;
             j.splits = p.splits, j.n = p.n, j.d = p.d, j.dn = dn;
@@ -801,7 +817,7 @@ static void loss_grad(const vs_rows* rows, const vs_softmax* q, const float* d_l
         }
         if (d_gw) {
             if (p.cosine) {
-                const uint32_t stm = p.large_s ? Large::TM : Small::TM;
+                const uint32_t stm = kTileM[p.shape_s];
                 hipLaunchKernelGGL(row_along_kernel, dim3((count + 255) / 256), dim3(256), 0, st, g.tpart, (p.n + stm - 1) / stm * 2, count, c.inv() + first,
                                    c.at<float>(p.o_coef));
                 launched("rows");
@@ -824,7 +840,7 @@ static void loss_grad(const vs_rows* rows, const vs_softmax* q, const float* d_l
             b.raw = p.w.data + (size_t)first * p.w.ld * size_of(p.w.scalar);
             b.raw_scalar = p.w.scalar;
             b.raw_ld = p.w.ld;
-            product<DW, EPI_ROWS>(b, p.large_w, false, st);
+            product<DW, EPI_ROWS>(b, p.shape_w, false, st);
         }
     }
 }
