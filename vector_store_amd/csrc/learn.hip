@@ -92,10 +92,10 @@ __device__ __forceinline__ void put_planes(uint16_t* to, uint64_t plane, uint32_
     *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
     if (nplanes > 1) *reinterpret_cast<uint4*>(to + plane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
 }
-// sum of squares and largest |element| of a row, by a wave
-__device__ __forceinline__ void row_extent(const void* p, int scalar, uint64_t at, uint32_t d, bool wide, uint32_t lane, float& ss, float& top) {
+// sum of squares and largest |element| of a row, by `lanes` lanes (a power of two, up to a wave)
+__device__ __forceinline__ void row_extent(const void* p, int scalar, uint64_t at, uint32_t d, bool wide, uint32_t lane, uint32_t lanes, float& ss, float& top) {
     ss = 0.f, top = 0.f;
-    for (uint32_t k = lane * 8u; k < d; k += 512) {
+    for (uint32_t k = lane * 8u; k < d; k += lanes * 8u) {
         float x[8];
         load8(p, scalar, at + k, d - k, wide, x);
 #pragma unroll
@@ -104,8 +104,10 @@ __device__ __forceinline__ void row_extent(const void* p, int scalar, uint64_t a
             top = fmaxf(top, fabsf(x[r]));
         }
     }
-    ss = wave_sum(ss);
-    top = wave_max(top);
+    for (uint32_t o = lanes >> 1; o; o >>= 1) {
+        ss += __shfl_xor(ss, (int)o);
+        top = fmaxf(top, __shfl_xor(top, (int)o));
+    }
 }
 
 // one wave per query: its norm, largest element, factors, and its planes
@@ -115,7 +117,7 @@ __global__ __launch_bounds__(256) void query_prep_kernel(QueryPrep a) {
     const uint32_t lane = threadIdx.x & 63u, i = blockIdx.x * 4u + (threadIdx.x >> 6);
     if (i >= a.n) return;
     float ss = 0.f, top = 0.f;
-    if (a.cosine || !a.raw || a.g) row_extent(a.q, a.scalar, (uint64_t)i * a.ld, a.d, a.wide, lane, ss, top);
+    if (a.cosine || !a.raw || a.g) row_extent(a.q, a.scalar, (uint64_t)i * a.ld, a.d, a.wide, lane, 64, ss, top);
     const float inv = !a.cosine ? 1.f : ss > 0.f ? 1.f / sqrtf(ss) : 0.f;
     const int32_t e = a.raw || a.cosine ? 0 : exponent_of(top);
     if (a.planes) {
@@ -222,14 +224,21 @@ template <int SC>
 __global__ __launch_bounds__(256) void rows_top_kernel(RowPrep a) {
     const uint32_t lane = threadIdx.x & 63u;
     float top = 0.f;
-    for (uint32_t j = blockIdx.x * 4u + (threadIdx.x >> 6); j < a.rows; j += gridDim.x * 4u) {
-        if (a.keys && a.keys[j] == ~0ull) continue;
-        for (uint32_t k = lane * 8u; k < a.d; k += 512) {
-            float x[8];
-            load8(a.w, SC, (uint64_t)j * a.ld + k, a.d - k, a.wide, x);
+    const auto take = [&](uint64_t at, uint32_t left, bool wide) {
+        float x[8];
+        load8(a.w, SC, at, left, wide, x);
 #pragma unroll
-            for (int r = 0; r < 8; ++r)
-                if (fabsf(x[r]) < __builtin_inff()) top = fmaxf(top, fabsf(x[r]));
+        for (int r = 0; r < 8; ++r)
+            if (fabsf(x[r]) < __builtin_inff()) top = fmaxf(top, fabsf(x[r]));
+    };
+    if (a.ld == a.d && !a.keys) {  // one stretch of memory
+        const uint64_t all = (uint64_t)a.rows * a.d;
+        const bool wide = ((uintptr_t)a.w & 15u) == 0;
+        for (uint64_t k = ((uint64_t)blockIdx.x * 256u + threadIdx.x) * 8u; k < all; k += (uint64_t)gridDim.x * 2048u) take(k, all - k < 8 ? (uint32_t)(all - k) : 8u, wide);
+    } else {
+        for (uint32_t j = blockIdx.x * 4u + (threadIdx.x >> 6); j < a.rows; j += gridDim.x * 4u) {
+            if (a.keys && a.keys[j] == ~0ull) continue;
+            for (uint32_t k = lane * 8u; k < a.d; k += 512) take((uint64_t)j * a.ld + k, a.d - k, a.wide);
         }
     }
     __shared__ float red[4];
@@ -239,10 +248,10 @@ __global__ __launch_bounds__(256) void rows_top_kernel(RowPrep a) {
     top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     if (threadIdx.x == 0 && top > 0.f) atomicMax(a.top, __float_as_uint(top));  // (a maximum: the same bits whatever the order)
 }
-// one wave per row of the piece
+// `lanes` lanes per row of the piece (8 .. 64: as many as a short row has pieces of 8 elements)
 template <int SC>
-__global__ __launch_bounds__(256) void rows_planes_kernel(RowPrep a) {
-    const uint32_t lane = threadIdx.x & 63u, j = blockIdx.x * 4u + (threadIdx.x >> 6);
+__global__ __launch_bounds__(256) void rows_planes_kernel(RowPrep a, uint32_t lanes) {
+    const uint32_t lane = threadIdx.x & (lanes - 1u), j = blockIdx.x * (256u / lanes) + threadIdx.x / lanes;
     const int32_t e = a.raw || a.cosine ? 0 : exponent_of(__uint_as_float(*a.top));
     if (blockIdx.x == 0 && threadIdx.x == 0 && a.wsc) *a.wsc = a.raw || a.cosine ? 1.f : ldexpf(1.f, e - 13);
     if (j >= a.rows) return;
@@ -250,11 +259,11 @@ __global__ __launch_bounds__(256) void rows_planes_kernel(RowPrep a) {
     float inv = 1.f;
     if (a.cosine && !a.raw) {
         float ss, top;
-        row_extent(a.w, SC, (uint64_t)j * a.ld, a.d, a.wide, lane, ss, top);
+        row_extent(a.w, SC, (uint64_t)j * a.ld, a.d, a.wide, lane, lanes, ss, top);
         inv = live && ss > 0.f ? 1.f / sqrtf(ss) : 0.f;
         if (lane == 0 && a.inv) a.inv[j] = inv;
     }
-    for (uint32_t k = lane * 8u; k < a.dp; k += 512) {
+    for (uint32_t k = lane * 8u; k < a.dp; k += lanes * 8u) {
         float x[8];
         load8(a.w, SC, (uint64_t)j * a.ld + k, live && k < a.d ? a.d - k : 0u, a.wide, x);
         if (!a.raw) {
@@ -269,7 +278,7 @@ __global__ __launch_bounds__(256) void rows_inverse_norm_kernel(const void* w, i
     const uint32_t lane = threadIdx.x & 63u, j = blockIdx.x * 4u + (threadIdx.x >> 6);
     if (j >= rows) return;
     float ss, top;
-    row_extent(w, scalar, (uint64_t)j * ld, d, wide, lane, ss, top);
+    row_extent(w, scalar, (uint64_t)j * ld, d, wide, lane, 64, ss, top);
     if (lane == 0) inv[j] = ss > 0.f ? 1.f / sqrtf(ss) : 0.f;
 }
 // ------------------------------------------------------------------------------------------------ joins
@@ -652,10 +661,14 @@ struct Call {  // what the two calls share
     template <int SC>
     void launch_rows(const RowPrep& a) const {
         if (!a.raw && !p.cosine) {
-            hipLaunchKernelGGL((rows_top_kernel<SC>), dim3(std::min<uint32_t>(512, (a.rows + 3) / 4)), dim3(256), 0, st, a);
+            const uint64_t blocks = ((uint64_t)a.rows * a.d + 8191) / 8192;  // (four loads per thread; few workgroups: each ends in an atomic on one word)
+            hipLaunchKernelGGL((rows_top_kernel<SC>), dim3((uint32_t)std::min<uint64_t>(1024, blocks)), dim3(256), 0, st, a);
             launched("rows");
         }
-        hipLaunchKernelGGL((rows_planes_kernel<SC>), dim3((a.rows + 3) / 4), dim3(256), 0, st, a);
+        uint32_t lanes = 8;
+        while (lanes < 64 && lanes * 16 <= a.dp) lanes *= 2;
+        const uint32_t per = 256 / lanes;
+        hipLaunchKernelGGL((rows_planes_kernel<SC>), dim3((a.rows + per - 1) / per), dim3(256), 0, st, a, lanes);
         launched("rows");
     }
     // a piece's rows re-laid: as they are (raw: bf16 or f16), or as f16 planes

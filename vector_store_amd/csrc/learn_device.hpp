@@ -78,6 +78,26 @@ __device__ __forceinline__ void store4(void* p, int scalar, uint64_t i, f32x4 v,
         if ((uint32_t)r < left) store_scalar(p, scalar, i + r, v[r]);
 }
 
+__device__ __forceinline__ f32x4 load4(const void* p, int scalar, uint64_t i, uint32_t left) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (scalar == SC_F32) {
+        const float* from = reinterpret_cast<const float*>(p) + i;
+        if (left >= 4 && ((uintptr_t)from & 15u) == 0) return *reinterpret_cast<const f32x4*>(from);
+    } else {
+        const uint16_t* from = reinterpret_cast<const uint16_t*>(p) + i;
+        if (left >= 4 && ((uintptr_t)from & 7u) == 0) {
+            const ushort4 o = *reinterpret_cast<const ushort4*>(from);
+            if (scalar == SC_F16) v = f32x4{from_half<false>(o.x), from_half<false>(o.y), from_half<false>(o.z), from_half<false>(o.w)};
+            else v = f32x4{from_half<true>(o.x), from_half<true>(o.y), from_half<true>(o.z), from_half<true>(o.w)};
+            return v;
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        if ((uint32_t)r < left) v[r] = load_scalar(p, scalar, i + r);
+    return v;
+}
+
 __device__ __forceinline__ float wave_sum(float v) {
     for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
     return v;

@@ -635,11 +635,7 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                 for (int j = 0; j < S::NT; ++j) {
                     const uint32_t c = cl + j * 16u;
                     f32x4 v = acc[i][j] * rf;
-                    if (tc != 0.f) {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (c + r < g.n) v[r] -= tc * (load_scalar(g.raw, g.raw_scalar, (uint64_t)row * g.raw_ld + c + r) * ti);
-                    }
+                    if (tc != 0.f && c < g.n) v -= load4(g.raw, g.raw_scalar, (uint64_t)row * g.raw_ld + c, g.n - c) * ti * tc;  // (in this order: 1 / |row|^2 may not exist in f32)
                     if (lines) o[j] = to_half4(g.out_scalar, v);
                     else if (has && c < g.n) store4(g.out, g.out_scalar, (uint64_t)row * g.out_ld + c, v, g.n - c);
                 }
