@@ -243,6 +243,28 @@ def test_wide_ranges():
     assert ((lse.double() - want).abs() <= 1e6 * 2 * (3 * 2.0 ** -22 + 480 * 2.0 ** -24) * (q.double().norm(dim=1) * 1.6) + 1).all()
 
 
+@pytest.mark.parametrize("scale", [0.0, -6.0, 1e-30, 40.0])
+def test_scales(scale):
+    """scores turned around, flattened to nothing, and stretched until one member holds nearly all"""
+    for t in (BF16, F32, F16):
+        for metric in (learn.IP, learn.COS):
+            q, w, y, gl = case(150, 1300, 72, t, t, seed=30)
+            check(q, w, y, gl, scale, metric)
+
+
+def test_only_the_label_or_one_row():
+    """a table of one row: the loss is 0 and nothing moves; every query labelled with the same row"""
+    q, w, y, gl = case(100, 1, 64, F32, F32, seed=31, pad=False)
+    loss, lse = learn.softmax_loss(q, w, y, 3.0)
+    gq, gw = learn.softmax_loss_grad(q, w, y, lse, gl, 3.0)
+    assert (loss == 0).all()
+    # p - 1 is off by the rounding of lse: half a step of at most 16, times log2(e), twice
+    assert gq.abs().max() <= 3 * 1.1 * 4 * 2.0 ** -21 * 2 and gw.abs().max() <= 3 * 110 * 4 * 2.0 ** -21 * 2
+    q, w, y, gl = case(200, 900, 96, BF16, BF16, seed=32)
+    y[:] = 17
+    check(q, w, y, gl, 8.0, learn.IP)
+
+
 def test_strides_alignment_and_id_types():
     """views with a row stride, rows that start off a 16-byte line, 32-bit labels: the values of contiguous copies, bit for bit"""
     for t in (BF16, F32, F16):
@@ -337,6 +359,19 @@ def test_lookup_and_gradient(n, v, d, t):
         close(into, want + before.double(), bound + (want.abs() + before.double().abs()) * (U[t] + 2 * U[F32]) + TINY[t], "added gradient")
 
 
+@pytest.mark.parametrize("n,v,d", [(1_300_000, 5000, 8), (5000, 3_000_000, 16), (4096, 10, 24), (4097, 2, 1), (200_000, 100_000, 520)])
+def test_many_ids_and_many_rows(n, v, d):
+    """long lists (several waves' worth of counts, long runs of one id), row numbers of more than two digits of the sort"""
+    g = gen(n)
+    ids = torch.where(torch.rand(n, generator=g, device=DEV) < 0.3, torch.zeros((), dtype=torch.int64, device=DEV), torch.randint(v, (n,), generator=g, device=DEV))
+    ids[::1001] = -1
+    grad = torch.randint(-3, 4, (n, d), generator=g, device=DEV).float()  # whole numbers: every sum below 2^24 is exact in any order
+    got = learn.lookup_grad(grad, ids, v)
+    ok = ids >= 0
+    want = torch.zeros(v, d, dtype=torch.float64, device=DEV).index_put_((ids[ok],), grad[ok].double(), accumulate=True)
+    assert want.abs().max() < 2 ** 24 and torch.equal(got.double(), want)
+
+
 def test_lookup_shapes_and_untouched_neighbours():
     w = torch.randn(50, 12, device=DEV)
     ids = torch.randint(50, (3, 4, 5), device=DEV)
@@ -429,6 +464,31 @@ def test_another_stream_and_two_calls_at_once():
     torch.cuda.synchronize()
     for o in out:
         assert all(torch.equal(x, z) for x, z in zip(o, (l0, s0, a0, b0)))
+
+
+def test_called_from_several_threads():
+    import threading
+    q, w, y, gl = case(130, 2500, 64, F32, F32, seed=17)
+    ids = torch.randint(2500, (700,), device=DEV)
+    want = learn.softmax_loss(q, w, y, 8.0)
+    want = want + learn.softmax_loss_grad(q, w, y, want[1], gl, 8.0) + (learn.lookup_grad(w[ids], ids, 2500),)
+    torch.cuda.synchronize()
+    bad = []
+
+    def run():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                l = learn.softmax_loss(q, w, y, 8.0)
+                got = l + learn.softmax_loss_grad(q, w, y, l[1], gl, 8.0) + (learn.lookup_grad(w[ids], ids, 2500),)
+                torch.cuda.current_stream().synchronize()
+                bad.extend(0 for a, b in zip(got, want) if not torch.equal(a, b))
+
+    threads = [threading.Thread(target=run) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
 
 
 def test_captured_and_replayed():

@@ -10,6 +10,7 @@ Work is enqueued on the current torch stream of the tensors' device and nothing 
 HIP graph.  Scratch is allocated per call from torch's caching allocator.  Wrong arguments raise VsError."""
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 
@@ -108,6 +109,11 @@ class _Source:
             self.c = _Rows(None, t.data_ptr(), _SCALAR[t.dtype], t.shape[0], t.shape[1], _stride(t))
 
 
+def _on(device):
+    """The tensors' device as the current one (a context only where it is not)."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
 def _work(nbytes: int, device):
     return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
 
@@ -122,7 +128,7 @@ def lookup(rows, ids, scale: float = 1.0, dtype=None):
     flat = _ids(ids, s.device, "ids").reshape(-1)
     dtype = dtype or s.dtype
     _need(dtype in _SCALAR, f"dtype: f32, f16 or bf16 is needed, got {dtype}", -7)
-    with torch.cuda.device(s.device):
+    with _on(s.device):
         out = torch.empty((flat.numel(), s.dim), dtype=dtype, device=s.device)
         _check(lib().vs_lookup_device(C.byref(s.c), flat.data_ptr(), _ID_BYTES[flat.dtype], flat.numel(), scale, out.data_ptr(), _SCALAR[dtype], s.dim,
                                       _stream(s.device)))
@@ -138,7 +144,7 @@ def lookup_grad(grad, ids, size: int, scale: float = 1.0, dtype=None, into=None)
     flat = _ids(ids, g.device, "ids").reshape(-1)
     _need(size >= 0, "size must not be negative")
     dim = g.shape[1]
-    with torch.cuda.device(g.device):
+    with _on(g.device):
         if into is not None:
             _need(isinstance(into, torch.Tensor) and into.device == g.device and into.dtype in _SCALAR and tuple(into.shape) == (size, dim),
                   "into: a (size, dim) tensor beside grad is needed")
@@ -172,7 +178,7 @@ def softmax_loss(queries, rows, labels, scale: float = 1.0, metric=None):
     metric COS: cosines instead of inner products.  A label outside [0, rows) marks padding: loss 0.  (IP unless `rows` is an index: its own.)"""
     s = _Source(rows)
     q, y, c = _softmax(queries, s, labels, scale, metric)
-    with torch.cuda.device(s.device):
+    with _on(s.device):
         loss = torch.empty(q.shape[0], dtype=torch.float32, device=s.device)
         lse = torch.empty_like(loss)
         n = lib().vs_softmax_loss_work(C.byref(s.c), C.byref(c))
@@ -190,7 +196,7 @@ def softmax_loss_grad(queries, rows, labels, lse, grad_loss, scale: float = 1.0,
         _need(isinstance(t, torch.Tensor) and t.device == s.device and t.dtype == torch.float32 and tuple(t.shape) == (q.shape[0],),
               f"{what}: one f32 per query is needed")
     lse, grad_loss = lse.detach().contiguous(), grad_loss.detach().contiguous()
-    with torch.cuda.device(s.device):
+    with _on(s.device):
         gq = torch.empty((q.shape[0], s.dim), dtype=q.dtype, device=s.device) if grad_queries else None
         gw = torch.empty((s.count, s.dim), dtype=s.dtype, device=s.device) if grad_rows else None
         n = lib().vs_softmax_loss_grad_work(C.byref(s.c), C.byref(c), int(grad_queries), int(grad_rows))
