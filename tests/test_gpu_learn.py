@@ -143,6 +143,55 @@ def test_large_tiles_and_pieces(tq, tw):
     check(q, w, y, gl, 8.0, learn.IP)
 
 
+@pytest.mark.parametrize("metric", [learn.IP, learn.COS], ids=["ip", "cos"])
+@pytest.mark.parametrize("v,d", [(515, 1), (4099, 4), (3001, 33), (70_003, 100), (20_011, 128), (1000, 516)])
+@pytest.mark.parametrize("n", [1, 2, 31, 64, 65, 128, 129])
+def test_few_f32_queries(n, v, d, metric):
+    """around the numbers of queries up to which f32 is multiplied as f32: rows in place and re-laid, depths that are no multiple of a step"""
+    q, w, y, gl = case(n, v, d, F32, F32, seed=40 + n + d)
+    check(q, w, y, gl, 8.0, metric)
+
+
+def test_few_f32_queries_of_wide_ranges_and_padding():
+    q, w, y, gl = case(50, 700, 96, F32, F32, seed=41)
+    gl = gl * torch.logspace(-12, 12, 50, device=DEV)
+    q2 = q * torch.logspace(-15, 15, 50, device=DEV)[:, None]
+    check(q * torch.logspace(-8, 0, 50, device=DEV)[:, None], w * torch.logspace(-6, 0, 700, device=DEV)[:, None], y, gl, 8.0, learn.IP)
+    check(q2, w * torch.logspace(-15, 15, 700, device=DEV)[:, None], y, gl, 8.0, learn.COS)
+    for metric in (learn.IP, learn.COS):
+        q, w, y, gl = case(50, 515, 100, F32, F32, seed=42, pad=False)
+        y[::7] = -1
+        y[3] = 515
+        off = (y < 0) | (y >= 515)
+        l0, s0 = learn.softmax_loss(q, w, y, 8.0, metric)
+        a0, b0 = learn.softmax_loss_grad(q, w, y, s0, gl, 8.0, metric)
+        for junk in (float("nan"), float("inf"), torch.finfo(F32).max, 0.0):
+            dirty, gl2 = q.clone(), gl.clone()
+            dirty[off], gl2[off] = junk, float("nan")
+            l1, s1 = learn.softmax_loss(dirty, w, y, 8.0, metric)
+            a1, b1 = learn.softmax_loss_grad(dirty, w, y, s1, gl2, 8.0, metric)
+            assert (l1[off] == 0).all() and (a1[off] == 0).all(), metric
+            assert torch.equal(l1, l0) and torch.equal(s1[~off], s0[~off]) and torch.equal(a1, a0) and torch.equal(b1, b0), metric
+
+
+@pytest.mark.parametrize("metric", [vs.IP, vs.COS], ids=["ip", "cos"])
+def test_few_f32_queries_of_an_index(metric):
+    ix, keys, base = build(F32, metric, 1500, 100, 1)
+    slots = torch.from_numpy(ix.slots(keys)).to(DEV)
+    stored = learn.lookup(ix, torch.arange(1500, device=DEV))
+    g = gen(43)
+    y = torch.randint(1500, (33,), generator=g, device=DEV)
+    q = stored[y] + 0.05 * torch.randn(33, 100, generator=g, device=DEV)
+    gl = torch.rand(33, generator=g, device=DEV)
+    check(q, stored, y, gl, 8.0, metric, rows=ix)
+    for k in keys[::5]:
+        assert ix.remove(int(k))
+    dead = torch.zeros(1500, dtype=torch.bool, device=DEV)
+    dead[slots[::5]] = True
+    _, _, _, dw = check(q, stored, y, gl, 8.0, metric, rows=ix, dead=dead)
+    assert (dw[dead] == 0).all()
+
+
 def test_widest_rows_and_one_query_over_many():
     q, w, y, gl = case(2, 513, 4096, F32, F32, seed=4, pad=False)
     check(q, w, y, gl, 4.0, learn.COS)

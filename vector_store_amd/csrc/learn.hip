@@ -32,7 +32,8 @@ static void launched(const char* what) { hip_ok(hipGetLastError(), what); }
 // Number formats.  Both sides bf16: the operands are used as they are (bf16 products are exact in f32).  Both sides f16, inner product: the
 // same on the f16 pipe.  Everything else (f32 anywhere, mixed types, f16 under cosine) is split into f16 planes, x = hi + lo with hi = f16(x),
 // lo = f16(x - hi): 22 bits of x.  Three of the four products of two such numbers are summed (lo lo is below 2^-22 of the result), which is
-// f32's accuracy at three times the f16 product's cost -- the matrix pipe's f32 product costs sixteen.  f16's narrow range is met by
+// f32's accuracy at three times the f16 product's cost -- the matrix pipe's f32 product costs sixteen.  (A few f32 queries of f32 rows are
+// multiplied as f32 all the same, probabilities included: the time is the rows' reading then; kFullLoss.)  f16's narrow range is met by
 // powers of two: a query row, the rows of a piece of the table (inner product), or the normalised vector (cosine) is scaled so that its
 // largest element lies in [2^12, 2^13]; what is 2^-36 of the largest is lost.
 // The gradients' products are f16 for every type: the probabilities are numbers this code rounds itself, and in bf16 their rounding would be
@@ -50,9 +51,10 @@ struct QueryPrep {
     uint32_t rows;                 // labels beyond are ignored
     const uint64_t* keys;          // labels of removed members too
     float scale;
-    uint32_t cosine, bf, raw;      // bf: bf16 operands; raw: planes hold the values themselves (bf16 or f16)
+    uint32_t cosine, raw;          // raw: the operands are the values themselves
+    int kind;                      // K_*
     bool wide;                     // 16-byte aligned rows
-    uint16_t* planes;              // nullptr: read in place
+    void* planes;                  // nullptr: read in place
     uint32_t nplanes;
     uint64_t plane;
     uint32_t* tops;                // the pieces' largest elements, zeroed for rows_top_kernel
@@ -75,8 +77,14 @@ __device__ __forceinline__ int32_t exponent_of(float x) {  // x < 2^e (0, infini
     return e;
 }
 
-// eight consecutive values of a row into its planes
-__device__ __forceinline__ void put_planes(uint16_t* to, uint64_t plane, uint32_t nplanes, bool bf, const float (&x)[8]) {
+// eight consecutive values of a row into its planes (to: element `at` of the first)
+__device__ __forceinline__ void put_planes(void* planes, uint64_t at, uint64_t plane, uint32_t nplanes, int kind, const float (&x)[8]) {
+    if (kind == K_F32) {
+        store8(planes, SC_F32, at, 8, true, x);
+        return;
+    }
+    const bool bf = kind == K_BF16;
+    uint16_t* to = reinterpret_cast<uint16_t*>(planes) + at;
     uint32_t hi[4], lo[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -120,15 +128,16 @@ __global__ __launch_bounds__(256) void query_prep_kernel(QueryPrep a) {
     if (a.cosine || !a.raw || a.g) row_extent(a.q, a.scalar, (uint64_t)i * a.ld, a.d, a.wide, lane, 64, ss, top);
     const float inv = !a.cosine ? 1.f : ss > 0.f ? 1.f / sqrtf(ss) : 0.f;
     const int32_t e = a.raw || a.cosine ? 0 : exponent_of(top);
+    const bool unit = a.cosine && a.kind == K_F32;  // (the planes hold the direction)
     if (a.planes) {
         for (uint32_t k = lane * 8u; k < a.dp; k += 512) {
             float x[8];
             load8(a.q, a.scalar, (uint64_t)i * a.ld + k, k < a.d ? a.d - k : 0u, a.wide, x);
-            if (!a.raw) {
+            if (!a.raw || unit) {
 #pragma unroll
-                for (int r = 0; r < 8; ++r) x[r] = a.cosine ? x[r] * (inv * 8192.f) : ldexpf(x[r], 13 - e);
+                for (int r = 0; r < 8; ++r) x[r] = a.cosine ? x[r] * (inv * (unit ? 1.f : 8192.f)) : ldexpf(x[r], 13 - e);
             }
-            put_planes(a.planes + (uint64_t)i * a.dp + k, a.plane, a.nplanes, a.bf, x);
+            put_planes(a.planes, (uint64_t)i * a.dp + k, a.plane, a.nplanes, a.kind, x);
         }
     }
     if (lane) return;
@@ -136,7 +145,7 @@ __global__ __launch_bounds__(256) void query_prep_kernel(QueryPrep a) {
     if (y < 0 || y >= (int64_t)a.rows || (a.keys && a.keys[y] == ~0ull)) y = -1;
     a.label[i] = (int32_t)y;
     const float s2 = a.scale * kLog2e;
-    float4 row = make_float4(a.raw ? s2 * inv : a.cosine ? s2 * 0x1p-26f : ldexpf(s2, e - 13), 0.f, 0.f, __int_as_float((int32_t)y));
+    float4 row = make_float4(unit ? s2 : a.raw ? s2 * inv : a.cosine ? s2 * 0x1p-26f : ldexpf(s2, e - 13), 0.f, 0.f, __int_as_float((int32_t)y));
     if (a.g) {
         // lse in base-2 units, in two parts: row.y and what its rounding lost, which goes into the factor
         const float lse = a.lse[i];
@@ -146,28 +155,30 @@ __global__ __launch_bounds__(256) void query_prep_kernel(QueryPrep a) {
         a.inv[i] = inv;
         const float g = y >= 0 ? a.g[i] : 0.f;
         // f16 probabilities: (p - [label]) * m * 2^15 with g = m * 2^x, 1/2 <= |m| < 1: below 2^15, off by at most 2^-11 of themselves or 2^-39
+        // (f32: the probability itself times the row's inverse length; the query's factors go to dq and, in front of dw, to the query)
         int x = 0;
         const float m = frexpf(g, &x);
-        row.z = m * 32768.f * exp2f(-lo);
-        a.df[i] = y >= 0 ? ldexpf(a.scale * (a.cosine ? inv * 0x1p-13f : 1.f), x - 15) : 0.f;
+        row.z = (a.kind == K_F32 ? 1.f : m * 32768.f) * exp2f(-lo);
+        a.df[i] = y < 0 ? 0.f : a.kind == K_F32 ? g * a.scale * inv : ldexpf(a.scale * (a.cosine ? inv * 0x1p-13f : 1.f), x - 15);
         a.ge[i] = x;
         a.xe[i] = y < 0 || !(g != 0.f) ? kNoExponent : x + exponent_of(a.cosine ? top * inv : top);
     }
     a.row[i] = row;
 }
 
-// The queries as an operand of dw = P^T q, in f16: rows of padding are zero whatever they held, every other row carries the power of two of its
-// loss gradient, relative to the largest; *wf undoes it.
+// The queries as an operand of dw = P^T q: rows of padding are zero whatever they held.  f16: every other row carries the power of two of its
+// loss gradient, relative to the largest; *wf undoes it.  f32: its loss gradient itself, the scale and (cosine) its inverse length.
 struct GradQueries {
     const void* q;
     int scalar;
     uint64_t ld;
     uint32_t n, d, dp, cosine, nplanes;
+    int kind;  // K_F16 or K_F32
     bool wide;
     const int32_t *label, *ge, *xe;
-    const float* inv;
+    const float *inv, *g;
     float scale;
-    uint16_t* planes;
+    void* planes;
     uint64_t plane;
     int32_t* top;  // [1]
     float* wf;     // [1]
@@ -190,19 +201,20 @@ __global__ __launch_bounds__(1024) void grad_exponent_kernel(GradQueries a) {
     if (threadIdx.x == 0) a.top[0] = top;
 }
 __global__ __launch_bounds__(256) void grad_queries_kernel(GradQueries a) {
-    const int32_t top = a.n <= kOwnExponent ? grad_exponent(a) : a.top[0];
+    const int32_t top = a.kind == K_F32 ? 0 : a.n <= kOwnExponent ? grad_exponent(a) : a.top[0];
     if (blockIdx.x == 0 && threadIdx.x == 0) a.wf[0] = ldexpf(a.scale, top - 28);
     const uint32_t lane = threadIdx.x & 63u, i = blockIdx.x * 4u + (threadIdx.x >> 6);
     if (i >= a.n) return;
     const bool on = a.label[i] >= 0 && a.xe[i] != kNoExponent;  // (padding, and queries whose loss nobody asks about)
-    const int32_t up = a.ge[i] - top + 13;
-    const float inv = a.cosine ? a.inv[i] : 1.f;
+    const bool full = a.kind == K_F32;
+    const int32_t up = full ? 0 : a.ge[i] - top + 13;
+    const float inv = a.cosine ? a.inv[i] : 1.f, f = full && on ? a.g[i] * a.scale : 1.f;
     for (uint32_t k = lane * 8u; k < a.dp; k += 512) {
         float x[8];
         load8(a.q, a.scalar, (uint64_t)i * a.ld + k, on && k < a.d ? a.d - k : 0u, a.wide, x);
 #pragma unroll
-        for (int r = 0; r < 8; ++r) x[r] = ldexpf(x[r] * inv, up);
-        put_planes(a.planes + (uint64_t)i * a.dp + k, a.plane, a.nplanes, false, x);
+        for (int r = 0; r < 8; ++r) x[r] = full ? x[r] * inv * f : ldexpf(x[r] * inv, up);
+        put_planes(a.planes, (uint64_t)i * a.dp + k, a.plane, a.nplanes, a.kind, x);
     }
 }
 
@@ -212,9 +224,10 @@ struct RowPrep {
     uint64_t ld;
     uint32_t rows, d, dp;
     const uint64_t* keys;  // of the piece
-    uint32_t cosine, bf, raw, nplanes;
+    uint32_t cosine, raw, nplanes;
+    int kind;
     bool wide;
-    uint16_t* planes;
+    void* planes;
     uint64_t plane;
     uint32_t* top;   // bits of the largest |element| of the piece (inner product planes)
     float* wsc;      // 2^(e - 13)
@@ -270,7 +283,7 @@ __global__ __launch_bounds__(256) void rows_planes_kernel(RowPrep a, uint32_t la
 #pragma unroll
             for (int r = 0; r < 8; ++r) x[r] = a.cosine ? x[r] * (inv * 8192.f) : ldexpf(x[r], 13 - e);
         }
-        put_planes(a.planes + (uint64_t)j * a.dp + k, a.plane, a.nplanes, a.bf, x);
+        put_planes(a.planes, (uint64_t)j * a.dp + k, a.plane, a.nplanes, a.kind, x);
     }
 }
 // 1 / |row| of a table whose rows are used as they are
@@ -365,35 +378,36 @@ __global__ __launch_bounds__(256) void row_along_kernel(const float* tpart, uint
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-template <class S, int FORM, int EPI, bool BF>
+template <class S, int FORM, int EPI, int KIND>
 static void run_product(const ProductArgs& g, hipStream_t st) {
     static const hipError_t allowed =
-        hipFuncSetAttribute(reinterpret_cast<const void*>(&product_kernel<S, FORM, EPI, BF>), hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS);
+        hipFuncSetAttribute(reinterpret_cast<const void*>(&product_kernel<S, FORM, EPI, KIND>), hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS);
     hip_ok(allowed, "shared memory of the product");
     const uint64_t tiles = (uint64_t)g.tiles_m * g.tiles_n * g.splits;
     if (tiles >= (1ull << 31)) fail(VS_ERR_UNSUPPORTED, "too many tiles");
     constexpr uint32_t resident = 256u * (160u * 1024u / S::LDS);
-    hipLaunchKernelGGL((product_kernel<S, FORM, EPI, BF>), dim3((uint32_t)std::min<uint64_t>((tiles + 7) / 8 * 8, resident)), dim3(S::NW * 64), S::LDS, st, g);
+    hipLaunchKernelGGL((product_kernel<S, FORM, EPI, KIND>), dim3((uint32_t)std::min<uint64_t>((tiles + 7) / 8 * 8, resident)), dim3(S::NW * 64), S::LDS, st, g);
     launched("product");
 }
 enum : int { LARGE = 0, MEDIUM = 1, SMALL = 2 };
 constexpr uint32_t kTileM[3] = {Large::TM, Medium::TM, Small::TM}, kTileN[3] = {Large::TN, Medium::TN, Small::TN};
-template <int FORM, int EPI, bool BF>
+template <int FORM, int EPI, int KIND>
 static void product_of(const ProductArgs& g, int shape, hipStream_t st) {
     switch (shape) {
-        case LARGE: return run_product<Large, FORM, EPI, BF>(g, st);
-        case MEDIUM: return run_product<Medium, FORM, EPI, BF>(g, st);
-        default: return run_product<Small, FORM, EPI, BF>(g, st);
+        case LARGE: return run_product<Large, FORM, EPI, KIND>(g, st);
+        case MEDIUM: return run_product<Medium, FORM, EPI, KIND>(g, st);
+        default: return run_product<Small, FORM, EPI, KIND>(g, st);
     }
 }
 template <int FORM, int EPI>
-static void product(ProductArgs g, int shape, bool bf, hipStream_t st) {
+static void product(ProductArgs g, int shape, int kind, hipStream_t st) {
     g.tiles_m = (g.m + kTileM[shape] - 1) / kTileM[shape];
     g.tiles_n = (g.n + kTileN[shape] - 1) / kTileN[shape];
-    if constexpr (FORM == SCORES) {  // (the gradients' products are f16 whatever the types)
-        if (bf) return product_of<FORM, EPI, true>(g, shape, st);
+    if (kind == K_F32) return run_product<Small, FORM, EPI, K_F32>(g, st);  // (shape: SMALL)
+    if constexpr (FORM == SCORES) {  // (the gradients' products of 16-bit operands are f16)
+        if (kind == K_BF16) return product_of<FORM, EPI, K_BF16>(g, shape, st);
     }
-    product_of<FORM, EPI, false>(g, shape, st);
+    product_of<FORM, EPI, K_F16>(g, shape, st);
 }
 // The tile for m x n outputs: the one whose rounds over the chip take least.  A round of large tiles (256 workgroups) is 1, of medium ones
 // 0.62, of small ones (512) 0.44 -- measured over 64 .. 4,096 x 131,072 outputs, 768 and 1,536 deep: 256 x 32,768 in 26.6 / 19.5 / 23.7 us,
@@ -482,8 +496,10 @@ struct Layout {  // offsets into the caller's scratch
 struct Plan {
     Rows w;
     uint32_t n = 0, v = 0, d = 0, dp = 0;
-    bool cosine = false, bf = false, raw = false, q_in_place = false, w_in_place = false, inv_own = false;
+    bool cosine = false, raw = false, q_in_place = false, w_in_place = false, inv_own = false;
     bool grad_q = false, grad_w = false;
+    int kind = K_F16, gkind = K_F16;                    // operands of the scores; of the gradients' products
+    uint32_t es = 2, ges = 2, bk = 64, gbk = 64;        // bytes per element and elements per step of both
     bool regrow = false;                                // the rows of dq are laid out apart from those of the scores
     uint32_t nq = 1, nw = 1, np = 1, nqg = 1, nwg = 1;  // planes of the queries, the rows, the probabilities, the queries of dw, the rows of dq
     uint32_t piece = 0, pieces = 0;
@@ -498,6 +514,11 @@ struct Plan {
 // larger pieces leave fewer CUs without a tile, and what the last-level cache (256 MiB) no longer holds costs about as much.
 constexpr size_t kPieceBytes = 640ull << 20;
 constexpr size_t kSplitBytes = 128ull << 20;    // f32 slices of dq
+// Up to this many f32 queries of f32 rows are multiplied as f32 (the loss; its gradient): the rows are then read once where the split re-lays them
+// first, about four times the traffic, and the f32 MFMA's sixteenth of the f16 rate does not show before more queries than that.  60,000 x 768, as
+// f32 / split: 40 queries 67 / 159 us and 219 / 304, 96: 114 / 161 and 331 / 327, 128: 116 / 162 and 359 / 333, 192: 165 / 185 and 502 / 391;
+// 64 by cosine 95 / 132 and 290 / 342.
+constexpr uint32_t kFullLoss = 128, kFullGrad = 64;
 
 // Rows per piece, at most `most`.  A workgroup per CU owns 256 x 256 outputs, so 257 tiles take as long as 512: of the sizes allowed, the one
 // whose products leave the fewest CUs idle (in steps of 64 k; a tile's epilogue counts 6, a piece's launches 10).
@@ -532,22 +553,27 @@ static Plan plan(const vs_rows* rows, const vs_softmax* q, bool grad_q, bool gra
     p.dp = (d + 63u) & ~63u;
     p.cosine = q->metric == VS_METRIC_COS;
     const int tq = q->scalar, tw = p.w.scalar;
-    p.bf = tq == VS_SCALAR_BF16 && tw == VS_SCALAR_BF16;
-    p.raw = p.bf || (tq == VS_SCALAR_F16 && tw == VS_SCALAR_F16 && !p.cosine);
-    p.q_in_place = p.raw && d % 8 == 0 && q->stride % 8 == 0 && (uintptr_t)q->d_queries % 16 == 0;
-    p.w_in_place = p.raw && !p.w.keys && d % 8 == 0 && p.w.ld % 8 == 0 && (uintptr_t)p.w.data % 16 == 0;
+    const bool bf = tq == VS_SCALAR_BF16 && tw == VS_SCALAR_BF16, full = tq == VS_SCALAR_F32 && tw == VS_SCALAR_F32 && n <= (grad_q || grad_w ? kFullGrad : kFullLoss);
+    p.kind = full ? K_F32 : bf ? K_BF16 : K_F16;
+    p.gkind = full ? K_F32 : K_F16;
+    p.es = full ? 4 : 2, p.bk = 128 / p.es;
+    p.ges = p.es, p.gbk = p.bk;
+    p.raw = full || bf || (tq == VS_SCALAR_F16 && tw == VS_SCALAR_F16 && !p.cosine);
+    const uint32_t line = 16 / p.es;
+    p.q_in_place = p.raw && !(full && p.cosine) && d % line == 0 && q->stride % line == 0 && (uintptr_t)q->d_queries % 16 == 0;
+    p.w_in_place = p.raw && !p.w.keys && d % line == 0 && p.w.ld % line == 0 && (uintptr_t)p.w.data % 16 == 0;
     p.inv_own = p.cosine && !(p.raw && p.w.inv);
     p.nq = !p.raw && (p.cosine || tq == VS_SCALAR_F32) ? 2 : 1;
     p.nw = !p.raw && (p.cosine || tw == VS_SCALAR_F32) ? 2 : 1;
     p.grad_q = grad_q;
     p.grad_w = grad_w;
     const bool grad = grad_q || grad_w;
-    p.np = (grad_q && tq != VS_SCALAR_BF16) || (grad_w && tw != VS_SCALAR_BF16) ? 2 : 1;
-    p.nqg = tw != VS_SCALAR_BF16 && (p.cosine || tq == VS_SCALAR_F32) ? 2 : 1;
-    p.regrow = p.bf && grad_q;
+    p.np = !full && ((grad_q && tq != VS_SCALAR_BF16) || (grad_w && tw != VS_SCALAR_BF16)) ? 2 : 1;
+    p.nqg = !full && tw != VS_SCALAR_BF16 && (p.cosine || tq == VS_SCALAR_F32) ? 2 : 1;
+    p.regrow = bf && grad_q;
     p.nwg = p.regrow ? 1 : p.nw;
     // pieces of the table: one, unless rows are re-laid or probabilities are kept for the two products that read them
-    const size_t per_row = (p.w_in_place ? 0 : (size_t)p.nw * p.dp * 2) + (p.regrow ? (size_t)p.dp * 2 : 0) + (grad ? (size_t)p.np * n * 2 : 0);
+    const size_t per_row = (p.w_in_place ? 0 : (size_t)p.nw * p.dp * p.es) + (p.regrow ? (size_t)p.dp * 2 : 0) + (grad ? (size_t)p.np * n * p.ges : 0);
     size_t piece = v;
     if (per_row) piece = std::min<size_t>(v, std::max<size_t>(2048, kPieceBytes / per_row));
     piece = std::min<size_t>(piece, 1u << 20);
@@ -556,12 +582,12 @@ static Plan plan(const vs_rows* rows, const vs_softmax* q, bool grad_q, bool gra
         p.pieces = (uint32_t)((v + piece - 1) / piece);
     }
     p.piece = (uint32_t)piece;
-    p.shape_s = choose_shape(n, piece, false);
-    p.shape_w = choose_shape(piece, d, false);
-    p.shape_q = choose_shape(n, d, true);
+    p.shape_s = full ? SMALL : choose_shape(n, piece, false);
+    p.shape_w = full ? SMALL : choose_shape(piece, d, false);
+    p.shape_q = full ? SMALL : choose_shape(n, d, true);
     const size_t qtiles = (size_t)((n + kTileM[p.shape_q] - 1) / kTileM[p.shape_q]) * ((d + kTileN[p.shape_q] - 1) / kTileN[p.shape_q]);
     const size_t dn = (d + 3u) & ~3u;
-    const uint32_t ksteps = (uint32_t)std::max<size_t>(1, (piece + 63) / 64);
+    const uint32_t ksteps = (uint32_t)std::max<size_t>(1, (piece + p.gbk - 1) / p.gbk);
     if (grad_q && n) {
         size_t s = std::max<size_t>(1, (p.shape_q == SMALL ? 512 : 256) / qtiles);
         s = std::min<size_t>(s, std::max<size_t>(1, kSplitBytes / (n * dn * 4)));
@@ -575,11 +601,11 @@ static Plan plan(const vs_rows* rows, const vs_softmax* q, bool grad_q, bool gra
     Layout l;
     p.o_label = l.take((size_t)n * 4);
     p.o_row = l.take((size_t)n * 16);
-    p.o_qplanes = l.take(p.q_in_place ? 0 : (size_t)p.nq * n * p.dp * 2);
+    p.o_qplanes = l.take(p.q_in_place ? 0 : (size_t)p.nq * n * p.dp * p.es);
     p.o_top = l.take((size_t)p.pieces * 4);
     p.o_wsc = l.take((size_t)p.pieces * 4);
     p.o_inv = l.take(p.inv_own ? (size_t)v * 4 : 0);
-    p.o_wplanes = l.take(p.w_in_place ? 0 : (size_t)p.nw * piece * p.dp * 2);
+    p.o_wplanes = l.take(p.w_in_place ? 0 : (size_t)p.nw * piece * p.dp * p.es);
     p.o_gwplanes = l.take(p.regrow ? piece * p.dp * 2 : 0);
     if (!grad) {
         p.o_part = l.take((size_t)n * p.tiles_v * 8);
@@ -591,8 +617,8 @@ static Plan plan(const vs_rows* rows, const vs_softmax* q, bool grad_q, bool gra
         p.o_ge = l.take((size_t)n * 4);
         p.o_xe = l.take((size_t)n * 4);
         p.o_exp = l.take(8);
-        p.o_gplanes = l.take(grad_w ? (size_t)p.nqg * n * p.dp * 2 : 0);
-        p.o_prob = l.take((size_t)p.np * n * (((size_t)piece + 7) & ~(size_t)7) * 2);
+        p.o_gplanes = l.take(grad_w ? (size_t)p.nqg * n * p.dp * p.ges : 0);
+        p.o_prob = l.take((size_t)p.np * n * (((size_t)piece + 7) & ~(size_t)7) * p.ges);
         p.o_tpart = l.take(grad_w && p.cosine ? (size_t)p.trows * piece * 4 : 0);
         p.o_coef = l.take(grad_w && p.cosine ? (size_t)piece * 4 : 0);
         p.o_qpart = l.take(grad_q ? (size_t)p.splits * n * dn * 4 : 0);
@@ -631,9 +657,9 @@ struct Call {  // what the two calls share
         a.rows = p.v;
         a.keys = p.w.keys;
         a.scale = q.scale;
-        a.cosine = p.cosine, a.bf = p.bf, a.raw = p.raw;
+        a.cosine = p.cosine, a.raw = p.raw, a.kind = p.kind;
         a.wide = wide_rows(a.q, a.scalar, a.ld);
-        a.planes = p.q_in_place ? nullptr : at<uint16_t>(p.o_qplanes);
+        a.planes = p.q_in_place ? nullptr : at<char>(p.o_qplanes);
         a.nplanes = p.nq;
         a.plane = (uint64_t)p.n * p.dp;
         a.tops = at<uint32_t>(p.o_top);
@@ -679,9 +705,9 @@ struct Call {  // what the two calls share
         a.ld = p.w.ld;
         a.rows = count, a.d = p.d, a.dp = p.dp;
         a.keys = p.w.keys ? p.w.keys + first : nullptr;
-        a.cosine = p.cosine, a.raw = raw, a.bf = raw && p.bf, a.nplanes = nplanes;
+        a.cosine = p.cosine, a.raw = raw, a.kind = raw ? p.kind : K_F16, a.nplanes = nplanes;
         a.wide = wide_rows(a.w, a.scalar, a.ld);
-        a.planes = at<uint16_t>(o_planes);
+        a.planes = at<char>(o_planes);
         a.plane = (uint64_t)p.piece * p.dp;
         a.top = at<uint32_t>(p.o_top) + x;
         a.wsc = at<float>(p.o_wsc) + x;
@@ -691,11 +717,12 @@ struct Call {  // what the two calls share
             case VS_SCALAR_F16: launch_rows<SC_F16>(a); break;
             default: launch_rows<SC_BF16>(a); break;
         }
-        return Operand{(const char*)a.planes, a.plane * 2, (uint64_t)p.dp * 2, count, p.dp};
+        const uint64_t es = raw ? p.es : 2;
+        return Operand{(const char*)a.planes, a.plane * es, (uint64_t)p.dp * es, count, p.dp};
     }
     // the piece's rows as an operand of the scores; of dq
     Operand rows(uint32_t x, uint32_t first, uint32_t count) const {
-        if (p.w_in_place) return Operand{p.w.data + (size_t)first * p.w.ld * size_of(p.w.scalar), 0, p.w.ld * 2, count, p.d};
+        if (p.w_in_place) return Operand{p.w.data + (size_t)first * p.w.ld * size_of(p.w.scalar), 0, p.w.ld * p.es, count, p.d};
         return relay(x, first, count, p.o_wplanes, p.nw, p.raw);
     }
     Operand grad_rows(const Operand& scores, uint32_t x, uint32_t first, uint32_t count) const {
@@ -704,13 +731,13 @@ struct Call {  // what the two calls share
     // scores of all queries against a piece: operands and factors
     ProductArgs scores(const Operand& w, uint32_t x, uint32_t first, uint32_t count) const {
         ProductArgs g = {};
-        g.a = p.q_in_place ? Operand{(const char*)q.d_queries, 0, q.stride * 2, p.n, p.d}
-                           : Operand{at<char>(p.o_qplanes), (uint64_t)p.n * p.dp * 2, (uint64_t)p.dp * 2, p.n, p.dp};
+        g.a = p.q_in_place ? Operand{(const char*)q.d_queries, 0, q.stride * p.es, p.n, p.d}
+                           : Operand{at<char>(p.o_qplanes), (uint64_t)p.n * p.dp * p.es, (uint64_t)p.dp * p.es, p.n, p.dp};
         g.b = w;
         g.m = p.n, g.n = count;
         g.k = std::min(g.a.cols, g.b.cols);  // (a re-laid operand's padding is zero)
         g.splits = 1;
-        g.ksteps = (g.k + 63) / 64;
+        g.ksteps = (g.k + p.bk - 1) / p.bk;
         plane_pairs(g, p.nq, p.nw, true);
         g.row = at<float4>(p.o_row);
         g.h = h() ? h() + first : nullptr;
@@ -744,7 +771,7 @@ static void loss(const vs_rows* rows, const vs_softmax* q, float* d_loss, float*
         g.part_ld = p.tiles_v;
         g.part0 = tile;
         g.zlab = c.at<float>(p.o_zlab);
-        product<SCORES, EPI_LOSS>(g, p.shape_s, p.bf, st);
+        product<SCORES, EPI_LOSS>(g, p.shape_s, p.kind, st);
         tile += (count + kTileN[p.shape_s] - 1) / kTileN[p.shape_s];
     }
     hipLaunchKernelGGL(loss_join_kernel, dim3(p.n), dim3(256), 0, st, c.at<float2>(p.o_part), p.tiles_v, p.n, c.at<int32_t>(p.o_label),
@@ -776,19 +803,19 @@ static void loss_grad(const vs_rows* rows, const vs_softmax* q, const float* d_l
         a.q = q->d_queries;
         a.scalar = q->scalar;
         a.ld = q->stride;
-        a.n = p.n, a.d = p.d, a.dp = p.dp, a.cosine = p.cosine, a.nplanes = p.nqg;
+        a.n = p.n, a.d = p.d, a.dp = p.dp, a.cosine = p.cosine, a.nplanes = p.nqg, a.kind = p.gkind;
         a.wide = wide_rows(a.q, a.scalar, a.ld);
         a.label = c.at<int32_t>(p.o_label), a.ge = c.at<int32_t>(p.o_ge), a.xe = c.at<int32_t>(p.o_xe);
-        a.inv = c.at<float>(p.o_qinv);
+        a.inv = c.at<float>(p.o_qinv), a.g = d_g;
         a.scale = q->scale;
-        a.planes = c.at<uint16_t>(p.o_gplanes);
+        a.planes = c.at<char>(p.o_gplanes);
         a.plane = (uint64_t)p.n * p.dp;
         a.top = c.at<int32_t>(p.o_exp);
         a.wf = c.at<float>(p.o_exp) + 1;
-        if (p.n > kOwnExponent) hipLaunchKernelGGL(grad_exponent_kernel, dim3(1), dim3(1024), 0, st, a);
+        if (p.gkind != K_F32 && p.n > kOwnExponent) hipLaunchKernelGGL(grad_exponent_kernel, dim3(1), dim3(1024), 0, st, a);
         hipLaunchKernelGGL(grad_queries_kernel, dim3((p.n + 3) / 4), dim3(256), 0, st, a);
         launched("queries");
-        gq = Operand{(const char*)a.planes, a.plane * 2, (uint64_t)p.dp * 2, p.n, p.dp};
+        gq = Operand{(const char*)a.planes, a.plane * p.ges, (uint64_t)p.dp * p.ges, p.n, p.dp};
     }
     const uint32_t dn = (p.d + 3u) & ~3u;
     for (uint32_t x = 0; x < p.pieces; ++x) {
@@ -802,9 +829,9 @@ static void loss_grad(const vs_rows* rows, const vs_softmax* q, const float* d_l
         g.prob_planes = p.np;
         g.tpart = d_gw && p.cosine ? c.at<float>(p.o_tpart) : nullptr;
         g.graw = d_g;
-        if (g.tpart) product<SCORES, EPI_PROB_ALONG>(g, p.shape_s, p.bf, st);
-        else product<SCORES, EPI_PROB>(g, p.shape_s, p.bf, st);
-        const Operand prob{(const char*)g.prob, g.prob_plane * 2, (uint64_t)g.prob_ld * 2, p.n, g.prob_ld};
+        if (g.tpart) product<SCORES, EPI_PROB_ALONG>(g, p.shape_s, p.kind, st);
+        else product<SCORES, EPI_PROB>(g, p.shape_s, p.kind, st);
+        const Operand prob{(const char*)g.prob, g.prob_plane * p.ges, (uint64_t)g.prob_ld * p.ges, p.n, g.prob_ld};
         if (d_gq) {
             ProductArgs b = {};
             b.a = prob;
@@ -815,7 +842,7 @@ static void loss_grad(const vs_rows* rows, const vs_softmax* q, const float* d_l
             plane_pairs(b, p.np, p.nwg, q->scalar != VS_SCALAR_BF16);
             b.lo_first = q->scalar != VS_SCALAR_BF16 && p.np > 1;
             b.out_part = c.at<float>(p.o_qpart);
-            product<DQ, EPI_PART>(b, p.shape_q, false, st);
+            product<DQ, EPI_PART>(b, p.shape_q, p.gkind, st);
             QueryJoin j = {};
             j.part = b.out_part;
             j.splits = p.splits, j.n = p.n, j.d = p.d, j.dn = dn;
@@ -840,20 +867,20 @@ static void loss_grad(const vs_rows* rows, const vs_softmax* q, const float* d_l
             b.b = gq;
             b.m = count, b.n = p.d, b.k = p.n;
             b.splits = 1;
-            b.ksteps = (p.n + 63) / 64;
+            b.ksteps = (p.n + p.gbk - 1) / p.gbk;
             plane_pairs(b, p.np, p.nqg, p.w.scalar != VS_SCALAR_BF16);
             b.lo_first = p.w.scalar != VS_SCALAR_BF16 && p.np > 1;
             b.out = (char*)d_gw + (size_t)first * gw_ld * size_of(p.w.scalar);
             b.out_scalar = p.w.scalar;
             b.out_ld = gw_ld;
-            b.wf = c.at<float>(p.o_exp) + 1;
-            b.rf = p.cosine ? c.inv() + first : nullptr;
+            b.wf = p.gkind == K_F32 ? nullptr : c.at<float>(p.o_exp) + 1;
+            b.rf = p.cosine && p.gkind != K_F32 ? c.inv() + first : nullptr;
             b.tcoef = p.cosine ? c.at<float>(p.o_coef) : nullptr;
             b.tinv = p.cosine ? c.inv() + first : nullptr;
             b.raw = p.w.data + (size_t)first * p.w.ld * size_of(p.w.scalar);
             b.raw_scalar = p.w.scalar;
             b.raw_ld = p.w.ld;
-            product<DW, EPI_ROWS>(b, p.shape_w, false, st);
+            product<DW, EPI_ROWS>(b, p.shape_w, p.gkind, st);
         }
     }
 }

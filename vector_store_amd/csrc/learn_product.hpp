@@ -1,16 +1,16 @@
-// learn_product.hpp -- the tiled matrix product behind the softmax loss (learn.hip): C = sum over plane pairs of A B, 16-bit operands, f32
-// accumulation on the matrix pipe, with the loss's own epilogues.
+// learn_product.hpp -- the tiled matrix product behind the softmax loss (learn.hip): C = sum over plane pairs of A B on the matrix pipe, f32
+// accumulation, with the loss's own epilogues.
 //
 //   SCORES  A [m x k] rows, B [n x k] rows      z = q w^T          both operands lie along k
 //   DQ      A [m x k] rows, B [k x n] rows      dq = P w           B lies across k
 //   DW      A [k x m] rows, B [k x n] rows      dw = P^T q         both lie across k
 //
-// A workgroup owns TM x TN outputs and walks k in steps of 64 through a ring of two LDS stages that the load units fill by themselves
+// A workgroup owns TM x TN outputs and walks k in steps of 128 bytes through a ring of two LDS stages that the load units fill by themselves
 // (buffer_load ... lds, 16 bytes per lane: no register round trip).  The buffer descriptors carry the operands' true bounds, so rows, columns
 // and k beyond the end arrive as zeros and no operand has to be padded.  LDS images:
-//   along k:   [row][64 k], 128 bytes per row, 16-byte chunks XOR-swizzled by the row (conflict-free ds_read_b128 fragments);
-//   across k:  [64 k][columns], 32-byte units XOR-swizzled by k; the fragments come through ds_read_b64_tr_b16, which hands each lane four
-//              consecutive k of one column: no transposed copy of P, the queries or the table is ever written.
+//   along k:   [row][a step], 128 bytes per row, 16-byte chunks XOR-swizzled by the row (conflict-free ds_read_b128 fragments);
+//   across k:  [k][columns], 32-byte units (f32: 64-byte ones) XOR-swizzled by k; the fragments of 16-bit operands come through
+//              ds_read_b64_tr_b16, which hands each lane four consecutive k of one column: no transposed copy of P, the queries or the table is ever written.
 // The swizzles are applied to the SOURCE address of the load (the LDS side of such a load is linear).
 // The operands of the MFMA are swapped (B first): a lane then holds four consecutive COLUMNS of one output row, so row-wise softmax sums are
 // mostly in-lane and stores are 8 / 16 bytes wide.
@@ -25,6 +25,7 @@ namespace vs {
 namespace learn {
 
 enum : int { SCORES = 0, DQ = 1, DW = 2 };
+enum : int { K_F16 = 0, K_BF16 = 1, K_F32 = 2 };  // what the operands hold
 enum : int { EPI_LOSS = 0, EPI_PROB = 1, EPI_PART = 2, EPI_ROWS = 3, EPI_PROB_ALONG = 4 };  // (.._ALONG: cosine, with the sums of c z per column)
 
 struct Operand {
@@ -32,14 +33,14 @@ struct Operand {
     uint64_t plane;   // bytes between planes
     uint64_t ld;      // bytes between stored rows
     uint32_t rows;    // stored rows
-    uint32_t cols;    // valid elements of a stored row (a multiple of 8)
+    uint32_t cols;    // valid elements of a stored row (a multiple of 16 bytes)
 };
 
 struct ProductArgs {
     Operand a, b;
     uint32_t m, n, k;            // outputs and depth
     uint32_t tiles_m, tiles_n;
-    uint32_t splits, ksteps;     // slices of k and 64-deep steps per slice
+    uint32_t splits, ksteps;     // slices of k and steps per slice
     uint32_t segs;               // plane pairs
     uint32_t seg_a, seg_b;       // 4 bits each: the planes of pair s
     uint32_t lo_first;           // the first pair's a is the probabilities' second plane, which is stored times 2^11
@@ -53,7 +54,8 @@ struct ProductArgs {
     float2* part;                // [m][part_ld] (maximum, sum of 2^(z2 - maximum)) per column tile
     uint32_t part_ld, part0;
     float* zlab;                 // z2 at the label
-    // EPI_PROB: P = f16((2^(z2 - lse2 - lo) - [label]) * pf), and 2^11 times what that loses; lo: what lse2 lost when it was rounded
+    // EPI_PROB: P = f16((2^(z2 - lse2 - lo) - [label]) * pf), and 2^11 times what that loses; lo: what lse2 lost when it was rounded.  f32 operands:
+    // P = (2^(z2 - lse2 - lo) - [label]) * pf * h[col] as f32
     const float* lo;
     uint16_t* prob;
     uint64_t prob_plane;         // elements
@@ -75,7 +77,11 @@ struct ProductArgs {
     uint64_t raw_ld;
 };
 
-constexpr int kBK = 64;
+// A step is 128 bytes of k: 64 16-bit elements, 32 f32.
+template <int KIND>
+constexpr uint32_t kES = KIND == K_F32 ? 4u : 2u;
+template <int KIND>
+constexpr uint32_t kBK = 128u / kES<KIND>;
 
 __device__ __forceinline__ uint32_t swz_row(uint32_t row) { return (row >> 1) & 7u; }
 template <int COLS>
@@ -86,8 +92,9 @@ __device__ __forceinline__ uint32_t swz_k(uint32_t k) {
 // One operand's stages: 64 deep, X output rows / columns wide (X * 128 bytes of LDS), brought in by NW waves in pieces of 1 KiB.  Between
 // two steps only a scalar moves; the instructions between a step's barrier and its first MFMA are what every wave of the CU waits for
 // (a descriptor computed per step cost 190 of 800 us at 4,096 x 131,072 x 768).
-template <int X, int NW, bool ACROSS>
+template <int X, int NW, bool ACROSS, int KIND>
 struct Loader {
+    static constexpr uint32_t ES = kES<KIND>, BK = kBK<KIND>;
     static constexpr int PIECES = X / 8 / NW;
     static_assert(X % (8 * NW) == 0, "whole pieces per wave");
     uint32_t off[PIECES];
@@ -98,8 +105,8 @@ struct Loader {
         for (int i = 0; i < PIECES; ++i) {
             const uint32_t at = (w * PIECES + i) * 1024u + lane * 16u;
             if constexpr (ACROSS) {
-                const uint32_t kr = at / (X * 2), cp = (at % (X * 2)) >> 4;
-                const uint32_t c = ((((cp >> 1) ^ swz_k<X>(kr)) << 1) | (cp & 1u));
+                const uint32_t kr = at / (X * ES), cp = (at % (X * ES)) >> 4;
+                const uint32_t c = KIND == K_F32 ? cp ^ (((kr >> 2) & 3u) << 2) : cp ^ (swz_k<X>(kr) << 1);
                 off[i] = kr * (uint32_t)ld + c * 16u;
             } else {
                 const uint32_t row = at >> 7, cp = (at >> 4) & 7u;
@@ -111,8 +118,8 @@ struct Loader {
     // x0: first output row / column of the tile; k0: first k of the step; kend: end of k
     __device__ __forceinline__ void open(const Operand& o, uint32_t plane, uint32_t x0, uint32_t k0, uint32_t kend) {
         if constexpr (ACROSS) {
-            base = o.p + plane * o.plane + (uint64_t)k0 * o.ld + (uint64_t)x0 * 2u;
-            full = x0 < o.cols ? clamped((kBK - 1u) * o.ld + (uint64_t)(o.cols - x0) * 2u) : 0u;
+            base = o.p + plane * o.plane + (uint64_t)k0 * o.ld + (uint64_t)x0 * ES;
+            full = x0 < o.cols ? clamped((BK - 1u) * o.ld + (uint64_t)(o.cols - x0) * ES) : 0u;
             depth(o, k0, kend);
         } else {
             base = o.p + plane * o.plane + (uint64_t)x0 * o.ld;
@@ -121,12 +128,12 @@ struct Loader {
     }
     __device__ __forceinline__ void depth(const Operand& o, uint32_t k0, uint32_t kend) {
         const uint32_t left = k0 < kend ? kend - k0 : 0u;
-        const uint32_t less = left < (uint32_t)kBK ? (kBK - left) * (uint32_t)o.ld : 0u;
+        const uint32_t less = left < BK ? (BK - left) * (uint32_t)o.ld : 0u;
         limit = left && less < full ? full - less : 0u;
     }
     __device__ __forceinline__ void advance(const Operand& o, uint32_t k0, uint32_t kend) {  // to the next step, at k0
         if constexpr (ACROSS) {
-            base += (uint64_t)kBK * o.ld;
+            base += (uint64_t)BK * o.ld;
             depth(o, k0, kend);
         }
     }
@@ -135,13 +142,13 @@ struct Loader {
         const uint32_t bytes = __builtin_amdgcn_readfirstlane(more ? limit : 0u), lo = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)base),
                        hi = __builtin_amdgcn_readfirstlane((uint32_t)((uintptr_t)base >> 32));
         const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)((uintptr_t)hi << 32 | lo), 0, (int)bytes, 0x00020000);
-        const bool tail = !ACROSS && k0 + kBK > kend;  // the last step of a depth that is no multiple of 64: chunks beyond it read nothing
-        const uint32_t shift = ACROSS || tail ? 0u : k0 * 2u;
+        const bool tail = !ACROSS && k0 + BK > kend;  // the last step of a depth that is no multiple of a step: chunks beyond it read nothing
+        const uint32_t shift = ACROSS || tail ? 0u : k0 * ES;
         uint32_t v = off[i];
         if (tail) {
             const uint32_t row = (w * PIECES + i) * 8u + (lane >> 3);
-            const uint32_t kc = ((lane & 7u) ^ swz_row(row)) * 8u;
-            v = k0 + kc < kend ? v + k0 * 2u : 0x7FFFFFF0u;
+            const uint32_t kc = ((lane & 7u) ^ swz_row(row)) * (16u / ES);
+            v = k0 + kc < kend ? v + k0 * ES : 0x7FFFFFF0u;
         }
         __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(lds + (w * PIECES + i) * 1024u), 16, v, shift, 0, 0);
     }
@@ -198,10 +205,19 @@ __device__ __forceinline__ void read_across2(const uint32_t* a, s16x8* f) {
     f[0] = __builtin_shufflevector(l0, h0, 0, 1, 2, 3, 4, 5, 6, 7);
     f[1] = __builtin_shufflevector(l1, h1, 0, 1, 2, 3, 4, 5, 6, 7);
 }
-// T fragments of one operand; at: LDS byte address of its stage
-template <int X, int T, bool ACROSS, int KK, class Frag>
+// T fragments of one operand; at: LDS byte address of its stage.  f32: a lane's four elements are those of four MFMAs, k = kk * 16 +
+// 4 * (lane / 16) + 0..3 (which k an MFMA multiplies does not matter as long as both operands agree).
+template <int X, int T, bool ACROSS, int KIND, int KK, class Frag>
 __device__ __forceinline__ void read_fragments(const char* lds, uint32_t at, uint32_t x, uint32_t lane, const uint32_t* addr, Frag* f) {
-    if constexpr (ACROSS) {
+    if constexpr (ACROSS && KIND == K_F32) {
+        const uint32_t g = lane >> 4;
+#pragma unroll
+        for (int i = 0; i < T; ++i) {
+            const uint32_t col = ((x + i * 16u + (lane & 15u)) * 4u) ^ (g << 6);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) f[i][t] = *reinterpret_cast<const float*>(lds + (KK * 16u + g * 4u + t) * (X * 4u) + col);
+        }
+    } else if constexpr (ACROSS) {
         uint32_t a[T];
         s16x8 v[T];
 #pragma unroll
@@ -223,15 +239,24 @@ __device__ __forceinline__ void read_fragments(const char* lds, uint32_t at, uin
     }
 }
 
-template <bool BF16>
-struct Half {
+// MFMAS: how many a fragment feeds
+template <int KIND>
+struct Matrix {
+    static constexpr int MFMAS = 1;
     using frag = __attribute__((ext_vector_type(8))) _Float16;
-    static __device__ __forceinline__ f32x4 mma(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ f32x4 mma(frag a, frag b, f32x4 c, int) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 template <>
-struct Half<true> {
+struct Matrix<K_BF16> {
+    static constexpr int MFMAS = 1;
     using frag = __attribute__((ext_vector_type(8))) __bf16;
-    static __device__ __forceinline__ f32x4 mma(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ f32x4 mma(frag a, frag b, f32x4 c, int) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Matrix<K_F32> {
+    static constexpr int MFMAS = 4;
+    using frag = f32x4;
+    static __device__ __forceinline__ f32x4 mma(frag a, frag b, f32x4 c, int t) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a[t], b[t], c, 0, 0, 0); }
 };
 
 // 16 rows x 64 columns of 16-bit values, four consecutive columns of a row per lane and block, to memory as whole 128-byte lines: straight
@@ -261,6 +286,46 @@ __device__ __forceinline__ void store_lines(char* scratch, const ushort4 (&v)[4]
     }
 }
 
+// 16 rows x 64 columns of f32 alike, 32 columns at a time.  tc: the row's (lane & 15) factor on `raw` * ti, subtracted on the way (0: nothing to
+// subtract; in this order: 1 / |row|^2 may not exist in f32).
+template <int ROWS>
+__device__ __forceinline__ void store_lines(char* scratch, const f32x4 (&v)[4], float* to, uint64_t ld, uint32_t row, uint32_t rows, uint32_t col, uint32_t cols,
+                                            uint32_t lane, const float* raw = nullptr, uint64_t raw_ld = 0, float tc = 0.f, float ti = 0.f) {
+    const uint32_t r = lane & 15u, q = lane >> 4, c = lane & 7u;
+#pragma unroll
+    for (uint32_t half = 0; half < 2; ++half)
+#pragma unroll
+        for (uint32_t part = 0; part < 16u / ROWS; ++part) {
+            f32x4 less[ROWS / 8];
+            const uint32_t at = col + half * 32u + c * 4u;
+            if (raw) {
+#pragma unroll
+                for (uint32_t h = 0; h < ROWS / 8; ++h) {
+                    const uint32_t rr = part * ROWS + h * 8u + (lane >> 3);
+                    less[h] = row + rr < rows && at < cols ? *reinterpret_cast<const f32x4*>(raw + (uint64_t)(row + rr) * raw_ld + at) : f32x4{0.f, 0.f, 0.f, 0.f};
+                }
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the last block has been read)
+            if (ROWS == 16 || r / ROWS == part) {
+#pragma unroll
+                for (uint32_t j = 0; j < 2; ++j) *reinterpret_cast<f32x4*>(scratch + (r % ROWS) * 128u + (((j * 4u + q) ^ (r & 7u)) << 4)) = v[half * 2u + j];
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (uint32_t h = 0; h < ROWS / 8; ++h) {
+                const uint32_t in = h * 8u + (lane >> 3), rr = part * ROWS + in;
+                f32x4 x = *reinterpret_cast<const f32x4*>(scratch + in * 128u + ((c ^ (in & 7u)) << 4));
+                if (raw) {
+                    const float t = __shfl(tc, rr), i = __shfl(ti, rr);
+                    if (t != 0.f) x -= less[h] * i * t;
+                }
+                if (row + rr < rows && at < cols) *reinterpret_cast<f32x4*>(to + (uint64_t)(row + rr) * ld + at) = x;
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+}
+
 // WM x WN waves, each MT x NT blocks of 16 x 16.
 template <int TM_, int TN_, int WM_, int WN_, int RING_>
 struct Shape {
@@ -278,10 +343,11 @@ using Large = Shape<256, 256, 2, 4, 2>;   // one workgroup per CU, 152 KiB of LD
 using Medium = Shape<128, 256, 2, 4, 3>;  // one workgroup per CU, 158 KiB
 using Small = Shape<64, 128, 2, 2, 2>;    // 58 KiB: two workgroups per CU
 
-template <class S, int FORM, int EPI, bool BF16>
+template <class S, int FORM, int EPI, int KIND>
 __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
     constexpr bool A_ACROSS = FORM == DW, B_ACROSS = FORM != SCORES;
-    using H = Half<BF16>;
+    constexpr uint32_t BK = kBK<KIND>;
+    using H = Matrix<KIND>;
     using frag = typename H::frag;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const uint32_t lane = threadIdx.x & 63u, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = w / S::WN, wn = w % S::WN;
@@ -304,8 +370,8 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
         tm = in / width;
         tn = group * GROUP + in % width;
     };
-    Loader<S::TM, S::NW, A_ACROSS> la;
-    Loader<S::TN, S::NW, B_ACROSS> lb;
+    Loader<S::TM, S::NW, A_ACROSS, KIND> la;
+    Loader<S::TN, S::NW, B_ACROSS, KIND> lb;
     la.init(g.a.ld, w, lane);
     lb.init(g.b.ld, w, lane);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
@@ -320,7 +386,7 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
     char* const row_buffers = lds + S::RING * S::STAGE;  // SOFTMAX: the row factors of RING tiles (a tile may be one step)
     uint32_t p = 0, p_tile = tile0, p_seg = 0, p_ks = 0, p_tm, p_tn, p_sp, p_k0, p_parity = 0;
     const auto open = [&]() {
-        p_k0 = p_sp * g.ksteps * kBK;
+        p_k0 = p_sp * g.ksteps * BK;
         la.open(g.a, (g.seg_a >> (4u * p_seg)) & 15u, p_tm * S::TM, p_k0, g.k);
         lb.open(g.b, (g.seg_b >> (4u * p_seg)) & 15u, p_tn * S::TN, p_k0, g.k);
     };
@@ -336,7 +402,7 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
     const auto advance = [&]() {
         ++p;
         if (++p_ks < g.ksteps) {
-            p_k0 += kBK;
+            p_k0 += BK;
             la.advance(g.a, p_k0, g.k);
             lb.advance(g.b, p_k0, g.k);
             return;
@@ -383,7 +449,7 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
             asm volatile("" ::: "memory");
             prefetch_rows();
             if constexpr (FORM != SCORES) {
-                if (g.lo_first && s == g.ksteps) {
+                if (KIND == K_F16 && g.lo_first && s == g.ksteps) {
 #pragma unroll
                     for (int i = 0; i < S::MT; ++i)
 #pragma unroll
@@ -396,12 +462,12 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
             // The next stage's loads go out one by one between the MFMAs of the step's first half: issued in a row they fill the queue of the
             // load unit (16 cycles each, 64 of them per CU), and every wave stands in front of its first MFMA until its own are through.
             frag fa[S::MT], fb[S::NT];
-            read_fragments<S::TM, S::MT, A_ACROSS, 0>(sa, lds0 + stage, wm * S::MT * 16u, lane, aa, fa);
-            read_fragments<S::TN, S::NT, B_ACROSS, 0>(sb, lds0 + stage + S::A_BYTES, wn * S::NT * 16u, lane, ab, fb);
+            read_fragments<S::TM, S::MT, A_ACROSS, KIND, 0>(sa, lds0 + stage, wm * S::MT * 16u, lane, aa, fa);
+            read_fragments<S::TN, S::NT, B_ACROSS, KIND, 0>(sb, lds0 + stage + S::A_BYTES, wn * S::NT * 16u, lane, ab, fb);
 #pragma unroll
             for (int i = 0; i < S::MT; ++i) {
 #pragma unroll
-                for (int j = 0; j < S::NT; ++j) acc[i][j] = H::mma(fb[j], fa[i], acc[i][j]);
+                for (int j = 0; j < S::NT; ++j) acc[i][j] = H::mma(fb[j], fa[i], acc[i][j], 0);
                 __builtin_amdgcn_sched_barrier(0x104);  // (scalar instructions and LDS reads may pass)
 #pragma unroll
                 for (int x = i * P / S::MT; x < (i + 1) * P / S::MT; ++x) {
@@ -410,12 +476,20 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                 }
                 __builtin_amdgcn_sched_barrier(0x104);
             }
-            read_fragments<S::TM, S::MT, A_ACROSS, 1>(sa, lds0 + stage, wm * S::MT * 16u, lane, aa, fa);
-            read_fragments<S::TN, S::NT, B_ACROSS, 1>(sb, lds0 + stage + S::A_BYTES, wn * S::NT * 16u, lane, ab, fb);
 #pragma unroll
-            for (int i = 0; i < S::MT; ++i)
+            for (int t = 1; t < H::MFMAS; ++t)
 #pragma unroll
-                for (int j = 0; j < S::NT; ++j) acc[i][j] = H::mma(fb[j], fa[i], acc[i][j]);
+                for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < S::NT; ++j) acc[i][j] = H::mma(fb[j], fa[i], acc[i][j], t);
+            read_fragments<S::TM, S::MT, A_ACROSS, KIND, 1>(sa, lds0 + stage, wm * S::MT * 16u, lane, aa, fa);
+            read_fragments<S::TN, S::NT, B_ACROSS, KIND, 1>(sb, lds0 + stage + S::A_BYTES, wn * S::NT * 16u, lane, ab, fb);
+#pragma unroll
+            for (int t = 0; t < H::MFMAS; ++t)
+#pragma unroll
+                for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < S::NT; ++j) acc[i][j] = H::mma(fb[j], fa[i], acc[i][j], t);
             advance();
             next_at = stage;
             stage = stage + S::STAGE < S::RING * S::STAGE ? stage + S::STAGE : 0u;
@@ -594,6 +668,15 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
 #pragma unroll
                             for (int r = 0; r < 4; ++r) v[j][r] = label < 0 ? 0.f : v[j][r];
                     }
+                    if constexpr (KIND == K_F32) {  // f32 probabilities carry every factor
+                        f32x4 x[S::NT];
+#pragma unroll
+                        for (int j = 0; j < S::NT; ++j)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) x[j][r] = plain || !((live[j] >> r) & 1u) ? v[j][r] * rf.z : v[j][r] * rf.z * h[j][r];
+                        store_lines<S::SCRATCH / 128>(scratch, x, reinterpret_cast<float*>(g.prob), g.prob_ld, row0 - (lane & 15u) + i * 16u, g.m, c0, g.prob_ld, lane);
+                        continue;
+                    }
                     ushort4 hi[S::NT], lo[S::NT];
 #pragma unroll
                     for (int j = 0; j < S::NT; ++j) {
@@ -613,17 +696,25 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
         } else if constexpr (EPI == EPI_PART) {
             float* to = g.out_part + (size_t)sp * g.m * g.n;
 #pragma unroll
-            for (int i = 0; i < S::MT; ++i) {
-                const uint32_t row = row0 + i * 16u;
-#pragma unroll
-                for (int j = 0; j < S::NT; ++j) {
-                    const uint32_t c = cl + j * 16u;
-                    if (row < g.m && c < g.n) *reinterpret_cast<f32x4*>(to + (size_t)row * g.n + c) = acc[i][j];  // (n: a multiple of 4)
-                }
-            }
+            for (int i = 0; i < S::MT; ++i) store_lines<S::SCRATCH / 128>(scratch, acc[i], to, g.n, row0 - (lane & 15u) + i * 16u, g.m, c0, g.n, lane);  // (n: a multiple of 4)
         } else {
             const float wf = g.wf ? *g.wf : 1.f;
-            const bool lines = g.out_scalar != SC_F32 && g.n % 8u == 0 && g.out_ld % 8u == 0 && ((uintptr_t)g.out & 15u) == 0;
+            const bool full = g.out_scalar == SC_F32, fits = g.n % 8u == 0 && g.out_ld % 8u == 0 && ((uintptr_t)g.out & 15u) == 0;
+            const bool lines = !full && fits, wide = full && fits && (!g.tcoef || (g.raw_ld % 4u == 0 && ((uintptr_t)g.raw & 15u) == 0));
+            if (wide) {
+#pragma unroll
+                for (int i = 0; i < S::MT; ++i) {
+                    const uint32_t row = row0 + i * 16u;
+                    const bool has = row < g.m;
+                    const float rf = has && g.rf ? g.rf[row] * wf : wf;
+                    f32x4 x[S::NT];
+#pragma unroll
+                    for (int j = 0; j < S::NT; ++j) x[j] = acc[i][j] * rf;
+                    store_lines<S::SCRATCH / 128>(scratch, x, (float*)g.out, g.out_ld, row - (lane & 15u), g.m, c0, g.n, lane, g.tcoef ? (const float*)g.raw : nullptr,
+                                                  g.raw_ld, has && g.tcoef ? g.tcoef[row] : 0.f, has && g.tcoef ? g.tinv[row] : 0.f);
+                }
+                continue;
+            }
 #pragma unroll
             for (int i = 0; i < S::MT; ++i) {
                 const uint32_t row = row0 + i * 16u;
