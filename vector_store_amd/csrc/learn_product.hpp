@@ -286,25 +286,23 @@ __device__ __forceinline__ void store_lines(char* scratch, const ushort4 (&v)[4]
     }
 }
 
-// 16 rows x 64 columns of f32 alike, 32 columns at a time.  tc: the row's (lane & 15) factor on `raw` * ti, subtracted on the way (0: nothing to
-// subtract; in this order: 1 / |row|^2 may not exist in f32).
+// 16 rows x 64 columns of f32 alike, 32 columns at a time.  less: what is subtracted on the way (load_lines of a table) times ti times tc, the row's
+// (lane & 15) factors (in this order: 1 / |row|^2 may not exist in f32; tc 0: nothing is).
+__device__ __forceinline__ void load_lines(const float* from, uint64_t ld, uint32_t row, uint32_t rows, uint32_t col, uint32_t cols, uint32_t lane, f32x4 (&v)[4]) {
+#pragma unroll
+    for (uint32_t x = 0; x < 4; ++x) {
+        const uint32_t rr = (x & 1u) * 8u + (lane >> 3), at = col + (x >> 1) * 32u + (lane & 7u) * 4u;
+        v[x] = row + rr < rows && at < cols ? *reinterpret_cast<const f32x4*>(from + (uint64_t)(row + rr) * ld + at) : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+}
 template <int ROWS>
 __device__ __forceinline__ void store_lines(char* scratch, const f32x4 (&v)[4], float* to, uint64_t ld, uint32_t row, uint32_t rows, uint32_t col, uint32_t cols,
-                                            uint32_t lane, const float* raw = nullptr, uint64_t raw_ld = 0, float tc = 0.f, float ti = 0.f) {
+                                            uint32_t lane, const f32x4* less = nullptr, float tc = 0.f, float ti = 0.f) {
     const uint32_t r = lane & 15u, q = lane >> 4, c = lane & 7u;
 #pragma unroll
     for (uint32_t half = 0; half < 2; ++half)
 #pragma unroll
         for (uint32_t part = 0; part < 16u / ROWS; ++part) {
-            f32x4 less[ROWS / 8];
-            const uint32_t at = col + half * 32u + c * 4u;
-            if (raw) {
-#pragma unroll
-                for (uint32_t h = 0; h < ROWS / 8; ++h) {
-                    const uint32_t rr = part * ROWS + h * 8u + (lane >> 3);
-                    less[h] = row + rr < rows && at < cols ? *reinterpret_cast<const f32x4*>(raw + (uint64_t)(row + rr) * raw_ld + at) : f32x4{0.f, 0.f, 0.f, 0.f};
-                }
-            }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the last block has been read)
             if (ROWS == 16 || r / ROWS == part) {
 #pragma unroll
@@ -314,11 +312,11 @@ __device__ __forceinline__ void store_lines(char* scratch, const f32x4 (&v)[4], 
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
             for (uint32_t h = 0; h < ROWS / 8; ++h) {
-                const uint32_t in = h * 8u + (lane >> 3), rr = part * ROWS + in;
+                const uint32_t in = h * 8u + (lane >> 3), rr = part * ROWS + in, at = col + half * 32u + c * 4u;
                 f32x4 x = *reinterpret_cast<const f32x4*>(scratch + in * 128u + ((c ^ (in & 7u)) << 4));
-                if (raw) {
+                if (less) {
                     const float t = __shfl(tc, rr), i = __shfl(ti, rr);
-                    if (t != 0.f) x -= less[h] * i * t;
+                    if (t != 0.f) x -= less[half * 2u + part * ROWS / 8u + h] * i * t;
                 }
                 if (row + rr < rows && at < cols) *reinterpret_cast<f32x4*>(to + (uint64_t)(row + rr) * ld + at) = x;
             }
@@ -346,7 +344,9 @@ using Small = Shape<64, 128, 2, 2, 2>;    // 58 KiB: two workgroups per CU
 template <class S, int FORM, int EPI, int KIND>
 __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
     constexpr bool A_ACROSS = FORM == DW, B_ACROSS = FORM != SCORES;
+    constexpr bool SOFTMAX = FORM == SCORES;
     constexpr uint32_t BK = kBK<KIND>;
+    constexpr int SCRATCH = S::SCRATCH;
     using H = Matrix<KIND>;
     using frag = typename H::frag;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
@@ -382,7 +382,6 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
     for (int j = 0; j < S::NT; ++j) ab[j] = B_ACROSS ? across_address<S::TN>((wn * S::NT + j) * 16u, lane) : 0u;
     const uint32_t steps = g.ksteps * g.segs;
     const uint32_t total = ((mine - 1u - tile0) / step + 1u) * steps;
-    constexpr bool SOFTMAX = FORM == SCORES;
     char* const row_buffers = lds + S::RING * S::STAGE;  // SOFTMAX: the row factors of RING tiles (a tile may be one step)
     uint32_t p = 0, p_tile = tile0, p_seg = 0, p_ks = 0, p_tm, p_tn, p_sp, p_k0, p_parity = 0;
     const auto open = [&]() {
@@ -437,11 +436,17 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
     for (uint32_t tile = tile0; tile < mine; tile += step, parity = parity + 1u < (uint32_t)S::RING ? parity + 1u : 0u) {
         uint32_t tm, tn, sp;
         place(tile, tm, tn, sp);
-        f32x4 acc[S::MT][S::NT];
+        // (f32 scores in two sums, added at the end: half of the terms and of the size each, so less rounding; four leave one wave per SIMD)
+        constexpr int SUMS = SOFTMAX && KIND == K_F32 ? 2 : 1;
+        f32x4 acc[S::MT][S::NT], more[SUMS][S::MT][S::NT];
 #pragma unroll
         for (int i = 0; i < S::MT; ++i)
 #pragma unroll
-            for (int j = 0; j < S::NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int j = 0; j < S::NT; ++j) {
+                acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int t = 1; t < SUMS; ++t) more[t][i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
         for (uint32_t s = 0; s < steps; ++s) {
             // (a wave's loads arrive in order: what may still be on its way are the P pieces of the stages after this one)
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S::RING - 2) * P) : "memory");
@@ -481,7 +486,10 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
 #pragma unroll
                 for (int i = 0; i < S::MT; ++i)
 #pragma unroll
-                    for (int j = 0; j < S::NT; ++j) acc[i][j] = H::mma(fb[j], fa[i], acc[i][j], t);
+                    for (int j = 0; j < S::NT; ++j) {
+                        f32x4& c = t % SUMS ? more[t % SUMS][i][j] : acc[i][j];
+                        c = H::mma(fb[j], fa[i], c, t);
+                    }
             read_fragments<S::TM, S::MT, A_ACROSS, KIND, 1>(sa, lds0 + stage, wm * S::MT * 16u, lane, aa, fa);
             read_fragments<S::TN, S::NT, B_ACROSS, KIND, 1>(sb, lds0 + stage + S::A_BYTES, wn * S::NT * 16u, lane, ab, fb);
 #pragma unroll
@@ -489,15 +497,24 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
 #pragma unroll
                 for (int i = 0; i < S::MT; ++i)
 #pragma unroll
-                    for (int j = 0; j < S::NT; ++j) acc[i][j] = H::mma(fb[j], fa[i], acc[i][j], t);
+                    for (int j = 0; j < S::NT; ++j) {
+                        f32x4& c = t % SUMS ? more[t % SUMS][i][j] : acc[i][j];
+                        c = H::mma(fb[j], fa[i], c, t);
+                    }
             advance();
             next_at = stage;
             stage = stage + S::STAGE < S::RING * S::STAGE ? stage + S::STAGE : 0u;
         }
+#pragma unroll
+        for (int t = 1; t < SUMS; ++t)
+#pragma unroll
+            for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+                for (int j = 0; j < S::NT; ++j) acc[i][j] += more[t][i][j];
         // lane: row (lane & 15) of a 16 x 16 block, columns 4 * (lane / 16) + 0..3
         const uint32_t row0 = tm * S::TM + wm * S::MT * 16u + (lane & 15u);
         const uint32_t c0 = tn * S::TN + wn * S::NT * 16u, cl = c0 + (lane >> 4) * 4u;
-        char* scratch = lds + S::RING * (S::STAGE + S::ROW_BYTES) + w * (uint32_t)S::SCRATCH;
+        char* scratch = lds + S::RING * (S::STAGE + S::ROW_BYTES) + w * (uint32_t)SCRATCH;
         if constexpr (SOFTMAX) {
             const float4* rows = reinterpret_cast<const float4*>(row_buffers + parity * S::ROW_BYTES);
             // columns that all exist and have no factor of their own: the common case, with fewer instructions per score (the epilogue's
@@ -674,7 +691,7 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                         for (int j = 0; j < S::NT; ++j)
 #pragma unroll
                             for (int r = 0; r < 4; ++r) x[j][r] = plain || !((live[j] >> r) & 1u) ? v[j][r] * rf.z : v[j][r] * rf.z * h[j][r];
-                        store_lines<S::SCRATCH / 128>(scratch, x, reinterpret_cast<float*>(g.prob), g.prob_ld, row0 - (lane & 15u) + i * 16u, g.m, c0, g.prob_ld, lane);
+                        store_lines<SCRATCH / 128>(scratch, x, reinterpret_cast<float*>(g.prob), g.prob_ld, row0 - (lane & 15u) + i * 16u, g.m, c0, g.prob_ld, lane);
                         continue;
                     }
                     ushort4 hi[S::NT], lo[S::NT];
@@ -688,20 +705,23 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                             lo[j].z = to_half<false>((v[j][2] - from_half<false>(hi[j].z)) * 2048.f), lo[j].w = to_half<false>((v[j][3] - from_half<false>(hi[j].w)) * 2048.f);
                         }
                     }
-                    store_lines<S::SCRATCH / 128>(scratch, hi, g.prob, g.prob_ld, row0 - (lane & 15u) + i * 16u, g.m, c0, g.prob_ld, lane);
-                    if (g.prob_planes > 1) store_lines<S::SCRATCH / 128>(scratch, lo, g.prob + g.prob_plane, g.prob_ld, row0 - (lane & 15u) + i * 16u, g.m, c0, g.prob_ld, lane);
+                    store_lines<SCRATCH / 128>(scratch, hi, g.prob, g.prob_ld, row0 - (lane & 15u) + i * 16u, g.m, c0, g.prob_ld, lane);
+                    if (g.prob_planes > 1) store_lines<SCRATCH / 128>(scratch, lo, g.prob + g.prob_plane, g.prob_ld, row0 - (lane & 15u) + i * 16u, g.m, c0, g.prob_ld, lane);
                     __builtin_amdgcn_sched_barrier(0);  // one block of rows at a time: interleaved, they do not fit the registers
                 }
             }
         } else if constexpr (EPI == EPI_PART) {
             float* to = g.out_part + (size_t)sp * g.m * g.n;
 #pragma unroll
-            for (int i = 0; i < S::MT; ++i) store_lines<S::SCRATCH / 128>(scratch, acc[i], to, g.n, row0 - (lane & 15u) + i * 16u, g.m, c0, g.n, lane);  // (n: a multiple of 4)
+            for (int i = 0; i < S::MT; ++i) store_lines<SCRATCH / 128>(scratch, acc[i], to, g.n, row0 - (lane & 15u) + i * 16u, g.m, c0, g.n, lane);  // (n: a multiple of 4)
         } else {
             const float wf = g.wf ? *g.wf : 1.f;
             const bool full = g.out_scalar == SC_F32, fits = g.n % 8u == 0 && g.out_ld % 8u == 0 && ((uintptr_t)g.out & 15u) == 0;
             const bool lines = !full && fits, wide = full && fits && (!g.tcoef || (g.raw_ld % 4u == 0 && ((uintptr_t)g.raw & 15u) == 0));
             if (wide) {
+                constexpr bool AHEAD = S::MT <= 4;  // a block of rows ahead, or each one's reading is waited for (the large tile has no registers left)
+                f32x4 less[2][4];
+                if (AHEAD && g.tcoef) load_lines((const float*)g.raw, g.raw_ld, row0 - (lane & 15u), g.m, c0, g.n, lane, less[0]);
 #pragma unroll
                 for (int i = 0; i < S::MT; ++i) {
                     const uint32_t row = row0 + i * 16u;
@@ -710,8 +730,12 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                     f32x4 x[S::NT];
 #pragma unroll
                     for (int j = 0; j < S::NT; ++j) x[j] = acc[i][j] * rf;
-                    store_lines<S::SCRATCH / 128>(scratch, x, (float*)g.out, g.out_ld, row - (lane & 15u), g.m, c0, g.n, lane, g.tcoef ? (const float*)g.raw : nullptr,
-                                                  g.raw_ld, has && g.tcoef ? g.tcoef[row] : 0.f, has && g.tcoef ? g.tinv[row] : 0.f);
+                    if (g.tcoef) {
+                        const int next = AHEAD ? i + 1 : i;
+                        if (next < S::MT) load_lines((const float*)g.raw, g.raw_ld, row0 - (lane & 15u) + next * 16u, g.m, c0, g.n, lane, less[next & 1]);
+                        store_lines<SCRATCH / 128>(scratch, x, (float*)g.out, g.out_ld, row - (lane & 15u), g.m, c0, g.n, lane, less[i & 1], has ? g.tcoef[row] : 0.f,
+                                                   has ? g.tinv[row] : 0.f);
+                    } else store_lines<SCRATCH / 128>(scratch, x, (float*)g.out, g.out_ld, row - (lane & 15u), g.m, c0, g.n, lane);
                 }
                 continue;
             }
@@ -730,7 +754,7 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                     if (lines) o[j] = to_half4(g.out_scalar, v);
                     else if (has && c < g.n) store4(g.out, g.out_scalar, (uint64_t)row * g.out_ld + c, v, g.n - c);
                 }
-                if (lines) store_lines<S::SCRATCH / 128>(scratch, o, (uint16_t*)g.out, g.out_ld, row0 - (lane & 15u) + i * 16u, g.m, c0, g.n, lane);
+                if (lines) store_lines<SCRATCH / 128>(scratch, o, (uint16_t*)g.out, g.out_ld, row0 - (lane & 15u) + i * 16u, g.m, c0, g.n, lane);
             }
         }
     }
