@@ -517,9 +517,9 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
         char* scratch = lds + S::RING * (S::STAGE + S::ROW_BYTES) + w * (uint32_t)SCRATCH;
         if constexpr (SOFTMAX) {
             const float4* rows = reinterpret_cast<const float4*>(row_buffers + parity * S::ROW_BYTES);
-            // columns that all exist and have no factor of their own: the common case, with fewer instructions per score (the epilogue's
-            // vector instructions are what a product of short rows waits for: 128 scores per lane)
-            const bool plain = !g.h && !g.keys && c0 + S::NT * 16u <= g.n;
+            // columns that all exist: the common case, with fewer instructions per score (the epilogue's vector instructions are what a product of
+            // short rows waits for: 128 scores per lane)
+            const bool plain = !g.keys && c0 + S::NT * 16u <= g.n;
             f32x4 h[S::NT];
             uint32_t live[S::NT];  // bit r: column j, r exists
             if (!plain) {
@@ -534,6 +534,17 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                         h[j][r] = in ? (g.h ? g.h[c] : 1.f) : 0.f;
                     }
                 }
+            } else if (g.h) {
+#pragma unroll
+                for (int j = 0; j < S::NT; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) h[j][r] = g.h[cl + j * 16u + r];
+            }
+            if (g.h) {
+#pragma unroll
+                for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < S::NT; ++j) acc[i][j] *= h[j];
             }
             if constexpr (EPI == EPI_LOSS) {
                 float2* red = reinterpret_cast<float2*>(lds + S::RING * (S::STAGE + S::ROW_BYTES));
@@ -564,7 +575,7 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                         for (int j = 0; j < S::NT; ++j)
 #pragma unroll
                             for (int r = 0; r < 4; ++r) {
-                                const float fh = plain ? f : f * h[j][r], z = acc[i][j][r] * fh;
+                                const float z = acc[i][j][r] * f;
                                 bool in = plain || ((live[j] >> r) & 1u);
                                 if (lab == j * 16u + r) {
                                     if (row0 + i * 16u < g.m) g.zlab[row0 + i * 16u] = z;
@@ -577,7 +588,7 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                         for (int j = 0; j < S::NT; ++j)
 #pragma unroll
                             for (int r = 0; r < 4; ++r) {
-                                const float e = exp2_fast(fmaf(acc[i][j][r], plain ? f : f * h[j][r], -base));
+                                const float e = exp2_fast(fmaf(acc[i][j][r], f, -base));
                                 sum += (plain || ((live[j] >> r) & 1u)) && lab != j * 16u + r ? e : 0.f;
                             }
                     }
@@ -636,8 +647,8 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                             asm volatile("" : "+v"(f));  // (or the compiler keeps all 128 probabilities for the next pass)
 #pragma unroll
                             for (int r = 0; r < 4; ++r) {
-                                const float fh = plain ? f : f * h[j][r], z = acc[i][j][r] * fh;
-                                const float q = exp2_fast(fmaf(acc[i][j][r], fh, -rf.y) - lo[i]) - (lab == (uint32_t)r ? 1.f : 0.f);
+                                const float z = acc[i][j][r] * f;
+                                const float q = exp2_fast(fmaf(acc[i][j][r], f, -rf.y) - lo[i]) - (lab == (uint32_t)r ? 1.f : 0.f);
                                 t[r] += __float_as_int(rf.w) >= 0 && (plain || ((live[j] >> r) & 1u)) ? q * z * gr[i] : 0.f;
                             }
                         }
@@ -669,7 +680,7 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
 #pragma unroll
                         for (int j = 0; j < S::NT; ++j)
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) v[j][r] = (live[j] >> r) & 1u ? exp2_fast(fmaf(acc[i][j][r], f * h[j][r], -rf.y)) : 0.f;
+                            for (int r = 0; r < 4; ++r) v[j][r] = (live[j] >> r) & 1u ? exp2_fast(fmaf(acc[i][j][r], f, -rf.y)) : 0.f;
                     }
                     if (__any(lab < S::NT * 16u)) {
                         const float one = lab < S::NT * 16u && row0 + i * 16u < g.m ? exp2_fast(g.lo[row0 + i * 16u]) : 1.f;
@@ -690,7 +701,7 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
 #pragma unroll
                         for (int j = 0; j < S::NT; ++j)
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) x[j][r] = plain || !((live[j] >> r) & 1u) ? v[j][r] * rf.z : v[j][r] * rf.z * h[j][r];
+                            for (int r = 0; r < 4; ++r) x[j][r] = g.h ? v[j][r] * rf.z * h[j][r] : v[j][r] * rf.z;  // (v is 0 where h is)
                         store_lines<SCRATCH / 128>(scratch, x, reinterpret_cast<float*>(g.prob), g.prob_ld, row0 - (lane & 15u) + i * 16u, g.m, c0, g.prob_ld, lane);
                         continue;
                     }
