@@ -33,7 +33,7 @@ static void launched(const char* what) { hip_ok(hipGetLastError(), what); }
 // same on the f16 pipe.  Everything else (f32 anywhere, mixed types, f16 under cosine) is split into f16 planes, x = hi + lo with hi = f16(x),
 // lo = f16(x - hi): 22 bits of x.  Three of the four products of two such numbers are summed (lo lo is below 2^-22 of the result), which is
 // f32's accuracy at three times the f16 product's cost -- the matrix pipe's f32 product costs sixteen.  (A few f32 queries of f32 rows are
-// multiplied as f32 all the same, probabilities included: the time is the rows' reading then; kFullLoss.)  f16's narrow range is met by
+// multiplied as f32 all the same, probabilities included: the time is the rows' reading then; kFullQueries.)  f16's narrow range is met by
 // powers of two: a query row, the rows of a piece of the table (inner product), or the normalised vector (cosine) is scaled so that its
 // largest element lies in [2^12, 2^13]; what is 2^-36 of the largest is lost.
 // The gradients' products are f16 for every type: the probabilities are numbers this code rounds itself, and in bf16 their rounding would be
@@ -297,7 +297,7 @@ __global__ __launch_bounds__(256) void rows_inverse_norm_kernel(const void* w, i
 // ------------------------------------------------------------------------------------------------ joins
 // natural logarithm of 2^x y, rounded once
 __device__ __forceinline__ float log_sum(float2 a) { return (float)(((double)a.x + log2((double)a.y)) * 0.69314718055994530942); }
-__global__ __launch_bounds__(256) void loss_join_kernel(const float2* part, uint32_t part_ld, uint32_t n, const int32_t* label, const float* zlab,
+__global__ __launch_bounds__(256) void loss_join_kernel(const float2* part, uint32_t part_ld, uint32_t n, const int32_t* label, const float2* zlab,
                                                         float* loss, float* lse) {
     __shared__ float2 red[4];
     const uint32_t i = blockIdx.x, lane = threadIdx.x & 63u;
@@ -314,8 +314,10 @@ __global__ __launch_bounds__(256) void loss_join_kernel(const float2* part, uint
         return;
     }
     // a: all columns but the label's
-    const float zy = zlab[i], apart = a.x - zy;
-    lse[i] = log_sum(join_sums(a, make_float2(zy, 1.f)));
+    // (what the label's score lost when it was rounded is half a step of lse: dropped, it is the largest error of p - 1 near p = 1)
+    const float2 zy = zlab[i];
+    const float apart = a.x - zy.x - zy.y;
+    lse[i] = log_sum(join_sums(a, make_float2(zy.x, exp2f(zy.y))));
     loss[i] = apart < 64.f ? log1pf(a.y * exp2f(apart)) : (apart + log2f(a.y)) * kLn2;
 }
 
@@ -514,11 +516,11 @@ struct Plan {
 // larger pieces leave fewer CUs without a tile, and what the last-level cache (256 MiB) no longer holds costs about as much.
 constexpr size_t kPieceBytes = 640ull << 20;
 constexpr size_t kSplitBytes = 128ull << 20;    // f32 slices of dq
-// Up to this many f32 queries of f32 rows are multiplied as f32 (the loss; its gradient): the rows are then read once where the split re-lays them
-// first, about four times the traffic, and the f32 MFMA's sixteenth of the f16 rate does not show before more queries than that.  60,000 x 768, as
-// f32 / split: 40 queries 67 / 159 us and 219 / 304, 96: 114 / 161 and 331 / 327, 128: 116 / 162 and 359 / 333, 192: 165 / 185 and 502 / 391;
-// 64 by cosine 95 / 132 and 290 / 342.
-constexpr uint32_t kFullLoss = 128, kFullGrad = 64;
+// Up to this many f32 queries of f32 rows are multiplied as f32: the rows are then read once where the split re-lays them first, about four times
+// the traffic, and the f32 MFMA's sixteenth of the f16 rate does not show before more queries than that.  60,000 x 768, as f32 / split, loss and
+// gradients: 40 queries 67 + 217 / 159 + 304 us, 72: 125 + 350 / 165 + 301, 128: 120 + 352 / 164 + 306; by cosine 64: 96 + 275 / 132 + 342, 72:
+// 144 + 392 / 137 + 309.  (One limit for the loss and its gradient: a probability near 1 is only as good as the two agree on its score.)
+constexpr uint32_t kFullQueries = 64;
 
 // Rows per piece, at most `most`.  A workgroup per CU owns 256 x 256 outputs, so 257 tiles take as long as 512: of the sizes allowed, the one
 // whose products leave the fewest CUs idle (in steps of 64 k; a tile's epilogue counts 6, a piece's launches 10).
@@ -553,7 +555,7 @@ static Plan plan(const vs_rows* rows, const vs_softmax* q, bool grad_q, bool gra
     p.dp = (d + 63u) & ~63u;
     p.cosine = q->metric == VS_METRIC_COS;
     const int tq = q->scalar, tw = p.w.scalar;
-    const bool bf = tq == VS_SCALAR_BF16 && tw == VS_SCALAR_BF16, full = tq == VS_SCALAR_F32 && tw == VS_SCALAR_F32 && n <= (grad_q || grad_w ? kFullGrad : kFullLoss);
+    const bool bf = tq == VS_SCALAR_BF16 && tw == VS_SCALAR_BF16, full = tq == VS_SCALAR_F32 && tw == VS_SCALAR_F32 && n <= kFullQueries;
     p.kind = full ? K_F32 : bf ? K_BF16 : K_F16;
     p.gkind = full ? K_F32 : K_F16;
     p.es = full ? 4 : 2, p.bk = 128 / p.es;
@@ -609,7 +611,7 @@ static Plan plan(const vs_rows* rows, const vs_softmax* q, bool grad_q, bool gra
     p.o_gwplanes = l.take(p.regrow ? piece * p.dp * 2 : 0);
     if (!grad) {
         p.o_part = l.take((size_t)n * p.tiles_v * 8);
-        p.o_zlab = l.take((size_t)n * 4);
+        p.o_zlab = l.take((size_t)n * 8);
     } else {
         p.o_df = l.take((size_t)n * 4);
         p.o_qinv = l.take((size_t)n * 4);
@@ -770,12 +772,12 @@ static void loss(const vs_rows* rows, const vs_softmax* q, float* d_loss, float*
         g.part = c.at<float2>(p.o_part);
         g.part_ld = p.tiles_v;
         g.part0 = tile;
-        g.zlab = c.at<float>(p.o_zlab);
+        g.zlab = c.at<float2>(p.o_zlab);
         product<SCORES, EPI_LOSS>(g, p.shape_s, p.kind, st);
         tile += (count + kTileN[p.shape_s] - 1) / kTileN[p.shape_s];
     }
     hipLaunchKernelGGL(loss_join_kernel, dim3(p.n), dim3(256), 0, st, c.at<float2>(p.o_part), p.tiles_v, p.n, c.at<int32_t>(p.o_label),
-                       c.at<float>(p.o_zlab), d_loss, d_lse);
+                       c.at<float2>(p.o_zlab), d_loss, d_lse);
     launched("join");
 }
 

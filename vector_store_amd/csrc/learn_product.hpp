@@ -53,7 +53,7 @@ struct ProductArgs {
     // EPI_LOSS
     float2* part;                // [m][part_ld] (maximum, sum of 2^(z2 - maximum)) per column tile
     uint32_t part_ld, part0;
-    float* zlab;                 // z2 at the label
+    float2* zlab;                // z2 at the label, and what its rounding lost
     // EPI_PROB: P = f16((2^(z2 - lse2 - lo) - [label]) * pf), and 2^11 times what that loses; lo: what lse2 lost when it was rounded.  f32 operands:
     // P = (2^(z2 - lse2 - lo) - [label]) * pf * h[col] as f32
     const float* lo;
@@ -578,7 +578,7 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                                 const float z = acc[i][j][r] * f;
                                 bool in = plain || ((live[j] >> r) & 1u);
                                 if (lab == j * 16u + r) {
-                                    if (row0 + i * 16u < g.m) g.zlab[row0 + i * 16u] = z;
+                                    if (row0 + i * 16u < g.m) g.zlab[row0 + i * 16u] = make_float2(z, fabsf(z) < __builtin_inff() ? fmaf(acc[i][j][r], f, -z) : 0.f);
                                     in = false;
                                 }
                                 top = in ? fmaxf(top, z) : top;
