@@ -482,8 +482,10 @@ inline LookupGradLayout lookup_grad_layout(size_t n, size_t rows, size_t dim) {
     l.small = n <= kSmallSort;
     l.items = (uint32_t)std::max<size_t>(256, ((n + 4095) / 4096 + 63) / 64 * 64);
     l.waves = (uint32_t)((n + l.items - 1) / l.items);
-    // short runs keep few ids spread over the chip; long ones leave fewer sums to be joined (131k ids in runs of 16 / 64: 97 + 36 us / 98 + 12 us)
-    l.run = n <= 8192 ? kBatch : 4 * kBatch;
+    // short runs keep few ids and short rows spread over the chip (a run is summed one entry after the other); long ones, once they fill it by
+    // themselves (65,536 threads), leave fewer sums to be joined.  In runs of 16 / 64, us: 14,569 ids x 128 53 / 75, 60,000 x 256 71 / 80,
+    // 131,072 x 128 109 / 112; 30,011 x 1536 99 / 88, 131,072 x 768 246 / 229
+    l.run = n * ((dim + 7) / 8) < ((size_t)4 << 20) ? kBatch : 4 * kBatch;
     l.runs = (uint32_t)((n + l.run - 1) / l.run);
     l.bits = 1;
     while (l.bits < 31 && (rows >> l.bits)) ++l.bits;  // keys 0 .. rows
