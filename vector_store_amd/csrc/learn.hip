@@ -55,6 +55,7 @@ struct QueryPrep {
     int kind;                      // K_*
     bool wide;                     // 16-byte aligned rows
     void* planes;                  // nullptr: read in place
+    void* gplanes;                 // f32: the queries as an operand of dw, or nullptr
     uint32_t nplanes;
     uint64_t plane;
     uint32_t* tops;                // the pieces' largest elements, zeroed for rows_top_kernel
@@ -125,10 +126,24 @@ __global__ __launch_bounds__(256) void query_prep_kernel(QueryPrep a) {
     const uint32_t lane = threadIdx.x & 63u, i = blockIdx.x * 4u + (threadIdx.x >> 6);
     if (i >= a.n) return;
     float ss = 0.f, top = 0.f;
-    if (a.cosine || !a.raw || a.g) row_extent(a.q, a.scalar, (uint64_t)i * a.ld, a.d, a.wide, lane, 64, ss, top);
+    if (a.cosine || !a.raw || (a.g && a.kind != K_F32)) row_extent(a.q, a.scalar, (uint64_t)i * a.ld, a.d, a.wide, lane, 64, ss, top);
     const float inv = !a.cosine ? 1.f : ss > 0.f ? 1.f / sqrtf(ss) : 0.f;
     const int32_t e = a.raw || a.cosine ? 0 : exponent_of(top);
     const bool unit = a.cosine && a.kind == K_F32;  // (the planes hold the direction)
+    int64_t y = a.label_bytes == 8 ? reinterpret_cast<const int64_t*>(a.labels)[i] : reinterpret_cast<const int32_t*>(a.labels)[i];
+    if (y < 0 || y >= (int64_t)a.rows || (a.keys && a.keys[y] == ~0ull)) y = -1;
+    const float g = a.g && y >= 0 ? a.g[i] : 0.f;
+    if (a.gplanes) {  // as grad_queries_kernel, with the factors themselves
+        const bool on = y >= 0 && g != 0.f;
+        const float f = g * a.scale;
+        for (uint32_t k = lane * 8u; k < a.dp; k += 512) {
+            float x[8];
+            load8(a.q, a.scalar, (uint64_t)i * a.ld + k, on && k < a.d ? a.d - k : 0u, a.wide, x);
+#pragma unroll
+            for (int r = 0; r < 8; ++r) x[r] = on ? x[r] * inv * f : 0.f;
+            put_planes(a.gplanes, (uint64_t)i * a.dp + k, 0, 1, a.kind, x);
+        }
+    }
     if (a.planes) {
         for (uint32_t k = lane * 8u; k < a.dp; k += 512) {
             float x[8];
@@ -141,8 +156,6 @@ __global__ __launch_bounds__(256) void query_prep_kernel(QueryPrep a) {
         }
     }
     if (lane) return;
-    int64_t y = a.label_bytes == 8 ? reinterpret_cast<const int64_t*>(a.labels)[i] : reinterpret_cast<const int32_t*>(a.labels)[i];
-    if (y < 0 || y >= (int64_t)a.rows || (a.keys && a.keys[y] == ~0ull)) y = -1;
     a.label[i] = (int32_t)y;
     const float s2 = a.scale * kLog2e;
     float4 row = make_float4(unit ? s2 : a.raw ? s2 * inv : a.cosine ? s2 * 0x1p-26f : ldexpf(s2, e - 13), 0.f, 0.f, __int_as_float((int32_t)y));
@@ -153,7 +166,6 @@ __global__ __launch_bounds__(256) void query_prep_kernel(QueryPrep a) {
         const float lo = fabsf(row.y) < __builtin_inff() ? fmaf(lse, kLog2e, -row.y) + lse * kLog2eLo : 0.f;
         a.lo[i] = lo;
         a.inv[i] = inv;
-        const float g = y >= 0 ? a.g[i] : 0.f;
         // f16 probabilities: (p - [label]) * m * 2^15 with g = m * 2^x, 1/2 <= |m| < 1: below 2^15, off by at most 2^-11 of themselves or 2^-39
         // (f32: the probability itself times the row's inverse length; the query's factors go to dq and, in front of dw, to the query)
         int x = 0;
@@ -166,17 +178,16 @@ __global__ __launch_bounds__(256) void query_prep_kernel(QueryPrep a) {
     a.row[i] = row;
 }
 
-// The queries as an operand of dw = P^T q: rows of padding are zero whatever they held.  f16: every other row carries the power of two of its
-// loss gradient, relative to the largest; *wf undoes it.  f32: its loss gradient itself, the scale and (cosine) its inverse length.
+// The queries as an operand of dw = P^T q, in f16: rows of padding are zero whatever they held, every other row carries the power of two of its
+// loss gradient, relative to the largest; *wf undoes it.
 struct GradQueries {
     const void* q;
     int scalar;
     uint64_t ld;
     uint32_t n, d, dp, cosine, nplanes;
-    int kind;  // K_F16 or K_F32
     bool wide;
     const int32_t *label, *ge, *xe;
-    const float *inv, *g;
+    const float* inv;
     float scale;
     void* planes;
     uint64_t plane;
@@ -201,20 +212,19 @@ __global__ __launch_bounds__(1024) void grad_exponent_kernel(GradQueries a) {
     if (threadIdx.x == 0) a.top[0] = top;
 }
 __global__ __launch_bounds__(256) void grad_queries_kernel(GradQueries a) {
-    const int32_t top = a.kind == K_F32 ? 0 : a.n <= kOwnExponent ? grad_exponent(a) : a.top[0];
+    const int32_t top = a.n <= kOwnExponent ? grad_exponent(a) : a.top[0];
     if (blockIdx.x == 0 && threadIdx.x == 0) a.wf[0] = ldexpf(a.scale, top - 28);
     const uint32_t lane = threadIdx.x & 63u, i = blockIdx.x * 4u + (threadIdx.x >> 6);
     if (i >= a.n) return;
     const bool on = a.label[i] >= 0 && a.xe[i] != kNoExponent;  // (padding, and queries whose loss nobody asks about)
-    const bool full = a.kind == K_F32;
-    const int32_t up = full ? 0 : a.ge[i] - top + 13;
-    const float inv = a.cosine ? a.inv[i] : 1.f, f = full && on ? a.g[i] * a.scale : 1.f;
+    const int32_t up = a.ge[i] - top + 13;
+    const float inv = a.cosine ? a.inv[i] : 1.f;
     for (uint32_t k = lane * 8u; k < a.dp; k += 512) {
         float x[8];
         load8(a.q, a.scalar, (uint64_t)i * a.ld + k, on && k < a.d ? a.d - k : 0u, a.wide, x);
 #pragma unroll
-        for (int r = 0; r < 8; ++r) x[r] = full ? x[r] * inv * f : ldexpf(x[r] * inv, up);
-        put_planes(a.planes, (uint64_t)i * a.dp + k, a.plane, a.nplanes, a.kind, x);
+        for (int r = 0; r < 8; ++r) x[r] = ldexpf(x[r] * inv, up);
+        put_planes(a.planes, (uint64_t)i * a.dp + k, a.plane, a.nplanes, K_F16, x);
     }
 }
 
@@ -585,7 +595,8 @@ static Plan plan(const vs_rows* rows, const vs_softmax* q, bool grad_q, bool gra
     }
     p.piece = (uint32_t)piece;
     p.shape_s = full ? SMALL : choose_shape(n, piece, false);
-    p.shape_w = full ? SMALL : choose_shape(piece, d, false);
+    // (dw of one step of k is its writing: 64 x 60,000 x 768 in bf16 169 us by large tiles, 161 by small ones)
+    p.shape_w = full || n <= 64 ? SMALL : choose_shape(piece, d, false);
     p.shape_q = full ? SMALL : choose_shape(n, d, true);
     const size_t qtiles = (size_t)((n + kTileM[p.shape_q] - 1) / kTileM[p.shape_q]) * ((d + kTileN[p.shape_q] - 1) / kTileN[p.shape_q]);
     const size_t dn = (d + 3u) & ~3u;
@@ -673,6 +684,7 @@ struct Call {  // what the two calls share
             a.lse = lse;
             a.df = at<float>(p.o_df), a.inv = at<float>(p.o_qinv), a.lo = at<float>(p.o_lo);
             a.ge = at<int32_t>(p.o_ge), a.xe = at<int32_t>(p.o_xe);
+            a.gplanes = p.grad_w && p.gkind == K_F32 ? at<char>(p.o_gplanes) : nullptr;
         }
         hipLaunchKernelGGL(query_prep_kernel, dim3((p.n + 3) / 4), dim3(256), 0, st, a);
         launched("queries");
@@ -799,25 +811,25 @@ static void loss_grad(const vs_rows* rows, const vs_softmax* q, const float* d_l
     const Call c{p, *q, (char*)work, st};
     c.queries(d_lse, d_g);
     c.tables();
-    Operand gq = {};
-    if (d_gw) {
+    const uint64_t gplane = (uint64_t)p.n * p.dp;
+    const Operand gq = {c.at<char>(p.o_gplanes), gplane * p.ges, (uint64_t)p.dp * p.ges, p.n, p.dp};
+    if (d_gw && p.gkind != K_F32) {
         GradQueries a = {};
         a.q = q->d_queries;
         a.scalar = q->scalar;
         a.ld = q->stride;
-        a.n = p.n, a.d = p.d, a.dp = p.dp, a.cosine = p.cosine, a.nplanes = p.nqg, a.kind = p.gkind;
+        a.n = p.n, a.d = p.d, a.dp = p.dp, a.cosine = p.cosine, a.nplanes = p.nqg;
         a.wide = wide_rows(a.q, a.scalar, a.ld);
         a.label = c.at<int32_t>(p.o_label), a.ge = c.at<int32_t>(p.o_ge), a.xe = c.at<int32_t>(p.o_xe);
-        a.inv = c.at<float>(p.o_qinv), a.g = d_g;
+        a.inv = c.at<float>(p.o_qinv);
         a.scale = q->scale;
         a.planes = c.at<char>(p.o_gplanes);
-        a.plane = (uint64_t)p.n * p.dp;
+        a.plane = gplane;
         a.top = c.at<int32_t>(p.o_exp);
         a.wf = c.at<float>(p.o_exp) + 1;
-        if (p.gkind != K_F32 && p.n > kOwnExponent) hipLaunchKernelGGL(grad_exponent_kernel, dim3(1), dim3(1024), 0, st, a);
+        if (p.n > kOwnExponent) hipLaunchKernelGGL(grad_exponent_kernel, dim3(1), dim3(1024), 0, st, a);
         hipLaunchKernelGGL(grad_queries_kernel, dim3((p.n + 3) / 4), dim3(256), 0, st, a);
         launched("queries");
-        gq = Operand{(const char*)a.planes, a.plane * p.ges, (uint64_t)p.dp * p.ges, p.n, p.dp};
     }
     const uint32_t dn = (p.d + 3u) & ~3u;
     for (uint32_t x = 0; x < p.pieces; ++x) {
