@@ -152,6 +152,23 @@ def test_few_f32_queries(n, v, d, metric):
     check(q, w, y, gl, 8.0, metric)
 
 
+@pytest.mark.parametrize("metric", [learn.IP, learn.COS], ids=["ip", "cos"])
+@pytest.mark.parametrize("v,d", [(515, 1), (4099, 8), (3001, 33), (20_011, 128), (1000, 520)])
+@pytest.mark.parametrize("n", [1, 64, 65, 256, 257])
+def test_few_bf16_queries(n, v, d, metric):
+    """around the number of queries up to which the probabilities of bf16 queries and rows are two bf16"""
+    q, w, y, gl = case(n, v, d, BF16, BF16, seed=50 + n + d)
+    check(q, w, y, gl, 8.0, metric)
+
+
+def test_few_bf16_queries_of_wide_ranges():
+    q, w, y, gl = case(50, 700, 96, BF16, BF16, seed=51)
+    gl = gl * torch.logspace(-12, 12, 50, device=DEV)
+    few = (q.float() * torch.logspace(-8, 0, 50, device=DEV)[:, None]).to(BF16)
+    check(few, (w.float() * torch.logspace(-6, 0, 700, device=DEV)[:, None]).to(BF16), y, gl, 8.0, learn.IP)
+    check(few, (w.float() * torch.logspace(-9, 9, 700, device=DEV)[:, None]).to(BF16), y, gl, 8.0, learn.COS)
+
+
 def test_few_f32_queries_of_wide_ranges_and_padding():
     q, w, y, gl = case(50, 700, 96, F32, F32, seed=41)
     gl = gl * torch.logspace(-12, 12, 50, device=DEV)

@@ -39,7 +39,7 @@ static void launched(const char* what) { hip_ok(hipGetLastError(), what); }
 // The gradients' products are f16 for every type: the probabilities are numbers this code rounds itself, and in bf16 their rounding would be
 // as large as the result's (measured at 4,096 x 131,072 x 768: 0.0025 of the gradient against 0.0017 for one rounding of the exact one).  One
 // f16 (2^-11) under a bf16 result, two under f16 and f32 ones (the second times 2^11: a probability below f16's normal range keeps its bits);
-// bf16 rows and queries are exact in a scaled f16.
+// bf16 rows and queries are exact in a scaled f16.  (For a few bf16 queries, two bf16 and the rows as they are: kFewQueries.)
 
 struct QueryPrep {
     const void* q;
@@ -52,10 +52,10 @@ struct QueryPrep {
     const uint64_t* keys;          // labels of removed members too
     float scale;
     uint32_t cosine, raw;          // raw: the operands are the values themselves
-    int kind;                      // K_*
+    int kind, gkind;               // K_*: of the scores' operands, of the gradients'
     bool wide;                     // 16-byte aligned rows
     void* planes;                  // nullptr: read in place
-    void* gplanes;                 // f32: the queries as an operand of dw, or nullptr
+    void* gplanes;                 // f32, bf16: the queries as an operand of dw, or nullptr
     uint32_t nplanes;
     uint64_t plane;
     uint32_t* tops;                // the pieces' largest elements, zeroed for rows_top_kernel
@@ -126,22 +126,22 @@ __global__ __launch_bounds__(256) void query_prep_kernel(QueryPrep a) {
     const uint32_t lane = threadIdx.x & 63u, i = blockIdx.x * 4u + (threadIdx.x >> 6);
     if (i >= a.n) return;
     float ss = 0.f, top = 0.f;
-    if (a.cosine || !a.raw || (a.g && a.kind != K_F32)) row_extent(a.q, a.scalar, (uint64_t)i * a.ld, a.d, a.wide, lane, 64, ss, top);
+    if (a.cosine || !a.raw || (a.g && a.gkind == K_F16)) row_extent(a.q, a.scalar, (uint64_t)i * a.ld, a.d, a.wide, lane, 64, ss, top);
     const float inv = !a.cosine ? 1.f : ss > 0.f ? 1.f / sqrtf(ss) : 0.f;
     const int32_t e = a.raw || a.cosine ? 0 : exponent_of(top);
     const bool unit = a.cosine && a.kind == K_F32;  // (the planes hold the direction)
     int64_t y = a.label_bytes == 8 ? reinterpret_cast<const int64_t*>(a.labels)[i] : reinterpret_cast<const int32_t*>(a.labels)[i];
     if (y < 0 || y >= (int64_t)a.rows || (a.keys && a.keys[y] == ~0ull)) y = -1;
     const float g = a.g && y >= 0 ? a.g[i] : 0.f;
-    if (a.gplanes) {  // as grad_queries_kernel, with the factors themselves
-        const bool on = y >= 0 && g != 0.f;
+    if (a.gplanes) {  // as grad_queries_kernel; f32: with the factors themselves, bf16: the probabilities carry them
+        const bool on = y >= 0 && g != 0.f, full = a.gkind == K_F32;
         const float f = g * a.scale;
         for (uint32_t k = lane * 8u; k < a.dp; k += 512) {
             float x[8];
             load8(a.q, a.scalar, (uint64_t)i * a.ld + k, on && k < a.d ? a.d - k : 0u, a.wide, x);
 #pragma unroll
-            for (int r = 0; r < 8; ++r) x[r] = on ? x[r] * inv * f : 0.f;
-            put_planes(a.gplanes, (uint64_t)i * a.dp + k, 0, 1, a.kind, x);
+            for (int r = 0; r < 8; ++r) x[r] = !on ? 0.f : full ? x[r] * inv * f : x[r];
+            put_planes(a.gplanes, (uint64_t)i * a.dp + k, 0, 1, a.gkind, x);
         }
     }
     if (a.planes) {
@@ -167,11 +167,12 @@ __global__ __launch_bounds__(256) void query_prep_kernel(QueryPrep a) {
         a.lo[i] = lo;
         a.inv[i] = inv;
         // f16 probabilities: (p - [label]) * m * 2^15 with g = m * 2^x, 1/2 <= |m| < 1: below 2^15, off by at most 2^-11 of themselves or 2^-39
-        // (f32: the probability itself times the row's inverse length; the query's factors go to dq and, in front of dw, to the query)
+        // f32: the probability itself times the row's inverse length; the query's factors go to dq and, in front of dw, to the query.  bf16, whose
+        // queries and rows are used as they are: times all of them.
         int x = 0;
         const float m = frexpf(g, &x);
-        row.z = (a.kind == K_F32 ? 1.f : m * 32768.f) * exp2f(-lo);
-        a.df[i] = y < 0 ? 0.f : a.kind == K_F32 ? g * a.scale * inv : ldexpf(a.scale * (a.cosine ? inv * 0x1p-13f : 1.f), x - 15);
+        row.z = (a.gkind == K_F32 ? 1.f : a.gkind == K_BF16 ? g * a.scale * inv : m * 32768.f) * exp2f(-lo);
+        a.df[i] = y < 0 ? 0.f : a.gkind == K_F32 ? g * a.scale * inv : a.gkind == K_BF16 ? 1.f : ldexpf(a.scale * (a.cosine ? inv * 0x1p-13f : 1.f), x - 15);
         a.ge[i] = x;
         a.xe[i] = y < 0 || !(g != 0.f) ? kNoExponent : x + exponent_of(a.cosine ? top * inv : top);
     }
@@ -416,9 +417,7 @@ static void product(ProductArgs g, int shape, int kind, hipStream_t st) {
     g.tiles_m = (g.m + kTileM[shape] - 1) / kTileM[shape];
     g.tiles_n = (g.n + kTileN[shape] - 1) / kTileN[shape];
     if (kind == K_F32) return run_product<Small, FORM, EPI, K_F32>(g, st);  // (shape: SMALL)
-    if constexpr (FORM == SCORES) {  // (the gradients' products of 16-bit operands are f16)
-        if (kind == K_BF16) return product_of<FORM, EPI, K_BF16>(g, shape, st);
-    }
+    if (kind == K_BF16) return product_of<FORM, EPI, K_BF16>(g, shape, st);
     product_of<FORM, EPI, K_F16>(g, shape, st);
 }
 // The tile for m x n outputs: the one whose rounds over the chip take least.  A round of large tiles (256 workgroups) is 1, of medium ones
@@ -531,6 +530,10 @@ constexpr size_t kSplitBytes = 128ull << 20;    // f32 slices of dq
 // gradients: 40 queries 67 + 217 / 159 + 304 us, 72: 125 + 350 / 165 + 301, 128: 120 + 352 / 164 + 306; by cosine 64: 96 + 275 / 132 + 342, 72:
 // 144 + 392 / 137 + 309.  (One limit for the loss and its gradient: a probability near 1 is only as good as the two agree on its score.)
 constexpr uint32_t kFullQueries = 64;
+// Up to this many bf16 queries of bf16 rows the probabilities are kept as two bf16, times all factors, instead of one f16: the gradients' products
+// then use rows and queries as they are -- twice the products, but the rows need not be laid out in f16 first.  Gradients of 64 x
+// 60,000 x 768 161 -> 125 us, 128: 184 / 136, 256: 219 / 185, 256 x 100,000 x 1536 595 / 573, by cosine 782 / 792.
+constexpr uint32_t kFewQueries = 256;
 
 // Rows per piece, at most `most`.  A workgroup per CU owns 256 x 256 outputs, so 257 tiles take as long as 512: of the sizes allowed, the one
 // whose products leave the fewest CUs idle (in steps of 64 k; a tile's epilogue counts 6, a piece's launches 10).
@@ -567,7 +570,7 @@ static Plan plan(const vs_rows* rows, const vs_softmax* q, bool grad_q, bool gra
     const int tq = q->scalar, tw = p.w.scalar;
     const bool bf = tq == VS_SCALAR_BF16 && tw == VS_SCALAR_BF16, full = tq == VS_SCALAR_F32 && tw == VS_SCALAR_F32 && n <= kFullQueries;
     p.kind = full ? K_F32 : bf ? K_BF16 : K_F16;
-    p.gkind = full ? K_F32 : K_F16;
+    p.gkind = full ? K_F32 : bf && n <= kFewQueries ? K_BF16 : K_F16;
     p.es = full ? 4 : 2, p.bk = 128 / p.es;
     p.ges = p.es, p.gbk = p.bk;
     p.raw = full || bf || (tq == VS_SCALAR_F16 && tw == VS_SCALAR_F16 && !p.cosine);
@@ -580,9 +583,9 @@ static Plan plan(const vs_rows* rows, const vs_softmax* q, bool grad_q, bool gra
     p.grad_q = grad_q;
     p.grad_w = grad_w;
     const bool grad = grad_q || grad_w;
-    p.np = !full && ((grad_q && tq != VS_SCALAR_BF16) || (grad_w && tw != VS_SCALAR_BF16)) ? 2 : 1;
+    p.np = p.gkind == K_BF16 || (!full && ((grad_q && tq != VS_SCALAR_BF16) || (grad_w && tw != VS_SCALAR_BF16))) ? 2 : 1;
     p.nqg = !full && tw != VS_SCALAR_BF16 && (p.cosine || tq == VS_SCALAR_F32) ? 2 : 1;
-    p.regrow = bf && grad_q;
+    p.regrow = bf && grad_q && p.gkind == K_F16;
     p.nwg = p.regrow ? 1 : p.nw;
     // pieces of the table: one, unless rows are re-laid or probabilities are kept for the two products that read them
     const size_t per_row = (p.w_in_place ? 0 : (size_t)p.nw * p.dp * p.es) + (p.regrow ? (size_t)p.dp * 2 : 0) + (grad ? (size_t)p.np * n * p.ges : 0);
@@ -670,7 +673,7 @@ struct Call {  // what the two calls share
         a.rows = p.v;
         a.keys = p.w.keys;
         a.scale = q.scale;
-        a.cosine = p.cosine, a.raw = p.raw, a.kind = p.kind;
+        a.cosine = p.cosine, a.raw = p.raw, a.kind = p.kind, a.gkind = p.gkind;
         a.wide = wide_rows(a.q, a.scalar, a.ld);
         a.planes = p.q_in_place ? nullptr : at<char>(p.o_qplanes);
         a.nplanes = p.nq;
@@ -684,7 +687,7 @@ struct Call {  // what the two calls share
             a.lse = lse;
             a.df = at<float>(p.o_df), a.inv = at<float>(p.o_qinv), a.lo = at<float>(p.o_lo);
             a.ge = at<int32_t>(p.o_ge), a.xe = at<int32_t>(p.o_xe);
-            a.gplanes = p.grad_w && p.gkind == K_F32 ? at<char>(p.o_gplanes) : nullptr;
+            a.gplanes = p.grad_w && p.gkind != K_F16 ? at<char>(p.o_gplanes) : nullptr;
         }
         hipLaunchKernelGGL(query_prep_kernel, dim3((p.n + 3) / 4), dim3(256), 0, st, a);
         launched("queries");
@@ -813,7 +816,7 @@ static void loss_grad(const vs_rows* rows, const vs_softmax* q, const float* d_l
     c.tables();
     const uint64_t gplane = (uint64_t)p.n * p.dp;
     const Operand gq = {c.at<char>(p.o_gplanes), gplane * p.ges, (uint64_t)p.dp * p.ges, p.n, p.dp};
-    if (d_gw && p.gkind != K_F32) {
+    if (d_gw && p.gkind == K_F16) {
         GradQueries a = {};
         a.q = q->d_queries;
         a.scalar = q->scalar;
@@ -841,6 +844,7 @@ static void loss_grad(const vs_rows* rows, const vs_softmax* q, const float* d_l
         g.prob_ld = (count + 7u) & ~7u;
         g.prob_plane = (uint64_t)p.n * g.prob_ld;
         g.prob_planes = p.np;
+        g.prob_kind = p.gkind;
         g.tpart = d_gw && p.cosine ? c.at<float>(p.o_tpart) : nullptr;
         g.graw = d_g;
         if (g.tpart) product<SCORES, EPI_PROB_ALONG>(g, p.shape_s, p.kind, st);
@@ -853,8 +857,9 @@ static void loss_grad(const vs_rows* rows, const vs_softmax* q, const float* d_l
             b.m = p.n, b.n = dn, b.k = count;
             b.splits = p.splits;
             b.ksteps = p.qsteps;
-            plane_pairs(b, p.np, p.nwg, q->scalar != VS_SCALAR_BF16);
-            b.lo_first = q->scalar != VS_SCALAR_BF16 && p.np > 1;
+            const bool both = q->scalar != VS_SCALAR_BF16 || p.gkind == K_BF16;
+            plane_pairs(b, p.np, p.nwg, both);
+            b.lo_first = both && p.np > 1;
             b.out_part = c.at<float>(p.o_qpart);
             product<DQ, EPI_PART>(b, p.shape_q, p.gkind, st);
             QueryJoin j = {};
@@ -882,13 +887,14 @@ static void loss_grad(const vs_rows* rows, const vs_softmax* q, const float* d_l
             b.m = count, b.n = p.d, b.k = p.n;
             b.splits = 1;
             b.ksteps = (p.n + p.gbk - 1) / p.gbk;
-            plane_pairs(b, p.np, p.nqg, p.w.scalar != VS_SCALAR_BF16);
-            b.lo_first = p.w.scalar != VS_SCALAR_BF16 && p.np > 1;
+            const bool both = p.w.scalar != VS_SCALAR_BF16 || p.gkind == K_BF16;
+            plane_pairs(b, p.np, p.nqg, both);
+            b.lo_first = both && p.np > 1;
             b.out = (char*)d_gw + (size_t)first * gw_ld * size_of(p.w.scalar);
             b.out_scalar = p.w.scalar;
             b.out_ld = gw_ld;
-            b.wf = p.gkind == K_F32 ? nullptr : c.at<float>(p.o_exp) + 1;
-            b.rf = p.cosine && p.gkind != K_F32 ? c.inv() + first : nullptr;
+            b.wf = p.gkind != K_F16 ? nullptr : c.at<float>(p.o_exp) + 1;
+            b.rf = p.cosine && p.gkind == K_F16 ? c.inv() + first : nullptr;
             b.tcoef = p.cosine ? c.at<float>(p.o_coef) : nullptr;
             b.tinv = p.cosine ? c.inv() + first : nullptr;
             b.raw = p.w.data + (size_t)first * p.w.ld * size_of(p.w.scalar);

@@ -55,7 +55,8 @@ struct ProductArgs {
     uint32_t part_ld, part0;
     float2* zlab;                // z2 at the label, and what its rounding lost
     // EPI_PROB: P = f16((2^(z2 - lse2 - lo) - [label]) * pf), and 2^11 times what that loses; lo: what lse2 lost when it was rounded.  f32 operands:
-    // P = (2^(z2 - lse2 - lo) - [label]) * pf * h[col] as f32
+    // P = (2^(z2 - lse2 - lo) - [label]) * pf * h[col] as f32; prob_kind K_BF16: the same as two bf16
+    int prob_kind;
     const float* lo;
     uint16_t* prob;
     uint64_t prob_plane;         // elements
@@ -706,6 +707,16 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                         continue;
                     }
                     ushort4 hi[S::NT], lo[S::NT];
+                    if (KIND == K_BF16 && g.prob_kind == K_BF16) {
+#pragma unroll
+                        for (int j = 0; j < S::NT; ++j)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const float x = g.h ? v[j][r] * rf.z * h[j][r] : v[j][r] * rf.z;
+                                const uint16_t b = to_half<true>(x);
+                                (&hi[j].x)[r] = b, (&lo[j].x)[r] = to_half<true>(x - from_half<true>(b));
+                            }
+                    } else
 #pragma unroll
                     for (int j = 0; j < S::NT; ++j) {
 #pragma unroll
