@@ -598,8 +598,7 @@ static Plan plan(const vs_rows* rows, const vs_softmax* q, bool grad_q, bool gra
     }
     p.piece = (uint32_t)piece;
     p.shape_s = full ? SMALL : choose_shape(n, piece, false);
-    // (dw of one step of k is its writing: 64 x 60,000 x 768 in bf16 169 us by large tiles, 161 by small ones)
-    p.shape_w = full || n <= 64 ? SMALL : choose_shape(piece, d, false);
+    p.shape_w = full ? SMALL : choose_shape(piece, d, false);
     p.shape_q = full ? SMALL : choose_shape(n, d, true);
     const size_t qtiles = (size_t)((n + kTileM[p.shape_q] - 1) / kTileM[p.shape_q]) * ((d + kTileN[p.shape_q] - 1) / kTileN[p.shape_q]);
     const size_t dn = (d + 3u) & ~3u;
