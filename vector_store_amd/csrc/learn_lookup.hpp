@@ -1,11 +1,14 @@
 // learn_lookup.hpp -- rows read by number, and the gradient that goes back to them.
 //
-// Forward: out[t] = scale * row[id[t]].  Bound by the memory: one 16-byte piece of a row per thread and load.
+// Forward: out[t] = scale * row[id[t]].  Bound by the memory: one 16-byte piece of a row per thread and load (40,001 bf16 rows of 768 out of
+// a million: 21 us, 5.7 TB/s read and written; 16 rows: 14 us a call, the launch).
 //
 // Backward: sums over the t that read a row, in the order of t, without float atomics (two calls give the same bits).  The (id, t) pairs are
 // sorted by id -- stable, so t ascends within an id --, the sorted list is cut into runs of 16 or 64 entries, a workgroup sums each run: an id
 // whose entries all lie in one run is written at once, the others leave a partial row at the run's head (the id began earlier) or tail
 // (it goes on), and a second kernel adds those up from the run where the id begins.  An id read n times costs n / 64 serial steps, not n.
+// Bound by the memory too: 131,072 bf16 gradients of 768 into 262,144 rows, a tenth of the reads going to 26 of them: zeros 53 us (7.6 TB/s), sort
+// 62, sums 101 (2 TB/s: rows in the order of the ids), join 12.
 #pragma once
 #include <hip/hip_runtime.h>
 
