@@ -16,7 +16,8 @@
  *  - Matrices are row-major with a row stride in ELEMENTS (>= the row's length); any stride and alignment of whole elements will do
  *    (16-byte aligned rows of a multiple of 8 elements are read in place, others are re-laid in d_work first).
  *  - Scalars: VS_SCALAR_F32, VS_SCALAR_F16, VS_SCALAR_BF16.  Sums are kept in f32.  Two calls with the same inputs give the same bits.
- *  - Rows, and queries with a label, hold finite numbers (an infinity or NaN among them reaches every loss and gradient).  Under
+ *  - Rows, and queries with a label, hold finite numbers (an infinity or NaN among them reaches every loss and gradient), their inner
+ *    products are finite in f32 before the scale is applied, and so are the gradients.  Under
  *    VS_METRIC_COS a vector's length lies between 1e-18 and 1e18 (its square is an f32; zero vectors are fine: their scores and gradients
  *    are 0), of bf16 vectors also a query's length times a row's between 1e-36 and 1e36.
  *  - Ids and labels: int32 (id_bytes 4) or int64 (8).

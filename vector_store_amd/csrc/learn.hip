@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <string>
 
@@ -393,9 +394,14 @@ __global__ __launch_bounds__(256) void row_along_kernel(const float* tpart, uint
 // ------------------------------------------------------------------------------------------------ host side
 template <class S, int FORM, int EPI, int KIND>
 static void run_product(const ProductArgs& g, hipStream_t st) {
-    static const hipError_t allowed =
-        hipFuncSetAttribute(reinterpret_cast<const void*>(&product_kernel<S, FORM, EPI, KIND>), hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS);
-    hip_ok(allowed, "shared memory of the product");
+    static std::atomic<uint64_t> allowed{0};  // a bit per device
+    int device = 0;
+    hip_ok(hipGetDevice(&device), "device");
+    if (device >= 64 || !(allowed.load(std::memory_order_relaxed) >> device & 1u)) {
+        hip_ok(hipFuncSetAttribute(reinterpret_cast<const void*>(&product_kernel<S, FORM, EPI, KIND>), hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS),
+               "shared memory of the product");
+        if (device < 64) allowed.fetch_or(1ull << device, std::memory_order_relaxed);
+    }
     const uint64_t tiles = (uint64_t)g.tiles_m * g.tiles_n * g.splits;
     if (tiles >= (1ull << 31)) fail(VS_ERR_UNSUPPORTED, "too many tiles");
     constexpr uint32_t resident = 256u * (160u * 1024u / S::LDS);

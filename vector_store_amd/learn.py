@@ -150,6 +150,7 @@ def lookup_grad(grad, ids, size: int, scale: float = 1.0, dtype=None, into=None)
                   "into: a (size, dim) tensor beside grad is needed")
             _need((dim <= 1 or into.stride(1) == 1) and (size <= 1 or into.stride(0) >= dim), "into: contiguous rows that do not overlap are needed")
             _need(dtype is None or dtype == into.dtype, "dtype: into has another")
+            _need(into.numel() == 0 or into.data_ptr() != g.data_ptr(), "into: memory apart from grad's is needed")
             out = into
         else:
             dtype = dtype or g.dtype
