@@ -119,6 +119,7 @@ struct HostExchange {
         if (p == MAP_FAILED) throw Fail{VS_ERR_OUT_OF_MEMORY, "mmap of the exchange segment failed"};
         base = (char*)p;
         registered = hipHostRegister(base, bytes, hipHostRegisterDefault) == hipSuccess;  // pageable copies work too, only slower
+        if (!registered) (void)hipGetLastError();  // (or the next launch on this thread reports the refusal as its own)
         ctl()->attached.fetch_add(1);
         // collective, like ncclCommInitRank: every rank of the world has attached when this returns
         const auto t0 = std::chrono::steady_clock::now();
