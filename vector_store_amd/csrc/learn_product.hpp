@@ -336,7 +336,7 @@ struct Shape {
     static constexpr int MT = TM_ / WM_ / 16, NT = TN_ / WN_ / 16;
     static constexpr int A_BYTES = TM_ * 128, B_BYTES = TN_ * 128, STAGE = A_BYTES + B_BYTES;
     // row factors of RING tiles, then EPI_LOSS: (maximum, sum) per wave column and row; else SCRATCH per wave
-    static constexpr int ROW_BYTES = TM_ * 16;
+    static constexpr int ROW_BYTES = TM_ * 16 < 1024 ? 1024 : TM_ * 16;  // (a wave brings 1024 at a time)
     static constexpr int SCRATCH = RING_ * (STAGE + ROW_BYTES) + NW * 2048 <= 160 * 1024 ? 2048 : 1024;  // of a wave: 16 or 8 rows of 128 bytes
     static constexpr int EPI_BYTES = RING_ * ROW_BYTES + (WN_ * TM_ * 8 > NW * SCRATCH ? WN_ * TM_ * 8 : NW * SCRATCH);
     static constexpr int LDS = RING_ * STAGE + EPI_BYTES;
@@ -344,6 +344,7 @@ struct Shape {
 using Large = Shape<256, 256, 2, 4, 2>;   // one workgroup per CU, 152 KiB of LDS
 using Medium = Shape<128, 256, 2, 4, 3>;  // one workgroup per CU, 158 KiB
 using Small = Shape<64, 128, 2, 2, 2>;    // 58 KiB: two workgroups per CU
+using Slim = Shape<32, 128, 1, 2, 2>;     // 46 KiB: three workgroups per CU, for up to 32 f32 queries (their padding to 64 is the small tile's time)
 
 template <class S, int FORM, int EPI, int KIND>
 __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
@@ -396,7 +397,7 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
     const auto prefetch_rows = [&]() {
         // (beyond the last step the operands have no bytes: the loads bring zeros nobody reads)
         if (SOFTMAX) {
-            if (p < total && p_ks == 0 && p_seg == 0 && w < (uint32_t)S::TM / 64u) {  // (rows beyond the last: zeros)
+            if (p < total && p_ks == 0 && p_seg == 0 && w < (S::TM + 63u) / 64u) {  // (rows beyond the last: zeros)
                 const uint32_t r0 = p_tm * S::TM;
                 stage_rows(g.row + r0, (g.m - r0) * 16u, w * 1024u + lane * 16u, row_buffers + p_parity * S::ROW_BYTES + w * 1024u);
             }
