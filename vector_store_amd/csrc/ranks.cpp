@@ -78,9 +78,12 @@ int guarded(F&& f) {
 // device (RCCL refuses to pair those: "duplicate GPU"), i.e. the one-GPU boxes the tests run on.  Everything around the
 // exchange is the product path unchanged: the walk writes this rank's packed block in place, the exchange fills the other
 // ranks' blocks of the same receive buffer on the communicator stream, the packed merge follows, two slots pipeline it.
-// Per slot and generation g: wait until every rank has consumed generation g - 1 of the slot, copy the block out (D2H),
-// publish "arrived", wait for every rank's arrival, copy the other blocks in (H2D), publish "consumed".  The waits run
-// as host functions on the communicator stream and give up after kWaitSeconds (the handle then reports the failure).
+// Per slot and generation g: copy the block out (D2H), wait until every rank has consumed generation g - 1 of the slot,
+// copy the block into the segment, publish "arrived", wait for every rank's arrival, copy the other blocks out of the
+// segment, publish "consumed", copy them in (H2D).  The device's copies are between its memory and PINNED memory of the
+// rank's own: a copy out of pageable memory is read when it is enqueued, before the other ranks have arrived, and a host
+// may refuse to pin the segment itself.  The waits run as host functions on the communicator stream and give up after
+// kWaitSeconds (the handle then reports the failure).
 struct HostExchange {
     static constexpr size_t kCtlBytes = 8192, kBlockCap = 8u << 20, kMaxWorld = 64;
     static constexpr int kWaitSeconds = 60;
@@ -93,12 +96,13 @@ struct HostExchange {
     char* base = nullptr;
     size_t bytes = 0;
     int rank = 0, world = 1;
-    bool registered = false;
+    char* pinned = nullptr;  // [2][world] blocks of this rank's own
     uint64_t gen[2] = {0, 0};
     std::atomic<bool> failed{false};
 
     Ctl* ctl() const { return reinterpret_cast<Ctl*>(base); }
     char* block(int slot, int r) const { return base + kCtlBytes + ((size_t)slot * (size_t)world + (size_t)r) * kBlockCap; }
+    char* own(int slot, int r) const { return pinned + ((size_t)slot * (size_t)world + (size_t)r) * kBlockCap; }
 
     void open(const uint8_t* id, int rank_, int world_) {
         rank = rank_;
@@ -118,8 +122,14 @@ struct HostExchange {
         close(fd);
         if (p == MAP_FAILED) throw Fail{VS_ERR_OUT_OF_MEMORY, "mmap of the exchange segment failed"};
         base = (char*)p;
-        registered = hipHostRegister(base, bytes, hipHostRegisterDefault) == hipSuccess;  // pageable copies work too, only slower
-        if (!registered) (void)hipGetLastError();  // (or the next launch on this thread reports the refusal as its own)
+        if (hipHostMalloc((void**)&pinned, 2 * (size_t)world * kBlockCap, hipHostMallocDefault) != hipSuccess) {
+            pinned = nullptr;
+            (void)hipGetLastError();  // (or the next launch on this thread reports it as its own)
+            munmap(base, bytes);
+            base = nullptr;
+            if (rank == 0) shm_unlink(name.c_str());
+            throw Fail{VS_ERR_OUT_OF_MEMORY, "pinned memory of the exchange"};
+        }
         ctl()->attached.fetch_add(1);
         // collective, like ncclCommInitRank: every rank of the world has attached when this returns
         const auto t0 = std::chrono::steady_clock::now();
@@ -133,7 +143,8 @@ struct HostExchange {
     }
     void close_segment() {
         if (!base) return;
-        if (registered) (void)hipHostUnregister(base);
+        if (pinned) (void)hipHostFree(pinned);
+        pinned = nullptr;
         const bool last = ctl()->attached.fetch_sub(1) == 1;
         munmap(base, bytes);
         base = nullptr;
@@ -142,8 +153,9 @@ struct HostExchange {
 
     struct Wait {
         HostExchange* x;
-        int slot, what;  // 0: every rank consumed generation g - 1; 1: publish arrival, wait for everyone's; 2: publish consumption
+        int slot;
         uint64_t g;
+        size_t bytes;  // of a block
     };
     static void host_step(void* p) {
         Wait* w = (Wait*)p;
@@ -162,23 +174,27 @@ struct HostExchange {
                 std::this_thread::sleep_for(std::chrono::microseconds(20));
             }
         };
-        if (w->what == 0) all_at_least(c->consumed[w->slot], w->g);
-        else if (w->what == 1) {
+        all_at_least(c->consumed[w->slot], w->g);
+        if (!x.failed) {
+            memcpy(x.block(w->slot, x.rank), x.own(w->slot, x.rank), w->bytes);
             c->arrived[w->slot][x.rank].store(w->g + 1, std::memory_order_release);
             all_at_least(c->arrived[w->slot], w->g + 1);
-        } else c->consumed[w->slot][x.rank].store(w->g + 1, std::memory_order_release);
+        }
+        if (!x.failed) {
+            for (int r = 0; r < x.world; ++r)
+                if (r != x.rank) memcpy(x.own(w->slot, r), x.block(w->slot, r), w->bytes);
+            c->consumed[w->slot][x.rank].store(w->g + 1, std::memory_order_release);
+        }
         delete w;
     }
     void all_gather(int slot, char* gathered, size_t block_bytes, hipStream_t st) {
         if (failed.load()) throw Fail{VS_ERR_DEVICE, "host exchange: a rank did not arrive within " + std::to_string(kWaitSeconds) + " s"};
         if (block_bytes > kBlockCap) throw Fail{VS_ERR_UNSUPPORTED, "host exchange: batch above 8 MiB per rank"};
         const uint64_t g = gen[slot]++;
-        HIP_OK(hipLaunchHostFunc(st, host_step, new Wait{this, slot, 0, g}));
-        HIP_OK(hipMemcpyAsync(block(slot, rank), gathered + (size_t)rank * block_bytes, block_bytes, hipMemcpyDeviceToHost, st));
-        HIP_OK(hipLaunchHostFunc(st, host_step, new Wait{this, slot, 1, g}));
+        HIP_OK(hipMemcpyAsync(own(slot, rank), gathered + (size_t)rank * block_bytes, block_bytes, hipMemcpyDeviceToHost, st));
+        HIP_OK(hipLaunchHostFunc(st, host_step, new Wait{this, slot, g, block_bytes}));
         for (int r = 0; r < world; ++r)
-            if (r != rank) HIP_OK(hipMemcpyAsync(gathered + (size_t)r * block_bytes, block(slot, r), block_bytes, hipMemcpyHostToDevice, st));
-        HIP_OK(hipLaunchHostFunc(st, host_step, new Wait{this, slot, 2, g}));
+            if (r != rank) HIP_OK(hipMemcpyAsync(gathered + (size_t)r * block_bytes, own(slot, r), block_bytes, hipMemcpyHostToDevice, st));
     }
 };
 
