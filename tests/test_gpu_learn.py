@@ -191,6 +191,15 @@ def test_few_f32_queries_of_wide_ranges_and_padding():
             assert torch.equal(l1, l0) and torch.equal(s1[~off], s0[~off]) and torch.equal(a1, a0) and torch.equal(b1, b0), metric
 
 
+@pytest.mark.parametrize("t", [F32, BF16], ids=["f32", "bf16"])
+def test_few_queries_over_several_pieces(t):
+    """more rows than one piece holds (2^20), re-laid and in place"""
+    for d, metric in ((5, learn.IP), (8, learn.COS)):
+        q, w, y, gl = case(3, 1_100_003, d, t, t, seed=44, pad=False)
+        y[1] = 1_100_002
+        check(q, w, y, gl, 8.0, metric)
+
+
 @pytest.mark.parametrize("metric", [vs.IP, vs.COS], ids=["ip", "cos"])
 def test_few_f32_queries_of_an_index(metric):
     ix, keys, base = build(F32, metric, 1500, 100, 1)
@@ -460,6 +469,13 @@ def test_lookup_shapes_and_untouched_neighbours():
     assert (learn.lookup_grad(ones, many, 3)[0] == 100_000).all()
 
 
+def test_a_gradient_is_not_added_onto_itself():
+    x = torch.ones(7, 4, device=DEV)
+    with pytest.raises(vs.VsError):
+        learn.lookup_grad(x, torch.arange(7, device=DEV), 7, into=x)
+    assert (x == 1).all()
+
+
 # ---------------------------------------------------------------------------------------------------- members of an index
 def build(t, metric, n, d, seed):
     g = np.random.default_rng(seed)
@@ -495,6 +511,27 @@ def test_members_of_an_index(t, metric):
     assert (dw[dead] == 0).all()
     read = learn.lookup(ix, torch.arange(1500, device=DEV))
     assert (read[dead] == 0).all() and torch.equal(read[~dead], stored[~dead])
+
+
+def test_members_added_and_updated_one_by_one():
+    """single adds and updates are staged: a call sees them all"""
+    ix, keys, base = build(F32, vs.IP, 300, 24, 4)
+    extra = np.random.default_rng(5).standard_normal((6, 24)).astype(np.float32)
+    for j in range(5):
+        ix.add(10_000 + j, extra[j])
+    assert ix.remove(int(keys[7]))
+    ix.add(int(keys[7]), extra[5])
+    slots = torch.from_numpy(ix.slots([10_000, 10_001, 10_002, 10_003, 10_004, int(keys[7]), int(keys[8])])).to(DEV)
+    want = torch.from_numpy(np.concatenate([extra, base[8:9]])).to(DEV)
+    assert torch.equal(learn.lookup(ix, slots), want)
+    loss, lse = learn.softmax_loss(want, ix, slots)
+    members = torch.from_numpy(np.concatenate([np.delete(base, 7, 0), extra])).to(DEV).double()
+    z = want.double() @ members.t()
+    # a score is off by |q| |w| (3 * 2^-22 + 3 (D + 64) * 2^-24), the sum and lse's rounding by 2^-24 (80 + 8 |z|), as in `reference`
+    e = float(want.norm(dim=1).max() * members.norm(dim=1).max()) * (3 * 2.0 ** -22 + 3 * (24 + 64) * 2.0 ** -24) + 2.0 ** -24 * (80 + 8 * float(z.abs().max()))
+    want_lse = torch.logsumexp(z, dim=1)
+    assert (lse.double() - want_lse).abs().max() <= e
+    assert (loss.double() - (want_lse - (want.double() ** 2).sum(1))).abs().max() <= 2 * e
 
 
 def test_index_types_and_metrics_that_are_refused():
@@ -590,6 +627,31 @@ def test_captured_and_replayed():
             graph2.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(x, z) for x, z in zip(first, want)) and all(torch.equal(x, z) for x, z in zip(out2, want)), rep
+
+
+def test_few_f32_queries_captured_and_on_another_stream():
+    for metric in (learn.IP, learn.COS):
+        q, w, y, gl = case(20, 3000, 96, F32, F32, seed=18)
+
+        def step():
+            l, s = learn.softmax_loss(q, w, y, 8.0, metric)
+            return (l, s) + learn.softmax_loss_grad(q, w, y, s, gl, 8.0, metric)
+
+        st = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(st):
+            other = step()
+        st.synchronize()
+        assert all(torch.equal(x, z) for x, z in zip(other, step()))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            out = step()
+        for rep in range(3):
+            q2, w2, y2, gl2 = case(20, 3000, 96, F32, F32, seed=60 + rep)
+            q.copy_(q2), w.copy_(w2), y.copy_(y2), gl.copy_(gl2)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, z) for x, z in zip(out, step())), rep
 
 
 def test_learn_then_index_then_search():

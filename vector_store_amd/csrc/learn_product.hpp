@@ -15,9 +15,9 @@
 // The operands of the MFMA are swapped (B first): a lane then holds four consecutive COLUMNS of one output row, so row-wise softmax sums are
 // mostly in-lane and stores are 8 / 16 bytes wide.
 // Persistent over the output tiles: the ring runs on into the next tile while the epilogue works.
-// Bound by the matrix pipe where both sides are long: 4,096 x 131,072 x 768 in bf16, scores and softmax 844 us (977 TFLOP/s; 1,344 is what a plain
-// product of 8,192^3 reaches here), scores and probabilities 985, dq 866, dw 844; 300 f16 queries, whose dw is its writing, 400 TFLOP/s.  By the
-// rows' reading where queries are few: one bf16 query against 10^6 rows of 768 257 us (6.0 TB/s), 40 f32 queries against 60,000 66 us (2.8 TB/s).
+// Bound by the matrix pipe where both sides are long: 4,096 x 131,072 x 768 in bf16, scores and softmax 692 us alone (1,190 TFLOP/s; 1,344 is what a plain
+// product of 8,192^3 reaches here) and 844 in a step, where the clock is lower; scores and probabilities 985, dq 866, dw 844; 300 f16 queries, whose dw is its writing, 400 TFLOP/s.  By the
+// rows' reading where queries are few: one bf16 query against 10^6 rows of 768 257 us (6.0 TB/s), one f32 query against 300,000 210 us (4.4 TB/s).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
