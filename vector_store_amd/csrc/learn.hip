@@ -519,7 +519,8 @@ struct Layout {  // offsets into the caller's scratch
 struct Plan {
     Rows w;
     uint32_t n = 0, v = 0, d = 0, dp = 0;
-    bool cosine = false, raw = false, q_in_place = false, w_in_place = false, inv_own = false;
+    bool cosine = false, raw = false, q_in_place = false, w_in_place = false;
+    bool inv_own = false, inv_scores = false;  // the rows' inverse lengths are computed here; by the scores' product
     bool grad_q = false, grad_w = false;
     int kind = K_F16, gkind = K_F16;                    // operands of the scores; of the gradients' products
     uint32_t es = 2, ges = 2, bk = 64, gbk = 64;        // bytes per element and elements per step of both
@@ -590,6 +591,7 @@ static Plan plan(const vs_rows* rows, const vs_softmax* q, bool grad_q, bool gra
     p.q_in_place = p.raw && !(full && p.cosine) && d % line == 0 && q->stride % line == 0 && (uintptr_t)q->d_queries % 16 == 0;
     p.w_in_place = p.raw && !p.w.keys && d % line == 0 && p.w.ld % line == 0 && (uintptr_t)p.w.data % 16 == 0;
     p.inv_own = p.cosine && !(p.raw && p.w.inv);
+    p.inv_scores = full && p.inv_own;
     p.nq = !p.raw && (p.cosine || tq == VS_SCALAR_F32) ? 2 : 1;
     p.nw = !p.raw && (p.cosine || tw == VS_SCALAR_F32) ? 2 : 1;
     p.grad_q = grad_q;
@@ -705,7 +707,7 @@ struct Call {  // what the two calls share
         launched("queries");
     }
     void tables() const {  // once per call, before the pieces
-        if (p.raw && p.inv_own) {
+        if (p.raw && p.inv_own && !p.inv_scores) {
             hipLaunchKernelGGL(rows_inverse_norm_kernel, dim3((p.v + 3) / 4), dim3(256), 0, st, p.w.data, p.w.scalar, (uint64_t)p.w.ld, p.v, p.d,
                                wide_rows(p.w.data, p.w.scalar, p.w.ld), at<float>(p.o_inv));
             launched("norms");
@@ -769,7 +771,8 @@ struct Call {  // what the two calls share
         g.ksteps = (g.k + p.bk - 1) / p.bk;
         plane_pairs(g, p.nq, p.nw, true);
         g.row = at<float4>(p.o_row);
-        g.h = h() ? h() + first : nullptr;
+        g.norms = p.inv_scores ? at<float>(p.o_inv) + first : nullptr;
+        g.h = h() && !p.inv_scores ? h() + first : nullptr;
         g.wsc = p.raw || p.cosine ? nullptr : at<float>(p.o_wsc) + x;
         g.keys = p.w.keys ? p.w.keys + first : nullptr;
         g.col0 = first;

@@ -49,7 +49,8 @@ struct ProductArgs {
     uint32_t lo_first;           // the first pair's a is the probabilities' second plane, which is stored times 2^11
     // EPI_LOSS / EPI_PROB: z2 = acc * zf * wsc * h[col] (base-2 exponent units); per row (zf, lse2, pf 2^-lo, label as bits)
     const float4* row;
-    const float* h;              // nullptr: 1
+    const float* h;              // nullptr: 1 (or norms)
+    float* norms;                // f32: 1 / |row| of the columns is computed here, used as h and written
     const float* wsc;            // nullptr: 1
     const uint64_t* keys;        // nullptr, or per column: ~0 = not a member
     uint32_t col0;               // first column of this piece (labels are columns of the whole table, -1 = ignored)
@@ -452,6 +453,11 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
 #pragma unroll
                 for (int t = 1; t < SUMS; ++t) more[t][i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
             }
+        // f32 rows under a cosine bring their lengths with them: a column's elements lie in the four lanes of its number
+        const bool own = SOFTMAX && KIND == K_F32 && g.norms;
+        float ss[S::NT];
+#pragma unroll
+        for (int j = 0; j < S::NT; ++j) ss[j] = 0.f;
         for (uint32_t s = 0; s < steps; ++s) {
             // (a wave's loads arrive in order: what may still be on its way are the P pieces of the stages after this one)
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S::RING - 2) * P) : "memory");
@@ -472,6 +478,15 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
             // The next stage's loads go out one by one between the MFMAs of the step's first half: issued in a row they fill the queue of the
             // load unit (16 cycles each, 64 of them per CU), and every wave stands in front of its first MFMA until its own are through.
             frag fa[S::MT], fb[S::NT];
+            const auto square = [&]() {
+                if constexpr (SOFTMAX && KIND == K_F32) {
+                    if (!own) return;
+#pragma unroll
+                    for (int j = 0; j < S::NT; ++j)
+#pragma unroll
+                        for (int t = 0; t < 4; ++t) ss[j] = fmaf(fb[j][t], fb[j][t], ss[j]);
+                }
+            };
             read_fragments<S::TM, S::MT, A_ACROSS, KIND, 0>(sa, lds0 + stage, wm * S::MT * 16u, lane, aa, fa);
             read_fragments<S::TN, S::NT, B_ACROSS, KIND, 0>(sb, lds0 + stage + S::A_BYTES, wn * S::NT * 16u, lane, ab, fb);
 #pragma unroll
@@ -495,6 +510,7 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                         f32x4& c = t % SUMS ? more[t % SUMS][i][j] : acc[i][j];
                         c = H::mma(fb[j], fa[i], c, t);
                     }
+            square();
             read_fragments<S::TM, S::MT, A_ACROSS, KIND, 1>(sa, lds0 + stage, wm * S::MT * 16u, lane, aa, fa);
             read_fragments<S::TN, S::NT, B_ACROSS, KIND, 1>(sb, lds0 + stage + S::A_BYTES, wn * S::NT * 16u, lane, ab, fb);
 #pragma unroll
@@ -506,6 +522,7 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                         f32x4& c = t % SUMS ? more[t % SUMS][i][j] : acc[i][j];
                         c = H::mma(fb[j], fa[i], c, t);
                     }
+            square();
             advance();
             next_at = stage;
             stage = stage + S::STAGE < S::RING * S::STAGE ? stage + S::STAGE : 0u;
@@ -527,6 +544,19 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
             const bool plain = !g.keys && c0 + S::NT * 16u <= g.n;
             f32x4 h[S::NT];
             uint32_t live[S::NT];  // bit r: column j, r exists
+            const bool scaled = own || g.h;
+            if (own) {
+#pragma unroll
+                for (int j = 0; j < S::NT; ++j) {
+                    ss[j] += __shfl_xor(ss[j], 16);
+                    ss[j] += __shfl_xor(ss[j], 32);
+                    const float inv = ss[j] > 0.f ? 1.f / sqrtf(ss[j]) : 0.f;
+                    const uint32_t c = c0 + j * 16u + lane;
+                    if (tm == 0 && wm == 0 && lane < 16u && c < g.n) g.norms[c] = inv;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) h[j][r] = __shfl(inv, (lane >> 4) * 4u + r);
+                }
+            }
             if (!plain) {
 #pragma unroll
                 for (int j = 0; j < S::NT; ++j) {
@@ -536,16 +566,16 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
                         const uint32_t c = cl + j * 16u + r;
                         const bool in = c < g.n && !(g.keys && g.keys[c] == ~0ull);
                         live[j] |= in ? 1u << r : 0u;
-                        h[j][r] = in ? (g.h ? g.h[c] : 1.f) : 0.f;
+                        h[j][r] = !in ? 0.f : own ? h[j][r] : g.h ? g.h[c] : 1.f;
                     }
                 }
-            } else if (g.h) {
+            } else if (g.h) {  // (own: they are there)
 #pragma unroll
                 for (int j = 0; j < S::NT; ++j)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) h[j][r] = g.h[cl + j * 16u + r];
             }
-            if (g.h) {
+            if (scaled) {
 #pragma unroll
                 for (int i = 0; i < S::MT; ++i)
 #pragma unroll
@@ -706,7 +736,7 @@ __global__ __launch_bounds__(S::NW * 64) void product_kernel(ProductArgs g) {
 #pragma unroll
                         for (int j = 0; j < S::NT; ++j)
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) x[j][r] = g.h ? v[j][r] * rf.z * h[j][r] : v[j][r] * rf.z;  // (v is 0 where h is)
+                            for (int r = 0; r < 4; ++r) x[j][r] = scaled ? v[j][r] * rf.z * h[j][r] : v[j][r] * rf.z;  // (v is 0 where h is)
                         store_lines<SCRATCH / 128>(scratch, x, reinterpret_cast<float*>(g.prob), g.prob_ld, row0 - (lane & 15u) + i * 16u, g.m, c0, g.prob_ld, lane);
                         continue;
                     }
