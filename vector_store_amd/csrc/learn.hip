@@ -540,8 +540,9 @@ constexpr size_t kPieceBytes = 640ull << 20;
 constexpr size_t kSplitBytes = 128ull << 20;    // f32 slices of dq
 // Up to this many f32 queries of f32 rows are multiplied as f32: the rows are then read once where the split re-lays them first, about four times
 // the traffic, and the f32 MFMA's sixteenth of the f16 rate does not show before more queries than that.  60,000 x 768, as f32 / split, loss and
-// gradients: 40 queries 67 + 217 / 159 + 304 us, 72: 125 + 350 / 165 + 301, 128: 120 + 352 / 164 + 306; by cosine 64: 96 + 275 / 132 + 342, 72:
-// 144 + 392 / 137 + 309.  (One limit for the loss and its gradient: a probability near 1 is only as good as the two agree on its score.)
+// gradients: 40 queries 67 + 217 / 159 + 304 us, 72: 125 + 350 / 165 + 301, 128: 120 + 352 / 164 + 306; by cosine 64: 72 + 253 / 132 +
+// 342, 72 (with the lengths in a pass of their own): 144 + 392 / 137 + 309.  (One limit for the loss and its gradient: a probability near 1 is
+// only as good as the two agree on its score.)
 constexpr uint32_t kFullQueries = 64;
 // Up to this many bf16 queries of bf16 rows the probabilities are kept as two bf16, times all factors, instead of one f16: the gradients' products
 // then use rows and queries as they are -- twice the products, but the rows need not be laid out in f16 first.  Gradients of 64 x
